@@ -21,6 +21,13 @@ _c_f32 = ctypes.c_float
 _c_size = ctypes.c_size_t
 _p = ctypes.c_void_p
 
+class RotaryPart(ctypes.Structure):
+    """mi355_dsa_rotary_part: one tensor of a rotary call."""
+    _fields_ = [("out", _p), ("x", _p), ("out_tok_stride", _c_i64), ("out_head_stride", _c_i64),
+                ("x_tok_stride", _c_i64), ("x_head_stride", _c_i64), ("n_head", _c_int),
+                ("dim", _c_int), ("offset", _c_int), ("dtype", _c_int), ("interleaved", _c_int)]
+
+
 # name -> (restype, argtypes); mirrors include/mi355_dsa.h
 SIGNATURES = {
     "mi355_dsa_last_error": (ctypes.c_char_p, []),
@@ -34,6 +41,16 @@ SIGNATURES = {
                                             _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
                                             _c_i64, _c_i64, _c_i64, _p, _p, _c_int, _c_int,
                                             _c_f32, _c_int, _p]),
+    "mi355_dsa_rotary": (_c_int, [_p, _c_int, _p, _c_int, _c_i64, _p, _c_i64, _c_int, _p]),
+    "mi355_dsa_rope_concat_and_cache_mla": (_c_int, [
+        _p, _c_int, _c_i64, _p, _c_i64, _p, _c_i64, _c_int, _c_i64, _p, _c_int, _p, _c_int, _p,
+        _c_i64, _c_int, _p, _p]),
+    "mi355_dsa_gather_latent_cache": (_c_int, [_p, _c_i64, _c_int, _c_i64, _p, _c_int, _c_int,
+                                               _c_i64, _c_int, _p, _c_int, _p, _p, _c_int, _p]),
+    "mi355_dsa_mla_tree_workspace_size": (_c_size, [_c_i64, _c_int]),
+    "mi355_dsa_mla_tree_attention": (_c_int, [_p, _p, _p, _c_i64, _c_int, _p, _c_int, _c_i64,
+                                              _c_int, _p, _c_int, _p, _p, _c_int, _p, _c_f32, _p,
+                                              _c_size, _p]),
     "mi355_dsa_indexer_shard_merge": (_c_int, [_p, _c_i64, _c_i64, _p, _c_int, _c_int, _c_int,
                                                _p, _c_int, _p]),
     "mi355_dsa_head_proj": (_c_int, [_p, _c_i64, _c_i64, _p, _c_i64, _c_i64, _p, _c_int, _c_int,

@@ -73,29 +73,12 @@ __device__ __forceinline__ void k_store_fp8_block(
   k_fp8_row_store(raw, store ? kv + row * (int64_t)kIdxkFp8RowBytes : nullptr, sub);
 }
 
-// MLA latent rows.  One wave per token: lane l holds latent dims 8l .. 8l+7
-// (16-lane group = one 128-dim fp8 tile), lanes 0..7 also carry RoPE dims
-// 8l .. 8l+7.  T16: uint16_t bit pattern of fp16 (BF16 = false) or bf16.
-// fp8_ds_mla row (656 B): [0,512) e4m3, [512,528) 4 fp32 tile scales,
-// [528,656) RoPE as the input's 16-bit values.  fp16 ("auto") row: 576 halves.
-template <bool FP8, bool BF16, typename SlotT>
-__device__ __forceinline__ void concat_cache_mla_block(
-    const uint8_t* __restrict__ kv_c, int64_t kv_c_stride, const uint8_t* __restrict__ k_pe,
-    int64_t k_pe_stride, const SlotT* __restrict__ slot, uint8_t* __restrict__ kv,
-    int64_t n_tok, int64_t n_rows, int bx) {
-  const int lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)bx * 4 + (threadIdx.x >> 6);
-  if (t >= n_tok) return;  // wave-uniform
-  // the token's data is loaded with its slot, before the slot is checked:
-  // one memory round trip instead of two (lanes 8.. re-read a RoPE piece
-  // they do not store)
-  const int64_t row = (int64_t)slot[t];
-  const u32x4 raw = *reinterpret_cast<const u32x4*>(kv_c + t * kv_c_stride + 16 * lane);
-  const u32x4 rope = *reinterpret_cast<const u32x4*>(k_pe + t * k_pe_stride + 16 * (lane & 7));
-  asm volatile("" ::"v"(raw), "v"(rope));  // keeps the loads ahead of the check
-  if (row < 0 || row >= n_rows) return;  // wave-uniform
+// The row at rp of a token whose latent dims 8 l .. 8 l + 7 lane l of a wave
+// holds in raw and whose RoPE dims 8 l .. 8 l + 7 lanes 0..7 hold in rope.
+template <bool FP8, bool BF16>
+__device__ __forceinline__ void latent_row_store(const u32x4 raw, const u32x4 rope, uint8_t* rp,
+                                                 int lane) {
   if constexpr (!FP8) {
-    uint8_t* rp = kv + row * (int64_t)(kLatentDim * 2);
     *reinterpret_cast<u32x4*>(rp + 16 * lane) = raw;
     if (lane < 8) *reinterpret_cast<u32x4*>(rp + 2 * kValueDim + 16 * lane) = rope;
     return;
@@ -119,11 +102,35 @@ __device__ __forceinline__ void concat_cache_mla_block(
     amax = max16(amax);  // the 16 lanes of this 128-dim tile
     const float scale = fmaxf(amax / 448.0f, FLT_MIN);
     const u32x2 q = e4m3_quant8(v, amax, scale);
-    uint8_t* rp = kv + row * (int64_t)kDsmlaRowBytes;
     *reinterpret_cast<u32x2*>(rp + 8 * lane) = q;
     if ((lane & 15) == 0) *reinterpret_cast<float*>(rp + kValueDim + 4 * (lane >> 4)) = scale;
     if (lane < 8) *reinterpret_cast<u32x4*>(rp + kValueDim + 16 + 16 * lane) = rope;
   }
+}
+
+// MLA latent rows.  One wave per token: lane l holds latent dims 8l .. 8l+7
+// (16-lane group = one 128-dim fp8 tile), lanes 0..7 also carry RoPE dims
+// 8l .. 8l+7.  T16: uint16_t bit pattern of fp16 (BF16 = false) or bf16.
+// fp8_ds_mla row (656 B): [0,512) e4m3, [512,528) 4 fp32 tile scales,
+// [528,656) RoPE as the input's 16-bit values.  fp16 ("auto") row: 576 halves.
+template <bool FP8, bool BF16, typename SlotT>
+__device__ __forceinline__ void concat_cache_mla_block(
+    const uint8_t* __restrict__ kv_c, int64_t kv_c_stride, const uint8_t* __restrict__ k_pe,
+    int64_t k_pe_stride, const SlotT* __restrict__ slot, uint8_t* __restrict__ kv,
+    int64_t n_tok, int64_t n_rows, int bx) {
+  const int lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)bx * 4 + (threadIdx.x >> 6);
+  if (t >= n_tok) return;  // wave-uniform
+  // the token's data is loaded with its slot, before the slot is checked:
+  // one memory round trip instead of two (lanes 8.. re-read a RoPE piece
+  // they do not store)
+  const int64_t row = (int64_t)slot[t];
+  const u32x4 raw = *reinterpret_cast<const u32x4*>(kv_c + t * kv_c_stride + 16 * lane);
+  const u32x4 rope = *reinterpret_cast<const u32x4*>(k_pe + t * k_pe_stride + 16 * (lane & 7));
+  asm volatile("" ::"v"(raw), "v"(rope));  // keeps the loads ahead of the check
+  if (row < 0 || row >= n_rows) return;  // wave-uniform
+  latent_row_store<FP8, BF16>(raw, rope, kv + row * (int64_t)(FP8 ? kDsmlaRowBytes : kLatentDim * 2),
+                              lane);
 }
 
 }  // namespace mi355dsa

@@ -1,0 +1,138 @@
+"""Rotary positions on the gfx950 kernel (csrc/rope.hip, C ABI mi355_dsa_rotary):
+the step in front of the layer's attention, which takes q, k_pe and the indexer's
+q and k rotated.
+
+A table row holds the cosines of a position's rot_dim / 2 pairs and then the
+sines, in fp32 (`rotary_table`, built in fp64).  In the interleaved layout pair i
+of the rotated part is (2 i, 2 i + 1), as MLA's rope dims are kept; in the half
+layout (i, i + rot_dim / 2), as the indexer's are.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+from .ops import _check, _stream
+
+_DTYPE_CODE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+MAX_TENSORS = 4  # of one launch
+
+
+def rotary_table(rot_dim: int, max_positions: int, base: float = 10000.0,
+                 scaling: dict | None = None, device="cuda") -> torch.Tensor:
+    """cos | sin fp32 [max_positions, rot_dim] of position * base^(-2 i / rot_dim).
+
+    scaling, for contexts longer than the model was trained on:
+      {"type": "linear", "factor": f}: positions divided by f;
+      {"type": "ntk", "factor": f}: base times f^(rot_dim / (rot_dim - 2));
+      {"type": "yarn", "factor": f, "original_max_positions": n, and optionally
+       "beta_fast" (32), "beta_slow" (1), "mscale" (1), "mscale_all_dim" (0)}: the
+      method of Peng et al. 2023 -- frequencies of more than beta_fast turns over
+      the n positions stay, those below beta_slow are divided by f, a linear ramp
+      over the dims between; cos and sin times m(mscale) / m(mscale_all_dim) with
+      m(s) = 0.1 s ln f + 1."""
+    _check(rot_dim > 0 and rot_dim % 2 == 0, "rotary_table: rot_dim must be even and > 0")
+    _check(max_positions >= 0, "rotary_table: max_positions must be >= 0")
+    _check(base > 0, "rotary_table: base must be > 0")
+    half = rot_dim // 2
+    exponent = torch.arange(half, dtype=torch.float64) * 2 / rot_dim
+    freq, mag = float(base) ** -exponent, 1.0
+    if scaling is not None:
+        kind, f = scaling.get("type"), float(scaling.get("factor", 1.0))
+        _check(kind in ("linear", "ntk", "yarn"), f"rotary_table: unknown scaling {kind!r}")
+        _check(f >= 1.0, "rotary_table: factor must be >= 1")
+        if kind == "linear":
+            freq = freq / f
+        elif kind == "ntk":
+            _check(rot_dim > 2, "rotary_table: ntk scaling needs rot_dim > 2")
+            freq = (base * f ** (rot_dim / (rot_dim - 2))) ** -exponent
+        else:
+            n = scaling.get("original_max_positions", 0)
+            _check(n > 0, "rotary_table: yarn needs original_max_positions")
+            _check(base > 1, "rotary_table: yarn needs base > 1")
+
+            def dim_of(turns):
+                return rot_dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+            lo = max(math.floor(dim_of(scaling.get("beta_fast", 32.0))), 0)
+            hi = min(math.ceil(dim_of(scaling.get("beta_slow", 1.0))), rot_dim - 1)
+            ramp = ((torch.arange(half, dtype=torch.float64) - lo)
+                    / (hi - lo if hi > lo else 0.001)).clamp(0, 1)
+            freq = freq / f * ramp + freq * (1 - ramp)
+
+            def m(s):
+                return 0.1 * s * math.log(f) + 1.0
+
+            mag = m(scaling.get("mscale", 1.0)) / m(scaling.get("mscale_all_dim", 0.0))
+    angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] \
+        * freq.to(device)
+    return (torch.cat([angle.cos(), angle.sin()], dim=1) * mag).float()
+
+
+def _strides3(x: torch.Tensor):
+    """(token, head) strides and head count of [T, H, D] or [T, D]."""
+    if x.dim() == 2:
+        return x.stride(0), x.shape[1], 1
+    return x.stride(0), x.stride(1), x.shape[1]
+
+
+def _part(x: torch.Tensor, out: torch.Tensor, offset: int, interleaved: bool, rot_dim: int,
+          n_tok: int) -> _lib.RotaryPart:
+    _check(x.dim() in (2, 3) and x.shape[0] == n_tok,
+           "apply_rotary: tensors are [tokens, heads, dim] or [tokens, dim]")
+    _check(x.dtype in _DTYPE_CODE, "apply_rotary: fp16, bf16 or fp32 tensors")
+    _check(out.shape == x.shape and out.dtype == x.dtype and out.device == x.device,
+           "apply_rotary: out must have x's shape, type and device")
+    _check((x.stride(-1) == 1 and out.stride(-1) == 1) or x.shape[-1] <= 1,
+           "apply_rotary: the last dim must be contiguous")
+    xt, xh, heads = _strides3(x)
+    ot, oh, _ = _strides3(out)
+    return _lib.RotaryPart(out.data_ptr(), x.data_ptr(), ot, oh, xt, xh, heads, x.shape[-1],
+                           int(offset), _DTYPE_CODE[x.dtype], int(bool(interleaved)))
+
+
+def _table_args(positions: torch.Tensor, table: torch.Tensor):
+    _check(positions.is_cuda and table.is_cuda and positions.device == table.device,
+           "positions and table must be on the GPU")
+    _check(positions.dim() == 1 and positions.dtype in (torch.int32, torch.int64),
+           "positions must be int32 or int64 [tokens]")
+    _check(table.dtype == torch.float32 and table.dim() == 2 and table.is_contiguous(),
+           "table must be contiguous fp32 [positions, rot_dim]")
+    return positions if positions.is_contiguous() else positions.contiguous()
+
+
+def apply_rotary(xs, positions: torch.Tensor, table: torch.Tensor, offsets=0, interleaved=True,
+                 outs=None):
+    """Rotates dims [offset, offset + rot_dim) of every head of x [T, H, D] or
+    [T, D] (fp16, bf16 or fp32, last dim contiguous) by the table row of the
+    token's position; other dims are copied.  xs is a tensor, or a list of up to
+    4 (a step's q, k_pe and the indexer's q and k) with one offset and layout
+    each, rotated in one launch.  outs: tensors to write, xs themselves for in
+    place (only the rotated part moves then); otherwise they must not overlap
+    xs.  A token whose position is outside the table (a padded one, -1) is not
+    rotated.  Returns what was written, a tensor or a list as xs."""
+    single = isinstance(xs, torch.Tensor)
+    xl = [xs] if single else list(xs)
+    _check(1 <= len(xl) <= MAX_TENSORS, f"apply_rotary: 1 to {MAX_TENSORS} tensors")
+    n = len(xl)
+    offs = [offsets] * n if isinstance(offsets, int) else list(offsets)
+    inter = [interleaved] * n if isinstance(interleaved, bool) else list(interleaved)
+    if outs is None:
+        ol = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xl]
+    else:
+        ol = [outs] if isinstance(outs, torch.Tensor) else list(outs)
+    _check(len(offs) == n and len(inter) == n and len(ol) == n,
+           "apply_rotary: one offset, layout and out for each tensor")
+    positions = _table_args(positions, table)
+    T, rot = positions.shape[0], table.shape[1]
+    dev = table.device
+    _check(all(x.device == dev for x in xl), "all tensors must be on one GPU")
+    parts = (_lib.RotaryPart * n)(*[_part(x, o, a, i, rot, T)
+                                    for x, o, a, i in zip(xl, ol, offs, inter)])
+    with torch.cuda.device(dev):
+        _lib.call("mi355_dsa_rotary", parts, n, positions.data_ptr(),
+                  int(positions.dtype == torch.int64), T, table.data_ptr(), table.shape[0], rot,
+                  _stream(table))
+    return ol[0] if single else ol

@@ -91,6 +91,82 @@ int mi355_dsa_concat_and_cache_mla(void* kv_cache, int kv_fp8, int64_t n_rows,
                                    void* stream);
 
 /*
+ * Rotary positions.  cos_sin fp32 [max_pos, rot_dim]: the cosines of a
+ * position's rot_dim / 2 pairs, then the sines.  Every part is a tensor
+ * [n_tok, n_head, dim] whose dims [offset, offset + rot_dim) of a head are
+ * rotated, pair i being (2 i, 2 i + 1) (interleaved = 1) or (i, i + rot_dim / 2)
+ * (interleaved = 0) of them: (a, b) -> (a c - b s, b c + a s) in fp32, rounded
+ * once to the part's dtype (0 fp16, 1 bf16, 2 fp32).  The other dims are
+ * copied; with out == x (and the same strides) they are not touched, otherwise
+ * out must not overlap x.  Strides in elements, the last dim dense.  A token
+ * whose position is outside [0, max_pos) is not rotated.  positions: int64
+ * (pos_i64 = 1) or int32 [n_tok].  Up to 4 parts share one launch.
+ * It has no counterpart in the reference, which takes rotated tensors.
+ */
+typedef struct {
+  void* out;
+  const void* x;
+  int64_t out_tok_stride, out_head_stride, x_tok_stride, x_head_stride;
+  int n_head, dim, offset, dtype, interleaved;
+} mi355_dsa_rotary_part;
+int mi355_dsa_rotary(const mi355_dsa_rotary_part* parts, int n_parts, const void* positions,
+                     int pos_i64, int64_t n_tok, const float* cos_sin, int64_t max_pos,
+                     int rot_dim, void* stream);
+
+/*
+ * mi355_dsa_concat_and_cache_mla of k_pe rows that are not rotated yet, and
+ * (q not null) mi355_dsa_rotary of q, in one launch: equal, bit for bit, to
+ * mi355_dsa_rotary of k_pe and q (rot_dim 64) followed by the writer.  k_pe
+ * itself is not changed.  q has the type of kv_c.
+ */
+int mi355_dsa_rope_concat_and_cache_mla(
+    void* kv_cache, int kv_fp8, int64_t n_rows, const void* kv_c, int64_t kv_c_stride,
+    const void* k_pe, int64_t k_pe_stride, int in_bf16, int64_t n_tok, const void* slot_mapping,
+    int slot_i64, const void* positions, int pos_i64, const float* cos_sin, int64_t max_pos,
+    int interleaved, const mi355_dsa_rotary_part* q, void* stream);
+
+/*
+ * Latent rows read back: out row t (of `total`; 576 values of out_dtype 0 fp16,
+ * 1 bf16, 2 fp32; row stride out_stride elements) <- position
+ * starts[r] + t - cu_seqlens[r] of the request r with cu_seqlens[r] <= t <
+ * cu_seqlens[r + 1] (int32 device arrays [n_req + 1], [n_req]; starts null:
+ * 0).  fp8 rows give RN(e4m3 * scale), the product in fp32; their 64 16-bit
+ * values are fp16 (pe_bf16 = 0) or bf16.  A position whose row does not resolve
+ * (negative, past the block table, page outside the cache) reads as zeros; out
+ * rows of no request are left as they were.  The context gather in front of
+ * the reference's run_prefill_context_chunk (sm70_triton.py:246-266).
+ */
+int mi355_dsa_gather_latent_cache(void* out, int64_t out_stride, int out_dtype, int64_t total,
+                                  const void* kv_cache, int kv_fp8, int pe_bf16, int64_t n_rows,
+                                  int page_size, const int32_t* block_table, int max_blocks,
+                                  const int32_t* cu_seqlens, const int32_t* starts, int n_req,
+                                  void* stream);
+
+/*
+ * Attention of drafted token trees over the paged latent cache.  Request r owns
+ * the token rows [cu_seqlens_q[r], cu_seqlens_q[r + 1]) of q fp16
+ * [n_tok, n_head, 576], n of them; token j of it stands at cache position
+ * seq_lens[r] - n + j.  It sees the positions below seq_lens[r] - n, and the
+ * drafted token i (i < 64) of its request where bit i of its tree_mask (int64
+ * [n_tok]) is set (its own bit too decides).  A position whose row does not
+ * resolve is not seen.  o fp16 [n_tok, n_head, 512] (16-byte aligned), lse fp32
+ * [n_tok, n_head] (natural log); a row that sees nothing gets o = 0,
+ * lse = -inf.  Rows of no request are left as they were.  kv_fp8 = 0: rows of
+ * 576 fp16; 1: fp8_ds_mla rows, which count as the fp16 values that
+ * mi355_dsa_gather_latent_cache gives.  Scores and sums are fp32, P is rounded
+ * to fp16 for the product with V.  A row that sees a drafted token whose cache
+ * row holds an infinity or NaN is NaN; a row that does not is not touched by it.
+ * The workspace (16-byte aligned) carries nothing between calls.
+ */
+size_t mi355_dsa_mla_tree_workspace_size(int64_t n_tok, int n_head);
+int mi355_dsa_mla_tree_attention(void* o, float* lse, const void* q, int64_t n_tok, int n_head,
+                                 const void* kv_cache, int kv_fp8, int64_t n_kv_rows,
+                                 int page_size, const int32_t* block_table, int max_blocks,
+                                 const int32_t* seq_lens, const int32_t* cu_seqlens_q, int n_req,
+                                 const int64_t* tree_mask, float scale, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
+/*
  * Dense MLA decode over a paged fp16 latent cache: for each token b and head
  * h, attention of q[b,h,:576] * scale over the cache rows of positions
  * [0, seq_lens[b]) (row(p) = bt[b, p/page]*page + p%page; a position whose
