@@ -10,13 +10,11 @@ gather_latent_cache reads rows back as values.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
-from . import _lib, rope
+from . import rope
 from ._sm70_ops import _op
-from .ops import DSMLA_ROW_BYTES, _check, _contig, _stream
+from .ops import DSMLA_ROW_BYTES, _check, _contig, _launch
 
 
 def concat_and_cache_mla(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache: torch.Tensor,
@@ -80,11 +78,8 @@ def rope_concat_and_cache_mla(positions: torch.Tensor, table: torch.Tensor, kv_c
     _check(kv_c.size(0) >= T and k_pe.size(0) >= T, "fewer kv_c / k_pe rows than slots")
     part = None
     if q is not None:
-        _check(q.dtype == kv_c.dtype and q.device == kv_c.device,
-               "q must have kv_c's type and device")
-        if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        part = rope._part(q, q_out, q_offset, interleaved, 64, T)
+        _check(q.dtype == kv_c.dtype, "q must have kv_c's type")
+        part, q_out = rope._part(q, q_out, q_offset, interleaved, T, kv_c.device)
     else:
         _check(q_out is None, "q_out without q")
 
@@ -94,14 +89,11 @@ def rope_concat_and_cache_mla(positions: torch.Tensor, table: torch.Tensor, kv_c
         return x if ok else x.contiguous()
 
     kv_c, k_pe, slot_mapping = rows16(kv_c), rows16(k_pe), _contig(slot_mapping)
-    with torch.cuda.device(kv_c.device):
-        _lib.call("mi355_dsa_rope_concat_and_cache_mla", kv_cache.data_ptr(), int(fp8), n_rows,
-                  kv_c.data_ptr(), kv_c.stride(0), k_pe.data_ptr(), k_pe.stride(0),
-                  int(kv_c.dtype == torch.bfloat16), T, slot_mapping.data_ptr(),
-                  int(slot_mapping.dtype == torch.int64), positions.data_ptr(),
-                  int(positions.dtype == torch.int64), table.data_ptr(), table.shape[0],
-                  int(bool(interleaved)), None if part is None else ctypes.byref(part),
-                  _stream(kv_c))
+    _launch("mi355_dsa_rope_concat_and_cache_mla", kv_c.device, kv_cache.data_ptr(), fp8, n_rows,
+            kv_c.data_ptr(), kv_c.stride(0), k_pe.data_ptr(), k_pe.stride(0),
+            kv_c.dtype == torch.bfloat16, T, slot_mapping.data_ptr(),
+            slot_mapping.dtype == torch.int64, positions.data_ptr(),
+            positions.dtype == torch.int64, table.data_ptr(), table.shape[0], interleaved, part)
     return q_out
 
 
@@ -146,10 +138,8 @@ def gather_latent_cache(kv_cache: torch.Tensor, block_table: torch.Tensor,
                "out rows must be contiguous and 16-byte aligned")
     block_table, cu_seqlens = _contig(block_table), _contig(cu_seqlens)
     starts = _contig(starts) if starts is not None else None
-    with torch.cuda.device(kv_cache.device):
-        _lib.call("mi355_dsa_gather_latent_cache", out.data_ptr(), out.stride(0),
-                  rope._DTYPE_CODE[dtype], total, kv_cache.data_ptr(), int(fp8),
-                  int(pe_dtype == torch.bfloat16), n_rows, kv_cache.size(-2),
-                  block_table.data_ptr(), block_table.size(1), cu_seqlens.data_ptr(),
-                  starts.data_ptr() if starts is not None else None, R, _stream(kv_cache))
+    _launch("mi355_dsa_gather_latent_cache", kv_cache.device, out.data_ptr(), out.stride(0),
+            rope._DTYPE_CODE[dtype], total, kv_cache.data_ptr(), fp8, pe_dtype == torch.bfloat16,
+            n_rows, kv_cache.size(-2), block_table.data_ptr(), block_table.size(1),
+            cu_seqlens.data_ptr(), starts.data_ptr() if starts is not None else None, R)
     return out

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import torch  # noqa: F401  (must precede the CDLL load, see module doc)
 
@@ -26,6 +27,11 @@ class RotaryPart(ctypes.Structure):
     _fields_ = [("out", _p), ("x", _p), ("out_tok_stride", _c_i64), ("out_head_stride", _c_i64),
                 ("x_tok_stride", _c_i64), ("x_head_stride", _c_i64), ("n_head", _c_int),
                 ("dim", _c_int), ("offset", _c_int), ("dtype", _c_int), ("interleaved", _c_int)]
+
+
+# the same structure packed at once: setting its fields one by one is most of a short call
+ROTARY_PART = struct.Struct("=QQqqqqiiiii4x")
+assert ROTARY_PART.size == ctypes.sizeof(RotaryPart)
 
 
 # name -> (restype, argtypes); mirrors include/mi355_dsa.h

@@ -13,7 +13,7 @@ import torch
 
 from . import _lib
 from ._cache_ops import _latent_rows
-from .ops import _check, _contig, _stream
+from .ops import _check, _contig, _launch
 
 MAX_DRAFT = 64  # drafted tokens of a request that a mask can name
 
@@ -79,10 +79,8 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
     cu_seqlens_q, tree_mask = _contig(cu_seqlens_q), _contig(tree_mask)
     need = _lib.lib().mi355_dsa_mla_tree_workspace_size(T, H)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    with torch.cuda.device(q.device):
-        _lib.call("mi355_dsa_mla_tree_attention", out.data_ptr(), lse.data_ptr(), q.data_ptr(), T,
-                  H, kv_cache.data_ptr(), int(fp8), n_rows, kv_cache.size(-2),
-                  block_table.data_ptr(), block_table.size(1), seq_lens.data_ptr(),
-                  cu_seqlens_q.data_ptr(), R, tree_mask.data_ptr(), float(scale), ws.data_ptr(),
-                  need, _stream(q))
+    _launch("mi355_dsa_mla_tree_attention", q.device, out.data_ptr(), lse.data_ptr(), q.data_ptr(),
+            T, H, kv_cache.data_ptr(), fp8, n_rows, kv_cache.size(-2), block_table.data_ptr(),
+            block_table.size(1), seq_lens.data_ptr(), cu_seqlens_q.data_ptr(), R,
+            tree_mask.data_ptr(), scale, ws.data_ptr(), need)
     return out, lse

@@ -14,7 +14,7 @@ import math
 import torch
 
 from . import _lib
-from .ops import _check, _stream
+from .ops import _check, _launch
 
 _DTYPE_CODE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 MAX_TENSORS = 4  # of one launch
@@ -71,30 +71,30 @@ def rotary_table(rot_dim: int, max_positions: int, base: float = 10000.0,
     return (torch.cat([angle.cos(), angle.sin()], dim=1) * mag).float()
 
 
-def _strides3(x: torch.Tensor):
-    """(token, head) strides and head count of [T, H, D] or [T, D]."""
-    if x.dim() == 2:
-        return x.stride(0), x.shape[1], 1
-    return x.stride(0), x.stride(1), x.shape[1]
-
-
-def _part(x: torch.Tensor, out: torch.Tensor, offset: int, interleaved: bool, rot_dim: int,
-          n_tok: int) -> _lib.RotaryPart:
-    _check(x.dim() in (2, 3) and x.shape[0] == n_tok,
+def _part(x: torch.Tensor, out: torch.Tensor | None, offset: int, interleaved: bool, n_tok: int,
+          dev: torch.device):
+    """(packed mi355_dsa_rotary_part, out) of x [T, H, D] or [T, D]; out allocated if None."""
+    shape, code = x.shape, _DTYPE_CODE.get(x.dtype)
+    _check(len(shape) in (2, 3) and shape[0] == n_tok,
            "apply_rotary: tensors are [tokens, heads, dim] or [tokens, dim]")
-    _check(x.dtype in _DTYPE_CODE, "apply_rotary: fp16, bf16 or fp32 tensors")
-    _check(out.shape == x.shape and out.dtype == x.dtype and out.device == x.device,
-           "apply_rotary: out must have x's shape, type and device")
-    _check((x.stride(-1) == 1 and out.stride(-1) == 1) or x.shape[-1] <= 1,
+    _check(code is not None, "apply_rotary: fp16, bf16 or fp32 tensors")
+    _check(x.device == dev, "all tensors must be on one GPU")
+    xs = x.stride()
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    elif out is not x:
+        _check(out.shape == shape and out.dtype == x.dtype and out.device == dev,
+               "apply_rotary: out must have x's shape, type and device")
+    os = out.stride()
+    _check((xs[-1] == 1 and os[-1] == 1) or shape[-1] <= 1,
            "apply_rotary: the last dim must be contiguous")
-    xt, xh, heads = _strides3(x)
-    ot, oh, _ = _strides3(out)
-    return _lib.RotaryPart(out.data_ptr(), x.data_ptr(), ot, oh, xt, xh, heads, x.shape[-1],
-                           int(offset), _DTYPE_CODE[x.dtype], int(bool(interleaved)))
+    heads = shape[1] if len(xs) == 3 else 1
+    return _lib.ROTARY_PART.pack(out.data_ptr(), x.data_ptr(), os[0], os[-2], xs[0], xs[-2], heads,
+                                 shape[-1], offset, code, interleaved), out
 
 
 def _table_args(positions: torch.Tensor, table: torch.Tensor):
-    _check(positions.is_cuda and table.is_cuda and positions.device == table.device,
+    _check(table.is_cuda and positions.device == table.device,
            "positions and table must be on the GPU")
     _check(positions.dim() == 1 and positions.dtype in (torch.int32, torch.int64),
            "positions must be int32 or int64 [tokens]")
@@ -114,25 +114,17 @@ def apply_rotary(xs, positions: torch.Tensor, table: torch.Tensor, offsets=0, in
     xs.  A token whose position is outside the table (a padded one, -1) is not
     rotated.  Returns what was written, a tensor or a list as xs."""
     single = isinstance(xs, torch.Tensor)
-    xl = [xs] if single else list(xs)
-    _check(1 <= len(xl) <= MAX_TENSORS, f"apply_rotary: 1 to {MAX_TENSORS} tensors")
+    xl = [xs] if single else xs
     n = len(xl)
-    offs = [offsets] * n if isinstance(offsets, int) else list(offsets)
-    inter = [interleaved] * n if isinstance(interleaved, bool) else list(interleaved)
-    if outs is None:
-        ol = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xl]
-    else:
-        ol = [outs] if isinstance(outs, torch.Tensor) else list(outs)
+    _check(1 <= n <= MAX_TENSORS, f"apply_rotary: 1 to {MAX_TENSORS} tensors")
+    offs = [offsets] * n if isinstance(offsets, int) else offsets
+    inter = [interleaved] * n if isinstance(interleaved, bool) else interleaved
+    ol = [None] * n if outs is None else [outs] if isinstance(outs, torch.Tensor) else outs
     _check(len(offs) == n and len(inter) == n and len(ol) == n,
            "apply_rotary: one offset, layout and out for each tensor")
     positions = _table_args(positions, table)
-    T, rot = positions.shape[0], table.shape[1]
-    dev = table.device
-    _check(all(x.device == dev for x in xl), "all tensors must be on one GPU")
-    parts = (_lib.RotaryPart * n)(*[_part(x, o, a, i, rot, T)
-                                    for x, o, a, i in zip(xl, ol, offs, inter)])
-    with torch.cuda.device(dev):
-        _lib.call("mi355_dsa_rotary", parts, n, positions.data_ptr(),
-                  int(positions.dtype == torch.int64), T, table.data_ptr(), table.shape[0], rot,
-                  _stream(table))
-    return ol[0] if single else ol
+    T, dev = positions.shape[0], table.device
+    parts = [_part(x, o, a, i, T, dev) for x, o, a, i in zip(xl, ol, offs, inter)]
+    _launch("mi355_dsa_rotary", dev, b"".join([p[0] for p in parts]), n, positions.data_ptr(),
+            positions.dtype == torch.int64, T, table.data_ptr(), table.shape[0], table.shape[1])
+    return parts[0][1] if single else [p[1] for p in parts]
