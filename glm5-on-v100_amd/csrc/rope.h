@@ -27,6 +27,7 @@ struct RotaryPart {
   int dtype;  // 0 fp16, 1 bf16, 2 fp32
   int interleaved, inplace, vec;
   int units;    // of a head
+  uint32_t units_mul, units_shift;  // x / units = x * mul >> shift for x < 2^31
   int per_tok;  // n_head * units
   int tpb;      // tokens of a workgroup (then bpt is 1)
   int bpt;      // workgroups of a token
@@ -236,7 +237,7 @@ __device__ __forceinline__ void rotary_block_t(const RotaryArgs& a, const Rotary
   const uint8_t* x = p.x + t * p.x_tok;
   uint8_t* out = p.out + t * p.o_tok;
   for (int i = lo; i < hi; i += step) {
-    const int h = i / p.units, u = i - h * p.units;
+    const int h = (int)((uint64_t)(uint32_t)i * p.units_mul >> p.units_shift), u = i - h * p.units;
     rotary_unit<DT>(p, a.rot, row, x + h * p.x_head, out + h * p.o_head, u);
   }
 }

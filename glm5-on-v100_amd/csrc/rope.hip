@@ -67,8 +67,13 @@ __global__ void __launch_bounds__(256) rope_concat_cache_mla_kernel(RopeCacheArg
 // Token t of the output belongs to request r with cu[r] <= t < cu[r + 1] and is
 // its position starts[r] + t - cu[r]; a position whose row does not resolve
 // reads as zeros.  One wave per kGatherRows tokens, their loads issued together:
-// lane l converts dims 8 l .. +7 of a row, lanes 0-7 a rope piece each.
-constexpr int kGatherRows = 4;
+// lane l converts dims 8 l .. +7 of every row, and one piece of rope of one row.
+// Bound: memory, 656 or 1152 bytes read and 1152 (fp32: 2304) written a token.  us
+// for fp8 to fp16, 2 / 4 / 8 tokens a wave, ordinary stores and past the L2: 4096
+// tokens 3.6 / 4.0 / 4.9 and 3.4 / 3.8 / 4.8, 49152 15.2 / 14.3 / 14.1 and 13.1 /
+// 13.1 / 14.0, 262144 107 / 94 / 98 and 65 / 64 / 65 (7.3 TB/s); fp16 rows 262144
+// 117 / 118 / 253 and 104 / 102 / 240.
+constexpr int kGatherRows = 2;
 
 struct GatherArgs {
   const uint8_t* kv;
@@ -82,13 +87,18 @@ struct GatherArgs {
   int64_t total;
 };
 
+// The rows are stored past the L2: what reads them next, a projection, does so from
+// every XCD, and the caches keep the latent rows.
+__device__ __forceinline__ void put16(uint8_t* dst, const u32x4 v) {
+  __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(dst));
+}
 template <int DT>
 __device__ __forceinline__ void store8(uint8_t* dst, const float (&v)[8]) {
   if constexpr (DT == 2) {
-    *reinterpret_cast<f32x4*>(dst) = (f32x4){v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<f32x4*>(dst + 16) = (f32x4){v[4], v[5], v[6], v[7]};
+    put16(dst, Piece<2>::store({v[0], v[1], v[2], v[3]}));
+    put16(dst + 16, Piece<2>::store({v[4], v[5], v[6], v[7]}));
   } else {
-    *reinterpret_cast<u32x4*>(dst) = Piece<DT>::store(v);
+    put16(dst, Piece<DT>::store(v));
   }
 }
 
@@ -96,102 +106,107 @@ __device__ __forceinline__ void store8(uint8_t* dst, const float (&v)[8]) {
 template <bool FP8, int DT, int PE>
 __global__ void __launch_bounds__(256) gather_latent_kernel(GatherArgs a) {
   constexpr int E = DT == 2 ? 4 : 2;
+  constexpr int ROWS = kGatherRows;
+  constexpr int kRowBytes = FP8 ? kDsmlaRowBytes : 2 * kLatentDim;
   const int lane = threadIdx.x & 63;
-  const int64_t t0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kGatherRows;
+  const int64_t t0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * ROWS;
   if (t0 >= a.total) return;  // wave-uniform
-  // requests that end at or before each token
-  int req[kGatherRows];
-#pragma unroll
-  for (int k = 0; k < kGatherRows; k++) req[k] = 0;
+  // lane 8 k + i looks up token k's row (eight lanes alike): requests that end at or
+  // before the token, then its position's page
+  const int k = lane >> 3;
+  const int64_t t = t0 + (k < ROWS ? k : ROWS - 1);
+  int r = 0;
   for (int r0 = 0; r0 < a.n_req; r0 += 64) {
     const int64_t end = r0 + lane < a.n_req ? (int64_t)a.cu[r0 + lane + 1] : INT64_MAX;
 #pragma unroll
-    for (int k = 0; k < kGatherRows; k++) req[k] += __popcll(__ballot(end <= t0 + k));
+    for (int i = 0; i < ROWS; i++) {
+      const int n = __popcll(__ballot(end <= t0 + i));
+      if (i == (k < ROWS ? k : ROWS - 1)) r += n;
+    }
   }
-  int64_t row[kGatherRows];
-  bool live[kGatherRows];
+  const bool mine = t < a.total && r < a.n_req && t >= a.cu[0];  // a request's token
+  int64_t row = -1;
+  if (mine) {
+    const int64_t p = (a.starts ? a.starts[r] : 0) + (t - a.cu[r]);
+    if (p >= 0 && p <= INT32_MAX) {
+      const int pg = (int)((uint32_t)p / (uint32_t)a.page_size);
+      if (pg < a.max_blocks) {
+        const int64_t blk = a.bt[(int64_t)r * a.max_blocks + pg];
+        const int64_t x = blk * a.page_size + (p - (int64_t)pg * a.page_size);
+        if (blk >= 0 && x < a.n_rows) row = x;
+      }
+    }
+  }
+  // rope: all rows at once, piece lane % 8 of token k
+  u32x4 pe = {0u, 0u, 0u, 0u};
+  if (row >= 0)
+    pe = *reinterpret_cast<const u32x4*>(a.kv + row * kRowBytes + (FP8 ? kValueDim + 16 : 2 * kValueDim) +
+                                         16 * (lane & 7));
+  int64_t rows[ROWS];
+  bool live[ROWS];
 #pragma unroll
-  for (int k = 0; k < kGatherRows; k++) {
-    const int r = req[k];
-    live[k] = t0 + k < a.total && r < a.n_req && t0 + k >= a.cu[0];
-    row[k] = -1;
-    if (!live[k]) continue;
-    const int64_t p = (a.starts ? a.starts[r] : 0) + (t0 + k - a.cu[r]);
-    if (p < 0 || p > INT32_MAX) continue;
-    const int pg = (int)((uint32_t)p / (uint32_t)a.page_size);
-    if (pg >= a.max_blocks) continue;
-    const int64_t blk = a.bt[(int64_t)r * a.max_blocks + pg];
-    const int64_t x = blk * a.page_size + (p - (int64_t)pg * a.page_size);
-    if (blk >= 0 && x < a.n_rows) row[k] = x;
+  for (int i = 0; i < ROWS; i++) {
+    rows[i] = ((int64_t)__builtin_amdgcn_readlane((int)(row >> 32), 8 * i) << 32) |
+              (uint32_t)__builtin_amdgcn_readlane((int)row, 8 * i);
+    live[i] = __builtin_amdgcn_readlane(mine ? 1 : 0, 8 * i) != 0;
   }
   if constexpr (FP8) {
-    u32x2 q[kGatherRows];
-    float sc[kGatherRows];
-    u32x4 pe[kGatherRows];
+    u32x2 q[ROWS];
+    float sc[ROWS];
 #pragma unroll
-    for (int k = 0; k < kGatherRows; k++) {
-      const uint8_t* rp = a.kv + (row[k] < 0 ? 0 : row[k]) * kDsmlaRowBytes;
-      q[k] = (u32x2){0u, 0u};
-      sc[k] = 0.f;
-      pe[k] = (u32x4){0u, 0u, 0u, 0u};
-      if (row[k] >= 0) {
-        q[k] = *reinterpret_cast<const u32x2*>(rp + 8 * lane);
-        sc[k] = *reinterpret_cast<const float*>(rp + kValueDim + 4 * (lane >> 4));
-        pe[k] = *reinterpret_cast<const u32x4*>(rp + kValueDim + 16 + 16 * (lane & 7));
+    for (int i = 0; i < ROWS; i++) {
+      q[i] = (u32x2){0u, 0u};
+      sc[i] = 0.f;
+      if (rows[i] >= 0) {
+        const uint8_t* rp = a.kv + rows[i] * kRowBytes;
+        q[i] = *reinterpret_cast<const u32x2*>(rp + 8 * lane);
+        sc[i] = *reinterpret_cast<const float*>(rp + kValueDim + 4 * (lane >> 4));
       }
     }
 #pragma unroll
-    for (int k = 0; k < kGatherRows; k++) {
-      if (!live[k]) continue;
-      uint8_t* dst = a.out + (t0 + k) * a.out_stride;
+    for (int i = 0; i < ROWS; i++) {
+      if (!live[i]) continue;
       float v[8];
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const f32x2 x = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[k][i], false);
-        const f32x2 y = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[k][i], true);
-        v[4 * i] = x[0] * sc[k];
-        v[4 * i + 1] = x[1] * sc[k];
-        v[4 * i + 2] = y[0] * sc[k];
-        v[4 * i + 3] = y[1] * sc[k];
+      for (int h = 0; h < 2; h++) {
+        const f32x2 x = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[i][h], false);
+        const f32x2 y = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[i][h], true);
+        v[4 * h] = x[0] * sc[i];
+        v[4 * h + 1] = x[1] * sc[i];
+        v[4 * h + 2] = y[0] * sc[i];
+        v[4 * h + 3] = y[1] * sc[i];
       }
-      store8<DT>(dst + 8 * E * lane, v);
-      if (lane < 8) {
-        uint8_t* const d = dst + E * (kValueDim + 8 * lane);
-        if constexpr (DT == PE) {
-          *reinterpret_cast<u32x4*>(d) = pe[k];
-        } else {
-          float w[8];
-          Piece<PE>::load(pe[k], w);
-          store8<DT>(d, w);
-        }
-      }
+      store8<DT>(a.out + (t0 + i) * a.out_stride + 8 * E * lane, v);
     }
   } else {
-    u32x4 x[kGatherRows], pe[kGatherRows];
+    u32x4 x[ROWS];
 #pragma unroll
-    for (int k = 0; k < kGatherRows; k++) {
-      const uint8_t* rp = a.kv + (row[k] < 0 ? 0 : row[k]) * (2 * kLatentDim);
-      x[k] = pe[k] = (u32x4){0u, 0u, 0u, 0u};
-      if (row[k] >= 0) {
-        x[k] = *reinterpret_cast<const u32x4*>(rp + 16 * lane);
-        pe[k] = *reinterpret_cast<const u32x4*>(rp + 2 * kValueDim + 16 * (lane & 7));
-      }
+    for (int i = 0; i < ROWS; i++) {
+      x[i] = (u32x4){0u, 0u, 0u, 0u};
+      if (rows[i] >= 0)
+        x[i] = *reinterpret_cast<const u32x4*>(a.kv + rows[i] * kRowBytes + 16 * lane);
     }
 #pragma unroll
-    for (int k = 0; k < kGatherRows; k++) {
-      if (!live[k]) continue;
-      uint8_t* dst = a.out + (t0 + k) * a.out_stride;
-      auto put = [&](const u32x4 raw, int dim) {
-        if constexpr (DT == 0) {
-          *reinterpret_cast<u32x4*>(dst + E * dim) = raw;
-        } else {
-          float w[8];
-          Piece<0>::load(raw, w);
-          store8<DT>(dst + E * dim, w);
-        }
-      };
-      put(x[k], 8 * lane);
-      if (lane < 8) put(pe[k], kValueDim + 8 * lane);
+    for (int i = 0; i < ROWS; i++) {
+      if (!live[i]) continue;
+      uint8_t* const d = a.out + (t0 + i) * a.out_stride + 8 * E * lane;
+      if constexpr (DT == 0) {
+        put16(d, x[i]);
+      } else {
+        float v[8];
+        Piece<0>::load(x[i], v);
+        store8<DT>(d, v);
+      }
+    }
+  }
+  if (mine && k < ROWS) {
+    uint8_t* const d = a.out + t * a.out_stride + E * (kValueDim + 8 * (lane & 7));
+    if constexpr (DT == PE) {
+      put16(d, pe);
+    } else {
+      float v[8];
+      Piece<PE>::load(pe, v);
+      store8<DT>(d, v);
     }
   }
 }
@@ -234,6 +249,10 @@ static int rotary_part(const mi355_dsa_rotary_part& s, int rot, int64_t n_tok, c
   p->units = ((p->inplace ? rot : s.dim) - joined) / n;
   DSA_CHECK((int64_t)p->units * s.n_head < ((int64_t)1 << 30), "%s: too many heads", what);
   p->per_tok = p->units * s.n_head;
+  // ceil(2^(31 + k) / units), 2^k >= units > 2^(k - 1): exact for x < 2^31
+  const int k = ilog2_pow2(p->units);
+  p->units_shift = 31 + k;
+  p->units_mul = (uint32_t)((((uint64_t)1 << (31 + k)) + p->units - 1) / p->units);
   p->tpb = p->per_tok <= 128 ? 256 / p->per_tok : 1;
   p->bpt = 1;
   p->span = p->per_tok;
