@@ -13,18 +13,35 @@
 //
 // All n x H (token, head) rows of a request attend to the same keys, so they
 // are the rows of one matrix product: a group of 128 rows shares every key tile.
-// Workgroup = 128 rows, 4 waves, one per SIMD (512 registers each); wave w owns
-// 32 rows end to end: Q (576 dims) and O^T (512 dims, fp32) stay in registers.
-//   * S^T = K Q^T, v_mfma_f32_32x32x16: 32 keys x 32 rows, keys from LDS;
-//   * softmax per row: lane (row c, half) holds 16 of its 32 scores;
-//   * O^T += V^T P^T: the S^T accumulator layout (keys 8 a + 4 half + r) is P^T's
-//     operand layout; V^T comes from transpose LDS reads in that order.
+// Workgroup = 128 rows, 4 waves of 32 rows, one per SIMD (512 registers each):
+//   * S^T = K Q^T, v_mfma_f32_32x32x16: 32 keys x 32 rows over 576 dims, Q in 144
+//     registers;
+//   * softmax per row: lane (row c, half) holds 16 of its 32 scores; the running
+//     maximum is moved, and O scaled, only where a score exceeds it by 2^8 or more;
+//   * O^T += V^T P^T: 512 dims x 32 rows in 256 accumulation registers; the S^T
+//     accumulator layout (keys 8 a + 4 half + r) is P^T's operand layout, so P stays
+//     in registers; V^T comes from transpose LDS reads in that order.
+// The exponentials of tile i run beside the scores of tile i + 1, the maxima of those
+// beside the PV product of tile i; one barrier per tile.  fp16 rows come to LDS by
+// LDS-DMA three tiles ahead, into a ring of four tiles; fp8 rows come as they are, two
+// tiles ahead of their conversion into a ring of three, which is spread over both
+// products.
 //
-// Division of the work: the key tiles of all groups of all requests stand on one
-// line, group after group, and each workgroup takes an equal run of it (`per`
-// tiles, from the lengths on the device), whatever the mix of trees and contexts.
-// A group that a run's border cuts leaves partials (fp32 O / l, m, l), at most two
-// of them per workgroup, which tree_merge_kernel joins; the others write o at once.
+// What bounds it: the clock under the matrix cores' power.  One request of 1024 rows
+// over 184320 fp16 keys (411 GFLOP): 375 us, 1.10 PFLOP/s; on zeros, at full clock,
+// 298 us; an fp16 library product of 16384^3 reaches 1.31 PFLOP/s on this card.
+// 16 requests of 2560 rows over 32768 fp8 keys (2924 GFLOP): 3.0 ms, 0.97 PFLOP/s; on
+// zeros 2.57 ms: 128 conversions a wave and tile do not all hide beside MFMAs.
+// Measured against it: converting from registers (loads a tile ahead) 3.12 ms; pairs
+// of waves that share 64 rows and each take half of the dims (half of the LDS reads,
+// but scores and P exchanged through LDS, two barriers per tile) 385 us and 3.05 ms;
+// no overlap of softmax and products 430 us and 3.29 ms.
+//
+// Division of the work: from the lengths on the device, either cells (a request's
+// keys cut in pieces, the groups of a piece side by side) or, with the key tiles of
+// all groups of all requests on one line, equal runs of it; see tree_plan.  A group
+// that is cut leaves partials (fp32 O / l, m, l), at most two per workgroup, which
+// tree_merge_kernel joins; the others write o at once.
 #include <float.h>
 #include <math.h>
 #include <stddef.h>
@@ -39,16 +56,20 @@ constexpr int kTreeWaves = 4;
 constexpr int kTreeThreads = 64 * kTreeWaves;
 constexpr int kTreeRows = 128;      // (token, head) rows of a group
 constexpr int kTreeTile = 32;       // keys
-constexpr int kTreeSlots = 4;       // key tiles in LDS
-constexpr int kTreeSeg = 2048;      // keys resolved at a time
+// key tiles in LDS
+__host__ __device__ constexpr int tree_slots(bool fp8) { return fp8 ? 3 : 4; }
+constexpr int kTreePages = 2048;    // block-table entries resolved at a time
 constexpr int kTreeMaxDraft = 64;   // tokens of a request that a mask can name
 constexpr int kTreeWGs = 256;       // runs of the line: one workgroup per CU
 constexpr int kTreeMinTiles = 2;    // tiles of a run at least
 constexpr int kTreeBlocks = kLatentDim / 32;                   // 64-byte blocks of an fp16 row
 constexpr int kTreeSlotBytes = kTreeBlocks * kTreeTile * 64;   // 36864
-constexpr int kTreeAhead = 3;       // LDS reads ahead of their MFMA
+// fp8 rows as they are, on their way: bytes of a wave's share of a tile (twice)
+constexpr int kTreeRaw = 64 * 64 + 256;
+// LDS reads ahead of their MFMA; fp8 rows leave no registers for a third
+__host__ __device__ constexpr int tree_ahead(bool fp8) { return fp8 ? 2 : 3; }
 constexpr float kTreeLazyMax = 8.f; // log2 that scores may exceed the running maximum by
-constexpr int kTreePartWave = 64 * 64 * 4 + 64;  // floats of a wave's partial: O^T, m, l
+constexpr int kTreePartWave = 64 * 64 * 4;  // floats of a wave's O^T in a partial
 
 struct TreeParams {
   const f16* q;
@@ -59,22 +80,29 @@ struct TreeParams {
   const int64_t* mask;
   f16* o;
   float* lse;
-  float* part;  // [2 kTreeWGs][part_waves][kTreePartWave]
+  float* part;  // [2 kTreeWGs] of part_waves x kTreePartWave, m [32 part_waves], l likewise
   int part_waves;
+  int64_t* plan;  // [2] of the workspace
   int R, T, H;
-  int max_blocks, page_size, page_shift;
+  int max_blocks, page_size;
+  uint32_t page_mul, page_shift;  // x / page_size = x * page_mul >> page_shift for x < 2^31
   int64_t n_kv_rows;
   float sl;      // |scale| log2 e (log2 e where scale is 0)
   float q_sign;  // -1, 0 or 1: sign of scale
 };
 
+template <bool FP8>
 struct TreeSmem {
-  uint8_t ring[kTreeSlots][kTreeSlotBytes];
-  int32_t rows[kTreeSeg];
-  uint32_t found[kTreeSeg / kTreeTile];  // of each tile of the segment: keys with a row
+  uint8_t ring[tree_slots(FP8)][kTreeSlotBytes];
+  uint8_t raw[FP8 ? 2 : 1][FP8 ? kTreeWaves : 1][FP8 ? kTreeRaw : 16];
+  uint64_t see[kTreeRows];      // masks of the rows' tokens
+  int32_t blk[kTreePages];      // cache blocks of the segment, -1: none
   uint32_t dirty[kTreeWaves];
+  int gap;  // some block of the segment is missing
+  int run[kTreeWaves];  // the workgroup's, parked over the loops
 };
-static_assert(sizeof(TreeSmem) <= 160 * 1024, "one workgroup per CU");
+static_assert(sizeof(TreeSmem<false>) <= 160 * 1024 && sizeof(TreeSmem<true>) <= 160 * 1024,
+              "one workgroup per CU");
 
 // The kernel's parameters, read anew: the phases between the tile loops (finding
 // the next group, writing o) take theirs from here, so that they do not occupy
@@ -87,6 +115,14 @@ __device__ __forceinline__ TreeParams tree_params() {
 #else
   return {};
 #endif
+}
+
+// threadIdx.x, not known to be the same from use to use: what follows from it is
+// computed where it is used, instead of a register for each over the tile loop.
+__device__ __forceinline__ int tree_tid() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
 }
 
 // ---- the line of tiles ----
@@ -115,7 +151,7 @@ __device__ __forceinline__ int64_t shfl64(int64_t v, int src) {
 }
 // inclusive sums over the lanes
 __device__ __forceinline__ int64_t scan64(int64_t v) {
-  const int lane = threadIdx.x & 63;
+  const int lane = tree_tid() & 63;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
     const int64_t u = __shfl_up(v, m, 64);
@@ -123,32 +159,70 @@ __device__ __forceinline__ int64_t scan64(int64_t v) {
   }
   return v;
 }
-__device__ __forceinline__ int64_t tree_line(const TreeParams& p) {
-  int64_t total = 0;
+struct TreePlan {
+  int kt;       // tiles of a cell at most; 0: equal runs of the line
+  int64_t per;  // tiles of a run of the line
+};
+// Groups of one request that work on the same keys at the same time share them in
+// the XCD's L2; apart, each fetches them for itself, more than memory gives (one
+// request of 8 groups at 180k, fp16 rows: 430 us with a group per XCD).  So requests
+// are cut into cells of kt tiles, the groups of a cell next to each other, kt the
+// smallest found that needs no more than one workgroup per CU.  Where that leaves
+// more than a fifth of the workgroups' time unused (many groups, uneven lengths),
+// the workgroups take equal runs of the line instead.
+__device__ __forceinline__ TreePlan tree_plan(const TreeParams& p) {
+  const int lane = tree_tid() & 63;
+  int64_t line = 0;
   for (int r0 = 0; r0 < p.R; r0 += 64) {
-    const TreeReq q = tree_req(p, r0 + (int)(threadIdx.x & 63));
-    total += shfl64(scan64((int64_t)q.groups * q.tiles), 63);
+    const TreeReq q = tree_req(p, r0 + lane);
+    line += shfl64(scan64((int64_t)q.groups * q.tiles), 63);
   }
-  return total;
-}
-__device__ __forceinline__ int64_t tree_per(int64_t line) {
-  const int64_t per = (line + kTreeWGs - 1) / kTreeWGs;
-  return per > kTreeMinTiles ? per : kTreeMinTiles;
+  TreePlan pl;
+  pl.per = max((int64_t)kTreeMinTiles, (line + kTreeWGs - 1) / kTreeWGs);
+  const int64_t most = max((int64_t)kTreeMinTiles, line / (kTreeWGs * 4 / 5));
+  int64_t kt = pl.per;
+  pl.kt = 0;
+  while (true) {
+    int64_t units = 0;
+    for (int r0 = 0; r0 < p.R; r0 += 64) {
+      const TreeReq q = tree_req(p, r0 + lane);
+      const int n = kt >= q.tiles ? 1 : (q.tiles + (int)kt - 1) / (int)kt;
+      units += shfl64(scan64((int64_t)q.groups * n), 63);
+    }
+    if (units <= kTreeWGs) {
+      pl.kt = (int)min(kt, (int64_t)INT32_MAX);
+      break;
+    }
+    if (kt >= most) break;
+    kt = min(most, kt + max((int64_t)1, kt * (min(units, (int64_t)2 * kTreeWGs) - kTreeWGs) / (2 * kTreeWGs)));
+  }
+  return pl;
 }
 struct TreeItem {
   int r;          // request, -1: none
   int first, n, len, tiles;
   int g;          // group
-  int64_t start;  // of the group on the line
+  int cell;       // cells: tiles of one (the request's cells are alike)
+  int64_t start;  // of the group on the line; cells: the group's first unit
+  int step;       // cells: units from one cell of the group to its next
+  int part;       // cells: which one
 };
-// The group at place `at` of the line (by_group: the at-th group).
-__device__ __forceinline__ TreeItem tree_find(const TreeParams& p, int64_t at, bool by_group) {
-  TreeItem it = {-1, 0, 0, 0, 1, 0, 0};
+// The group (by_group: the at-th one) or the piece of one at place `at`: of the line,
+// or unit `at` of the cells, which stand request by request, cell by cell, group by
+// group.
+__device__ __forceinline__ TreeItem tree_find(const TreeParams& p, const TreePlan& pl, int64_t at,
+                                              bool by_group) {
+  TreeItem it = {-1, 0, 0, 0, 1, 0, 1, 0, 1, 0};
   int64_t base = 0, line = 0;
   for (int r0 = 0; r0 < p.R; r0 += 64) {
-    const int lane = threadIdx.x & 63;
-    const TreeReq q = tree_req(p, r0 + lane);
-    const int64_t cost = (int64_t)q.groups * q.tiles;
+    const TreeReq q = tree_req(p, r0 + (tree_tid() & 63));
+    int cell = q.tiles, n = 1;
+    if (pl.kt > 0 && q.tiles > pl.kt) {
+      n = (q.tiles + pl.kt - 1) / pl.kt;
+      cell = (q.tiles + n - 1) / n;
+      n = (q.tiles + cell - 1) / cell;
+    }
+    const int64_t cost = (int64_t)q.groups * (pl.kt > 0 ? n : q.tiles);  // units, or tiles
     const int64_t size = by_group ? q.groups : cost;
     const int64_t incl = base + scan64(size);
     const uint64_t hit = __ballot(at < incl && size > 0);
@@ -160,9 +234,19 @@ __device__ __forceinline__ TreeItem tree_find(const TreeParams& p, int64_t at, b
       it.n = __builtin_amdgcn_readlane(q.n, k);
       it.len = __builtin_amdgcn_readlane(q.len, k);
       it.tiles = __builtin_amdgcn_readlane(q.tiles, k);
-      const int64_t in = at - shfl64(incl - size, k);
-      it.g = (int)(by_group ? in : in / it.tiles);
-      it.start = shfl64(lsum - cost, k) + (int64_t)it.g * it.tiles;
+      it.cell = __builtin_amdgcn_readlane(cell, k);
+      const int groups = __builtin_amdgcn_readlane(q.groups, k);
+      const int in = (int)(at - shfl64(incl - size, k));
+      const int64_t from = shfl64(lsum - cost, k);
+      if (pl.kt > 0) {
+        it.part = by_group ? 0 : in / groups;
+        it.g = in - it.part * groups;
+        it.start = from + it.g;
+        it.step = groups;
+      } else {
+        it.g = by_group ? in : in / it.tiles;
+        it.start = from + (int64_t)it.g * it.tiles;
+      }
       return it;
     }
     base = shfl64(incl, 63);
@@ -170,10 +254,11 @@ __device__ __forceinline__ TreeItem tree_find(const TreeParams& p, int64_t at, b
   }
   return it;
 }
-// The partial of a group's piece in run w: a run's first group, cut from an
-// earlier run, has its first place, and a group that begins in the run its second.
-__device__ __forceinline__ float* tree_part(const TreeParams& p, int w, bool begins, int wave) {
-  return p.part + ((int64_t)(2 * w + (begins ? 1 : 0)) * p.part_waves + wave) * kTreePartWave;
+// Partial k of the workspace.  Of the line, a run's first group, cut from an earlier
+// run, has place 2 run, and a group that begins in the run 2 run + 1; a cell has its
+// unit's number.
+__device__ __forceinline__ float* tree_part(const TreeParams& p, int64_t k) {
+  return p.part + k * p.part_waves * (kTreePartWave + 64);
 }
 
 // ---- key tiles ----
@@ -183,50 +268,74 @@ __device__ __forceinline__ float* tree_part(const TreeParams& p, int w, bool beg
 // Wave w brings blocks 9 (w / 2) .. +8 of keys 16 (w % 2) .. +15, four lanes a key.
 __device__ __align__(16) const uint8_t kTreeZeroRow[kLatentDim * 2] = {};
 
-// fp8_ds_mla rows come through registers: a thread's share of a tile is 64
-// e4m3 values (quads 4 (w / 2) .. +3 of 64 dims of key drow, 16 dims of each), their
-// two scales and one rope piece.
-struct TreeRaw {
-  u32x4 e[4];
-  f32x2 sc;
-  u32x4 pe;
-};
-__device__ __forceinline__ void tree_load(TreeRaw& x, const uint8_t* row, int w) {
-  const int j = threadIdx.x & 3, q = 4 * (w >> 1);
-#pragma unroll
-  for (int u = 0; u < 4; u++)
-    x.e[u] = *reinterpret_cast<const u32x4*>(row + 64 * (q + u) + 16 * j);
-  x.sc = *reinterpret_cast<const f32x2*>(row + kValueDim + 2 * q);
-  x.pe = *reinterpret_cast<const u32x4*>(row + kValueDim + 16 + 64 * (w >> 1) + 16 * j);
+__device__ __forceinline__ void tree_dma_rope(const uint8_t* row, uint8_t* slot, int w) {
+  const int lane = tree_tid() & 63;
+  dma16(row + kValueDim + 16 + 64 * (w >> 1) + 16 * ((lane & 3) ^ ((lane >> 4) & 3)),
+        slot + 2048 * (16 + (w >> 1)) + 1024 * (w & 1));
 }
-// RN(e4m3 * scale) of the values, written to the tile in LDS.  Quad q holds blocks
-// 2 q and 2 q + 1; lane j of the four has pieces 2 (j % 2) and + 1 of block 2 q + j / 2.
-// Lanes 2 and 3 write their second piece first, so that the four lanes' banks differ.
-__device__ __forceinline__ void tree_store(const TreeRaw& x, uint8_t* slot, int w) {
-  const int lane = threadIdx.x & 63, j = lane & 3, q = 4 * (w >> 1);
-  const int key = 16 * (w & 1) + (lane >> 2), sw = (key >> 2) & 3;
-  uint8_t* const at = slot + 64 * key;
-#pragma unroll
-  for (int u = 0; u < 4; u++) {
-    const float sc = x.sc[u >> 1];
-    f16x8 v[2];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)x.e[u][i], false);
-      const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)x.e[u][i], true);
-      f16x8& d = v[i >> 1];
-      d[4 * (i & 1)] = (f16)(a[0] * sc);
-      d[4 * (i & 1) + 1] = (f16)(a[1] * sc);
-      d[4 * (i & 1) + 2] = (f16)(b[0] * sc);
-      d[4 * (i & 1) + 3] = (f16)(b[1] * sc);
-    }
-    uint8_t* const blk = at + 2048 * (2 * (q + u) + (j >> 1));
-    const int first = 2 * (j & 1) + (j >> 1), second = 2 * (j & 1) + 1 - (j >> 1);
-    const f16x8 x0 = j >> 1 ? v[1] : v[0], x1 = j >> 1 ? v[0] : v[1];
-    *reinterpret_cast<f16x8*>(blk + 16 * (first ^ sw)) = x0;
-    *reinterpret_cast<f16x8*>(blk + 16 * (second ^ sw)) = x1;
-  }
-  *reinterpret_cast<u32x4*>(at + 2048 * (16 + (w >> 1)) + 16 * (j ^ sw)) = x.pe;
+// fp8_ds_mla rows: a wave's share of a tile, 256 e4m3 values of 16 keys (quads
+// 4 (w / 2) .. +3 of 64 dims; lane j of a key's four has 16 of each quad) and the keys'
+// scales, comes by LDS-DMA as it is, to be converted by the wave that fetched it.
+__device__ __forceinline__ void tree_dma_raw(const uint8_t* row, uint8_t* raw, int w) {
+  const int l = tree_tid() & 63;
+  const uint8_t* src = row + 256 * (w >> 1) + 16 * (l & 3);
+  dma16_at<0>(src, raw);
+  dma16_at<64>(src, raw + 1024);
+  dma16_at<128>(src, raw + 2048);
+  dma16_at<192>(src, raw + 3072);
+  dma4(row + kValueDim + 4 * (l & 3), raw + 4096);
+}
+// Addresses of a conversion.  In a tile quad q holds blocks 2 q and 2 q + 1; lane j of
+// the four has pieces 2 (j % 2) and + 1 of block 2 q + j / 2.  Lanes 2 and 3 take
+// their second piece first, so that the four lanes' banks differ.
+struct TreeConv {
+  uint32_t from0, from1;  // the first and second 8 values of quad 0 in the share
+  uint32_t to0, to1;      // their pieces in the tile
+  uint32_t sc;            // the key's two scales
+};
+__device__ __forceinline__ TreeConv tree_conv(uint32_t raw, uint32_t slot, int w) {
+  const int l = tree_tid() & 63, j = l & 3, key = 16 * (w & 1) + (l >> 2);
+  TreeConv c;
+  c.from0 = raw + 16 * l + 8 * (j >> 1);
+  c.from1 = c.from0 ^ 8u;
+  c.to0 = slot + 64 * key + 2048 * (8 * (w >> 1) + (j >> 1)) +
+          16 * ((2 * (j & 1) + (j >> 1)) ^ ((key >> 2) & 3));
+  c.to1 = c.to0 ^ 16u;
+  c.sc = raw + 4096 + 16 * (l >> 2) + 8 * (w >> 1);
+  asm volatile("" : "+v"(c.from0), "+v"(c.from1), "+v"(c.to0), "+v"(c.to1));
+  return c;
+}
+typedef __attribute__((address_space(3))) f32x2 lds_f32x2;
+typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
+typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+// values 8 h .. +7 of the share's quad I / 2, h = I % 2 in the order of the writes
+template <int I>
+__device__ __forceinline__ u32x2 tree_raw(const TreeConv& c) {
+  return *(const lds_u32x2*)((I % 2 ? c.from1 : c.from0) + 1024u * (I / 2));
+}
+// RN(e4m3 * scale) of dword H of them, the second one with the write of the piece
+template <int I, int H>
+__device__ __forceinline__ void tree_convert(const TreeConv& c, const u32x2 x, const f32x2 sc,
+                                             f16x8& v) {
+  const float s = sc[I / 4];
+  const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)x[H], false);
+  const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)x[H], true);
+  v[4 * H] = (f16)(a[0] * s);
+  v[4 * H + 1] = (f16)(a[1] * s);
+  v[4 * H + 2] = (f16)(b[0] * s);
+  v[4 * H + 3] = (f16)(b[1] * s);
+  if constexpr (H == 1) *(lds_f16x8*)((I % 2 ? c.to1 : c.to0) + 4096u * (I / 2)) = v;
+}
+__device__ __forceinline__ void tree_convert_all(uint32_t raw, uint32_t slot, int w) {
+  const TreeConv c = tree_conv(raw, slot, w);
+  const f32x2 sc = *(const lds_f32x2*)c.sc;
+  unroll<8>([&](auto ic) {
+    constexpr int i = ic;
+    const u32x2 x = tree_raw<i>(c);
+    f16x8 v;
+    tree_convert<i, 0>(c, x, sc, v);
+    tree_convert<i, 1>(c, x, sc, v);
+  });
 }
 
 template <int I>
@@ -234,65 +343,80 @@ __device__ __forceinline__ void tree_dma1(const uint8_t* src, uint8_t* dst) {
   dma16_at<64 * I>(src, dst + 2048 * I);
 }
 
-// S^T of a tile: step t covers dims 16 t + 8 hf .. +7.  DMA: an LDS-DMA piece of
-// the tile three ahead goes out every fourth step.
-template <bool DMA>
-__device__ __forceinline__ void tree_qk(f32x16& s, const f16x8 (&qf)[36], uint32_t slot,
-                                        uint32_t ka0, const uint8_t* src, uint8_t* dst) {
-  const uint32_t kb = slot + ka0;
-  auto kread = [&](int t) {
-    return *(const lds_f16x8*)(((t & 1) ? (kb ^ 32u) : kb) + 2048u * (t >> 1));
-  };
-  constexpr int NS = 36;
-  f16x8 kf[kTreeAhead + 1];
+// Operands of the next MFMAs, read from LDS A steps early.
+template <int A>
+struct TreeFrag {
+  f16x8 x[A + 1];
+};
+// Two addresses of a tile, the second one ^ 32, from which every read of it is an
+// instruction's offset.  Opaque to the compiler, which otherwise computes an address
+// for each: a wave alone on its SIMD has room for about five other instructions
+// beside an MFMA of 32 cycles, and pays some 5 cycles for each beyond that (measured:
+// 4 VALU 33.1 cycles, 6 35.8, 8 43.7; one LDS read 35.1, with 4 VALU 44.7).
+struct TreeAddr {
+  uint32_t a, b;
+};
+__device__ __forceinline__ TreeAddr tree_addr(uint32_t a, uint32_t more) {
+  TreeAddr r = {a, (a + more) ^ 32u};
+  asm volatile("" : "+v"(r.a), "+v"(r.b));
+  return r;
+}
+// K of step t (dims 16 t + 8 hf .. +7), from slot + ka0
+__device__ __forceinline__ f16x8 tree_kread(const TreeAddr& k, int t) {
+  return *(const lds_f16x8*)(((t & 1) ? k.b : k.a) + 2048u * (t >> 1));
+}
+// V^T of step u (dims 32 (u % 16) .. +31, half u / 16 of the keys), from slot + va0
+__device__ __forceinline__ f16x8 tree_vread(const TreeAddr& v, int u) {
+  const int t = u % 16, t2 = u / 16;
+  const s16x4 x =
+      __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(v.a + 2048u * t + 1024u * t2));
+  const s16x4 y =
+      __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(v.b + 2048u * t + 1024u * t2));
+  const f16x4 x0 = __builtin_bit_cast(f16x4, x), x1 = __builtin_bit_cast(f16x4, y);
+  return (f16x8){x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+}
+template <int A>
+__device__ __forceinline__ void tree_kfirst(TreeFrag<A>& k, const TreeAddr& kb) {
 #pragma unroll
-  for (int t = 0; t < kTreeAhead; t++) kf[t] = kread(t);
+  for (int t = 0; t < A; t++) k.x[t] = tree_kread(kb, t);
+}
+template <int A>
+__device__ __forceinline__ void tree_vfirst(TreeFrag<A>& v, const TreeAddr& vb) {
+#pragma unroll
+  for (int u = 0; u < A; u++) v.x[u] = tree_vread(vb, u);
+}
+
+// S^T of a tile whose first operands are in k.  side(t): work beside the MFMA of
+// step t.
+template <int A, class F>
+__device__ __forceinline__ void tree_qk(f32x16& s, const f16x8 (&qf)[36], TreeFrag<A>& k,
+                                        const TreeAddr& kb, F&& side) {
+  constexpr int NS = 36;
   __builtin_amdgcn_sched_barrier(0);
   unroll<NS>([&](auto tc) {
     constexpr int t = tc;
-    if constexpr (t + kTreeAhead < NS) kf[(t + kTreeAhead) % (kTreeAhead + 1)] = kread(t + kTreeAhead);
-    if constexpr (t == 0) hw_qk0(s, kf[0], qf[0]);
-    else hw_qk(s, kf[t % (kTreeAhead + 1)], qf[t]);
-    if constexpr (DMA && t % 4 == 0) tree_dma1<t / 4>(src, dst);
+    if constexpr (t + A < NS) k.x[(t + A) % (A + 1)] = tree_kread(kb, t + A);
+    if constexpr (t == 0) hw_qk0(s, k.x[0], qf[0]);
+    else hw_qk(s, k.x[t % (A + 1)], qf[t]);
+    side(tc);
     __builtin_amdgcn_sched_barrier(0);
   });
 }
 
-// O^T += V^T P^T of a tile, p = 2^(s sl - ml); returns this lane's sum of p.
-__device__ __forceinline__ float tree_pv(const f32x16& s, float sl, float ml, uint32_t slot,
-                                         uint32_t va0) {
-  const uint32_t vb0 = slot + va0, vb1 = (vb0 + 512u) ^ 32u;
-  auto vread = [&](int u) {
-    const int t = u % 16, t2 = u / 16;
-    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_s16x4*)(vb0 + 2048u * t + 1024u * t2));
-    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_s16x4*)(vb1 + 2048u * t + 1024u * t2));
-    const f16x4 x0 = __builtin_bit_cast(f16x4, x), x1 = __builtin_bit_cast(f16x4, y);
-    return (f16x8){x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
-  };
-  f16x8 vf[kTreeAhead + 1], pb[2];
-#pragma unroll
-  for (int u = 0; u < kTreeAhead; u++) vf[u] = vread(u);
-  __builtin_amdgcn_sched_barrier(0);
-  float ls = 0.f;
-  auto pexp = [&](int e) {
-    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], sl, -ml));
-    ls += x;
-    pb[e >> 3][e & 7] = (f16)x;
-  };
-#pragma unroll
-  for (int e = 0; e < 8; e++) pexp(e);
+// O^T += V^T P^T of a tile whose first operands are in v; side(u): work beside the
+// MFMA of step u.
+template <int A, class F>
+__device__ __forceinline__ void tree_pv(const f16x8 (&pb)[2], TreeFrag<A>& v, const TreeAddr& vb,
+                                        F&& side) {
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("s_nop 1");  // P is written
   unroll<32>([&](auto uc) {
     constexpr int u = uc;
-    if constexpr (u + kTreeAhead < 32) vf[(u + kTreeAhead) % (kTreeAhead + 1)] = vread(u + kTreeAhead);
-    hw_mma<u % 16>(vf[u % (kTreeAhead + 1)], pb[u / 16]);
-    if constexpr (u < 8) pexp(8 + u);
+    if constexpr (u + A < 32) v.x[(u + A) % (A + 1)] = tree_vread(vb, u + A);
+    hw_mma<u % 16>(v.x[u % (A + 1)], pb[u / 16]);
+    side(uc);
     __builtin_amdgcn_sched_barrier(0);
   });
-  return ls;
 }
 
 // Keys of a tile that a row with the mask `see` sees; drafted token 0 is the
@@ -303,13 +427,21 @@ __device__ __forceinline__ uint32_t tree_visible(uint64_t see, int shift) {
   return shift > -kTreeMaxDraft ? (uint32_t)(see >> -shift) : 0;
 }
 
+// a where the bit of the lane's score e is set in keys, else b, without a compare:
+// sixteen of those would take 32 scalar registers
+__device__ __forceinline__ float tree_pick(uint32_t keys, int e, float a, float b) {
+  const uint32_t on = __builtin_amdgcn_sbfe((int)keys, 8 * (e >> 2) + (e & 3), 1);
+  return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, a) & on) |
+                                       (__builtin_bit_cast(uint32_t, b) & ~on));
+}
+
 // A tile with drafted tokens, which not every row sees: 0 * inf would reach the
 // rows that do not.  Key rows that hold an infinity or NaN become zeros in LDS,
 // and their keys bits of the returned mask (to every wave, after a barrier): the
 // scores of the rows that see them are made NaN instead.  Wave w looks after
 // keys 8 w .. +7, eight lanes a key.
-__device__ __forceinline__ uint32_t tree_clean(TreeSmem& sh, uint8_t* slot, int w) {
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ uint32_t tree_clean(uint32_t* flags, uint8_t* slot, int w) {
+  const int lane = tree_tid() & 63;
   // the lane's pieces: places q = lane % 8 + 8 i of the key's 72, four to a block
   uint8_t* const key = slot + 64 * (8 * w + (lane >> 3)) + 16 * (lane & 3) + 2048 * ((lane >> 2) & 1);
   bool bad = false;
@@ -323,69 +455,83 @@ __device__ __forceinline__ uint32_t tree_clean(TreeSmem& sh, uint8_t* slot, int 
   uint32_t keys = 0;
 #pragma unroll
   for (int k = 0; k < 8; k++) keys |= ((lanes >> (8 * k)) & 0xff) != 0 ? 1u << k : 0u;
-  if (lane == 0) sh.dirty[w] = keys;
+  if (lane == 0) flags[w] = keys;
   if (keys) {
     if ((keys >> (lane >> 3)) & 1)
       for (int i = 0; i < 9; i++) *reinterpret_cast<u32x4*>(key + 4096 * i) = (u32x4){0u, 0u, 0u, 0u};
   }
   lds_barrier();
-  return __builtin_amdgcn_readfirstlane(sh.dirty[0] | sh.dirty[1] << 8 | sh.dirty[2] << 16 |
-                                        sh.dirty[3] << 24);
+  return __builtin_amdgcn_readfirstlane(flags[0] | flags[1] << 8 | flags[2] << 16 | flags[3] << 24);
 }
 
 template <bool FP8>
 __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  TreeSmem& sh = *reinterpret_cast<TreeSmem*>(smem_raw);
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = lane & 31, hf = lane >> 5;
+  TreeSmem<FP8>& sh = *reinterpret_cast<TreeSmem<FP8>*>(smem_raw);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
   // neighbouring runs on one XCD (workgroups go round the eight of them)
   const int run = (int)(blockIdx.x & 7) * (kTreeWGs / 8) + (int)(blockIdx.x >> 3);
-  int64_t at;
-  int left;  // tiles of the run from there on
-  {
-    const int64_t line = tree_line(p), per = tree_per(line);
-    at = run * per;
-    left = (int)max((int64_t)0, min(per, line - at));
+  sh.run[w] = run;
+  TreePlan plan = tree_plan(p);
+  if (run == 0 && threadIdx.x == 0) {  // for the merge
+    p.plan[0] = plan.kt;
+    p.plan[1] = plan.per;
+  }
+  int64_t at = run;
+  int left = 1;  // cells: one unit; tiles of the run from there on
+  if (plan.kt == 0) {
+    at = run * plan.per;
+    left = (int)min(plan.per, (int64_t)INT32_MAX);
   }
 
   // LDS addresses within a slot
+  uint32_t ka0, va0;
+  {
+    const int lane = threadIdx.x & 63, c = lane & 31, hf = lane >> 5;
+    // QK steps 0, 2, ..; ^ 32: 1, 3, ..
+    ka0 = 64 * c + 16 * (hf ^ ((c >> 2) & 3));
+    // transpose reads: keys 4 hf + ti / 4 (+ 8, + 16 t2), dims 32 t + 16 td + 4 (ti % 4) .. +3
+    const int ti = lane & 15, td = (lane >> 4) & 1;
+    va0 = 64 * (4 * hf + (ti >> 2)) + 16 * ((2 * td + ((ti >> 1) & 1)) ^ hf) +
+          8 * (ti & 1);
+  }
   const uint32_t lds0 = (uint32_t)(uintptr_t)(&sh.ring[0][0]);
-  const uint32_t ka0 = 64 * c + 16 * (hf ^ ((c >> 2) & 3));  // QK steps 0, 2, ..; ^ 32: 1, 3, ..
-  // transpose reads: keys 4 hf + ti / 4 (+ 8, + 16 t2), dims 32 t + 16 td + 4 (ti % 4) .. +3
-  const int ti = lane & 15, td = (lane >> 4) & 1;
-  const uint32_t va0 =
-      64 * (4 * hf + (ti >> 2)) + 16 * ((2 * td + ((ti >> 1) & 1)) ^ hf) + 8 * (ti & 1);
-  const int drow = 16 * (w & 1) + (lane >> 2);  // the key whose pieces this lane fetches
-  const int dbyte = 64 * 9 * (w >> 1) + 16 * ((lane & 3) ^ ((lane >> 4) & 3));
   const int dlds = 2048 * 9 * (w >> 1) + 1024 * (w & 1);
+  auto lds_at = [](const void* x) { return (uint32_t)(uintptr_t)x; };
+  auto wave = [&]() {  // w where nothing that derives from it is to be kept over the kernel
+    int x = w;
+    asm volatile("" : "+s"(x));
+    return x;
+  };
 
   while (left > 0) {
     const TreeParams p = tree_params();
-    const TreeItem it = tree_find(p, at, false);
-    if (it.r < 0) break;
+    const TreeItem it = tree_find(p, plan, at, false);
+    if (it.r < 0) break;  // past the last one
     const int M = it.n * p.H;  // rows of the request
     const int m0 = it.g * kTreeRows + 32 * w;
     const bool active = m0 < M;
-    const int t_lo = (int)(at - it.start);
-    const int t_hi = min(it.tiles, t_lo + left);
+    const bool cells = plan.kt > 0;
+    const int t_lo = cells ? it.part * it.cell : (int)(at - it.start);
+    const int t_hi = (int)min((int64_t)it.tiles, (int64_t)t_lo + (cells ? it.cell : left));
     const bool whole = t_lo == 0 && t_hi == it.tiles;
+    const bool first = t_lo == 0;
     at += t_hi - t_lo;
-    left -= t_hi - t_lo;
-    const int k_lo = t_lo * kTreeTile, k_hi = min(t_hi * kTreeTile, it.len);
+    left = cells ? 0 : left - (t_hi - t_lo);
+    const int k_hi = min(t_hi * kTreeTile, it.len);
     const int draft0 = max(0, p.seq_lens[it.r]) - it.n;  // position of drafted token 0
 
     // ---- Q (B operand): row c, dims 16 s + 8 hf .. +7 of step s ----
     f16x8 qf[kLatentDim / 16];
-    uint64_t see = 0;
     {
+      const int c = tree_tid() & 31, hf = (tree_tid() >> 5) & 1;
       const int m = min(m0 + c, M - 1);
       const f16* qrow = p.q + ((int64_t)it.first * p.H + m) * kLatentDim;
 #pragma unroll
       for (int s = 0; s < kLatentDim / 16; s++)
         qf[s] = *reinterpret_cast<const f16x8*>(qrow + 16 * s + 8 * hf);
-      see = (uint64_t)p.mask[it.first + (uint32_t)m / (uint32_t)p.H];
+      sh.see[32 * w + c] = (uint64_t)p.mask[it.first + (uint32_t)m / (uint32_t)p.H];
       const f16 sg = (f16)p.q_sign;
       const f16x8 sg8 = {sg, sg, sg, sg, sg, sg, sg, sg};
 #pragma unroll
@@ -396,103 +542,285 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
     unroll<256>([&](auto i) { hw_zero<i>(); });
     float m_run = -1e30f, l_part = 0.f;  // m: of the raw scores; l: this lane's keys only
 
-    for (int seg_lo = k_lo; seg_lo < k_hi; seg_lo += kTreeSeg) {
-      const int nkeys = min(k_hi - seg_lo, kTreeSeg);
-      const int ntiles = (nkeys + kTreeTile - 1) / kTreeTile;
-      __syncthreads();  // rows and the ring are free
-      for (int j = threadIdx.x; j < ntiles * kTreeTile; j += kTreeThreads) {
-        int row = -1;
-        if (j < nkeys) {
-          const int pos = seg_lo + j;
-          const int pg = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
-          const int blk = p.bt[(int64_t)it.r * p.max_blocks + pg];
-          const int64_t x = (int64_t)blk * p.page_size + (pos - pg * p.page_size);
-          if (blk >= 0 && x < p.n_kv_rows) row = (int)x;
+    auto page_of = [&](int pos) { return (int)((uint64_t)(uint32_t)pos * p.page_mul >> p.page_shift); };
+    for (int seg = t_lo; seg < t_hi && seg * kTreeTile < k_hi;) {
+      // tiles of this segment: as many as its pages cover
+      const int pg0 = page_of(seg * kTreeTile);
+      const int64_t room = (int64_t)(pg0 + kTreePages) * p.page_size - (int64_t)seg * kTreeTile;
+      const int ntiles = (int)min((int64_t)(min(t_hi * kTreeTile, k_hi + kTreeTile - 1) / kTreeTile - seg),
+                                  room / kTreeTile);
+      const int seg_lo = seg * kTreeTile;
+      seg += ntiles;
+      const int keys = min(ntiles * kTreeTile, k_hi - seg_lo);  // of the segment
+      __syncthreads();  // blk and the ring are free
+      if (threadIdx.x == 0) sh.gap = 0;
+      __syncthreads();
+      {
+        const int n = page_of(seg_lo + keys - 1) - pg0 + 1;
+        const int64_t blocks = (p.n_kv_rows + p.page_size - 1) / p.page_size;
+        bool gap = p.n_kv_rows % p.page_size != 0;
+        for (int j = tree_tid(); j < n; j += kTreeThreads) {
+          const int b = p.bt[(int64_t)it.r * p.max_blocks + pg0 + j];
+          const bool ok = b >= 0 && b < blocks;
+          gap |= !ok;
+          sh.blk[j] = ok ? b : -1;
         }
-        sh.rows[j] = row;
-        const uint64_t found = __ballot(row >= 0);
-        if ((lane & 31) == 0) sh.found[j / kTreeTile] = (uint32_t)(found >> (lane & 32));
+        if (__any(gap) && (tree_tid() & 63) == 0) sh.gap = 1;
       }
       __syncthreads();
-      auto source = [&](int tile) {
-        const int row = tile < ntiles ? sh.rows[tile * kTreeTile + drow] : -1;
-        if constexpr (FP8) return row >= 0 ? p.kv + (int64_t)row * kDsmlaRowBytes : kTreeZeroRow;
-        else
-          return (row >= 0 ? p.kv + (int64_t)row * (kLatentDim * 2) : kTreeZeroRow) + dbyte;
+      const bool gaps = __builtin_amdgcn_readfirstlane(sh.gap) != 0;  // keys without a row
+      // cache row of a key of the segment, -1: none
+      auto row_at = [&](int key) {
+        if (key >= keys) return -1;
+        const int pos = seg_lo + key;
+        const int pg = page_of(pos);
+        const int b = sh.blk[pg - pg0];
+        const uint32_t row = (uint32_t)b * (uint32_t)p.page_size + (uint32_t)(pos - pg * p.page_size);
+        return b >= 0 && row < (uint32_t)p.n_kv_rows ? (int)row : -1;
       };
-      TreeRaw raw;
+      // the row of the key that this lane fetches of a tile, and its bytes
+      auto row_of = [&](int tile) {
+        return row_at(tile * kTreeTile + 16 * (wave() & 1) + ((tree_tid() & 63) >> 2));
+      };
+      // .. in two steps, for the loop
+      int row_blk = 0, row_off = 0;
+      auto row_begin = [&](int tile) {
+        const int key = tile * kTreeTile + 16 * (w & 1) + ((tree_tid() & 63) >> 2);
+        const int pos = seg_lo + min(key, keys - 1), pg = page_of(pos);
+        row_off = key < keys ? pos - pg * p.page_size : -1;
+        row_blk = sh.blk[pg - pg0];
+      };
+      auto row_end = [&]() {
+        const uint32_t row = (uint32_t)row_blk * (uint32_t)p.page_size + (uint32_t)row_off;
+        return (row_blk | row_off) >= 0 && row < (uint32_t)p.n_kv_rows ? (int)row : -1;
+      };
+      auto bytes_of = [&](int row) {
+        if constexpr (FP8) {
+          return row >= 0 ? p.kv + (int64_t)row * kDsmlaRowBytes : kTreeZeroRow;
+        } else {
+          const int l = tree_tid();
+          return (row >= 0 ? p.kv + (int64_t)row * (kLatentDim * 2) : kTreeZeroRow) +
+                 64 * 9 * (w >> 1) + 16 * ((l & 3) ^ ((l >> 4) & 3));
+        }
+      };
+      // Scores of tile i + 1 are computed beside the exponentials of tile i, their
+      // maximum beside the product of P and V of tile i.  Every chain of dependent
+      // instructions is spread over the steps (a wave alone on its SIMD waits for
+      // each), and the first operands of a product are read in the one before it.
+      auto is_draft = [&](int tile) { return seg_lo + tile * kTreeTile + kTreeTile > draft0; };
+      // slots of the tiles i .. i + 3, bytes
+      int s0 = 0, s1 = kTreeSlotBytes, s2 = 2 * kTreeSlotBytes, s3 = FP8 ? 0 : 3 * kTreeSlotBytes;
+      uint32_t dirty = 0;
       if constexpr (FP8) {
-        tree_load(raw, source(0), w);
-        tree_store(raw, sh.ring[0], w);
-        tree_load(raw, source(1), w);
+        // tiles 0 and 1 converted, 2 and 3 on their way
+        const int ww = wave();
+        for (int k = 0; k < 4; k++) {
+          const uint8_t* src = bytes_of(row_of(k));
+          if (k >= 2)
+            tree_convert_all(lds_at(sh.raw[k - 2][ww]), lds0 + (k - 2) * kTreeSlotBytes, ww);
+          if (k < 3) tree_dma_rope(src, sh.ring[k < 3 ? k : 0], ww);
+          tree_dma_raw(src, sh.raw[k & 1][ww], ww);
+          if (k == 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        asm volatile("s_waitcnt vmcnt(5)" ::: "memory");
       } else {
 #pragma unroll 1
-        for (int k = 0; k < kTreeSlots - 1; k++) {
-          const uint8_t* src = source(k);
+        for (int k = 0; k < 3; k++) {
+          const uint8_t* src = bytes_of(row_of(k));
           int to = k * kTreeSlotBytes + dlds;
           asm volatile("" : "+s"(to));  // the loop's addresses are not kept over the kernel
           unroll<9>([&](auto i) { tree_dma1<i>(src, sh.ring[0] + to); });
         }
+        asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
       }
-      for (int tile = 0; tile < ntiles; tile++) {
-        // two more tiles may stay in flight
-        if constexpr (!FP8) asm volatile("s_waitcnt vmcnt(18)" ::: "memory");
-        lds_barrier();  // the tile is in; every wave is done with the one before it
-        const int pos0 = seg_lo + tile * kTreeTile;
-        const bool draft = pos0 + kTreeTile > draft0;
-        uint32_t dirty = 0;
-        if (draft) dirty = tree_clean(sh, sh.ring[tile % kTreeSlots], w);
-        const uint8_t* src = nullptr;
-        uint8_t* dst = nullptr;
-        if constexpr (FP8) {
-          tree_store(raw, sh.ring[(tile + 1) % kTreeSlots], w);
-          tree_load(raw, source(tile + 2), w);
-          if (!active) continue;
-        } else {
-          src = source(tile + kTreeSlots - 1);
-          dst = sh.ring[(tile + kTreeSlots - 1) % kTreeSlots] + dlds;
-        }
-        if (!FP8 && !active) {
-          unroll<9>([&](auto i) { tree_dma1<i>(src, dst); });
-          continue;
-        }
-        const uint32_t slot = lds0 + (tile % kTreeSlots) * kTreeSlotBytes;
-        f32x16 s;
-        tree_qk<!FP8>(s, qf, slot, ka0, src, dst);
+      lds_barrier();  // tiles 0 and 1 are in
+      if (is_draft(0)) dirty = tree_clean(sh.dirty, sh.ring[0], wave());
+
+      constexpr int A = tree_ahead(FP8);
+      f32x16 s;             // scores of tile i, then their exponentials
+      float mt = 0.f;       // the largest score
+      float ml = 0.f, alpha = 1.f;  // of the exponents; of O
+      int up = 0;           // O has to be scaled
+      TreeFrag<A> kf, vf;
+      TreeAddr kb;
+      auto mask = [&](int tile) {
+        const bool draft = is_draft(tile);
+        if (!gaps && !draft && (tile + 1) * kTreeTile <= keys) return;
         hw_settle();
         asm volatile("" : "+v"(s));  // no use of S above the wait
-        uint32_t vis = __builtin_amdgcn_readfirstlane(sh.found[tile]);  // keys with a row
-        if (draft || vis != ~0u) {
-          if (draft) vis &= tree_visible(see, draft0 - pos0);
-          vis >>= 4 * hf;
+        const int l = tree_tid(), h4 = (l >> 3) & 4;  // 4 hf
+        // keys with a row; 32 lanes look at one each
+        uint32_t vis = (uint32_t)__ballot(row_at(tile * kTreeTile + (l & 31)) >= 0);
+        if (draft) vis &= tree_visible(sh.see[32 * wave() + (l & 31)], draft0 - seg_lo - tile * kTreeTile);
+        vis >>= h4;
 #pragma unroll
-          for (int e = 0; e < 16; e++)
-            s[e] = vis & (1u << (8 * (e >> 2) + (e & 3))) ? s[e] : -INFINITY;
-          if (dirty) {
-            const uint32_t nan = vis & (dirty >> (4 * hf));
+        for (int e = 0; e < 16; e++) s[e] = tree_pick(vis, e, s[e], -INFINITY);
+        if (dirty) {
+          const uint32_t nan = vis & (dirty >> h4);
 #pragma unroll
-            for (int e = 0; e < 16; e++)
-              s[e] = nan & (1u << (8 * (e >> 2) + (e & 3))) ? NAN : s[e];
-          }
+          for (int e = 0; e < 16; e++) s[e] = tree_pick(nan, e, NAN, s[e]);
         }
-        float mt = fmaxf(s[0], s[1]);
+      };
+      // The running maximum follows mt where that exceeds it by far
+      auto follow = [&](bool first) {
+        const bool more = (mt - m_run) * p.sl > kTreeLazyMax;
+        up = __any(more);
+        if (up) {
+          const float m_new = more ? mt : m_run;
+          alpha = __builtin_amdgcn_exp2f((m_run - m_new) * p.sl);
+          m_run = m_new;
+          l_part *= alpha;
+          if (first) up = 0;  // O is zero
+        }
+        ml = m_run * p.sl;
+      };
+      if (active) {
+        kb = tree_addr(lds0 + ka0, 0);
+        tree_kfirst(kf, kb);
+        tree_qk(s, qf, kf, kb, [](auto) {});
+        mask(0);
+        hw_settle();
+        asm volatile("" : "+v"(s));
+        mt = fmaxf(s[0], s[1]);
 #pragma unroll
         for (int e = 2; e < 16; e++) mt = fmaxf(mt, s[e]);
         mt = xor32_max(mt);
-        const bool up = (mt - m_run) * p.sl > kTreeLazyMax;
-        if (__any(up)) {
-          const float m_new = up ? mt : m_run;
-          const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * p.sl);
-          const bool some = __any(m_run > -1e29f);  // O holds something
-          m_run = m_new;
-          l_part *= alpha;
-          if (some) {
-            hw_settle();
-            unroll<64>([&](auto i) { hw_scale<4 * i>(alpha); });
+        follow(seg_lo == t_lo * kTreeTile);
+        kb = tree_addr(lds0 + s1 + ka0, 0);
+        tree_kfirst(kf, kb);
+      }
+      if constexpr (FP8) lds_barrier();  // rope of tile 0 is done with
+      int row = row_of(FP8 ? 4 : 3);  // of tile i + 4, or i + 3
+      int rope_row = FP8 ? row_of(3) : 0;
+#pragma unroll 1
+      for (int i = 0; i < ntiles; i++) {
+        const bool more = i + 1 < ntiles;
+        // tile i + 1 is in, and every wave is done with tile i - 1, in whose place
+        // tile i + 3 goes
+        if (more && is_draft(i + 1)) dirty = tree_clean(sh.dirty, sh.ring[0] + s1, wave());
+        uint8_t* const raw = sh.raw[FP8 ? i & 1 : 0][FP8 ? w : 0];
+        // fp8: the wave's share of tile i + 2 has landed
+        if constexpr (FP8) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+        if (!active) {
+          const uint8_t* src = bytes_of(row);
+          if constexpr (FP8) {
+            const int ww = wave();
+            tree_dma_rope(bytes_of(rope_row), sh.ring[0] + s0, ww);
+            tree_convert_all(lds_at(raw), lds0 + s2, ww);
+            tree_dma_raw(src, raw, ww);
+            asm volatile("s_waitcnt vmcnt(11)" ::: "memory");
+          } else {
+            unroll<9>([&](auto k) { tree_dma1<k>(src, sh.ring[0] + s3 + dlds); });
+            asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
           }
+          rope_row = row;
+          row = row_of(i + (FP8 ? 5 : 4));
+          lds_barrier();
+        } else {
+          if (up) {
+            hw_settle();
+            unroll<64>([&](auto k) { hw_scale<4 * k>(alpha); });
+          }
+          f16x8 pb[2];
+          // stages of the exponential of element e
+          auto arg = [&](int e) { s[e] = __builtin_fmaf(s[e], p.sl, -ml); };
+          auto ex = [&](int e) { s[e] = __builtin_amdgcn_exp2f(s[e]); };
+          auto sum = [&](int e) {
+            l_part += s[e];
+            if (e & 1) {
+              const f16x2 h = {(f16)s[e - 1], (f16)s[e]};
+              pb[e >> 3][(e & 7) - 1] = h[0];
+              pb[e >> 3][e & 7] = h[1];
+            }
+          };
+          f32x16 sn;
+          TreeAddr vb;
+          const uint8_t* src;
+          TreeConv cv;
+          f32x2 sc;
+          u32x2 x[2];
+          f16x8 v;
+          auto side = [&](auto tc) {
+            constexpr int t = tc;
+            if constexpr (t == 1) {
+              src = bytes_of(row);
+              if constexpr (FP8) src += 256 * (w >> 1) + 16 * (tree_tid() & 3);
+            }
+            if constexpr (!FP8 && t % 4 == 3) tree_dma1<t / 4>(src, sh.ring[0] + s3 + dlds);
+            if constexpr (t % 2 == 0 && t / 2 < 16) arg(t / 2);
+            if constexpr (t >= 2 && t % 2 == 0 && t / 2 - 1 < 16) ex(t / 2 - 1);
+            if constexpr (t >= 5 && t % 2 == 1 && (t - 5) / 2 < 16) sum((t - 5) / 2);
+            if constexpr (t == 30) vb = tree_addr(lds0 + s0 + va0, 512);
+            if constexpr (t >= 36 - A) vf.x[t - 36 + A] = tree_vread(vb, t - 36 + A);
+            if constexpr (FP8) {  // a quarter of tile i + 2 is converted
+              if constexpr (t == 0) cv = tree_conv(lds_at(raw), lds0 + s2, w);
+              if constexpr (t == 2) sc = *(const lds_f32x2*)cv.sc;
+              if constexpr (t == 2) x[0] = tree_raw<0>(cv);
+              if constexpr (t == 4) x[1] = tree_raw<1>(cv);
+              if constexpr (t == 4) tree_dma_rope(bytes_of(rope_row), sh.ring[0] + s0, w);
+              if constexpr (t == 9) tree_convert<0, 0>(cv, x[0], sc, v);
+              if constexpr (t == 15) tree_convert<0, 1>(cv, x[0], sc, v);
+              if constexpr (t == 21) tree_convert<1, 0>(cv, x[1], sc, v);
+              if constexpr (t == 27) tree_convert<1, 1>(cv, x[1], sc, v);
+              if constexpr (t == 30) dma16_at<0>(src, raw);
+              if constexpr (t == 33)
+                dma4(src + kValueDim - 256 * (w >> 1) - 12 * (tree_tid() & 3), raw + 4096);
+            }
+          };
+          if (more) tree_qk(sn, qf, kf, kb, side);
+          else unroll<36>(side);
+          s = sn;
+          if (more) mask(i + 1);
+          float m2 = -INFINITY;
+          constexpr int kLast = 31 - A;  // the last V operand is read here
+          tree_pv(pb, vf, vb, [&](auto uc) {
+            constexpr int u = uc;
+            if constexpr (u == 3) asm volatile("" : "+v"(s));  // S is complete
+            if constexpr (u >= 4 && u < 12) m2 = fmaxf(fmaxf(m2, s[2 * (u - 4)]), s[2 * (u - 4) + 1]);
+            if constexpr (u == 13) mt = xor32_max(m2);
+            if constexpr (u == 14) {
+              up = 0;
+              if (more) follow(false);
+            }
+            if constexpr (FP8) {  // the rest of tile i + 2; tile i + 4 sets out
+              if constexpr (u < 24 && u % 2 == 1) {
+                constexpr int k = u / 2, I = 2 + k / 2;
+                tree_convert<I, k % 2>(cv, x[I % 2], sc, v);
+              }
+              if constexpr (u == 0) {
+                x[0] = tree_raw<2>(cv);
+                x[1] = tree_raw<3>(cv);
+              }
+              if constexpr (u >= 3 && u < 19 && u % 4 == 3) {
+                constexpr int I = 4 + u / 4;
+                x[I % 2] = tree_raw<I>(cv);
+              }
+              if constexpr (u == 8) dma16_at<64>(src, raw + 1024);
+              if constexpr (u == 16) dma16_at<128>(src, raw + 2048);
+              if constexpr (u == 24) dma16_at<192>(src, raw + 3072);
+            }
+            if constexpr (u == 20) row_begin(i + (FP8 ? 5 : 4));
+            if constexpr (u == 26) {
+              rope_row = row;
+              row = row_end();
+            }
+            if constexpr (u == kLast) {
+              // tile i + 2 is in (more may be in flight); no wave reads tile i any more
+              // after the barrier
+              if constexpr (FP8) asm volatile("s_waitcnt vmcnt(11)" ::: "memory");
+              else asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
+              lds_barrier();
+              kb = tree_addr(lds0 + s2 + ka0, 0);
+              tree_kfirst(kf, kb);
+            }
+          });
+          hw_own_agprs();
         }
-        l_part += tree_pv(s, p.sl, m_run * p.sl, slot, va0);
-        hw_own_agprs();
+        const int was = s0;
+        s0 = s1;
+        s1 = s2;
+        s2 = FP8 ? was : s3;
+        s3 = was;
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the DMA past the end too
     }
@@ -500,6 +828,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
     // ---- o and lse, or the piece's partial ----
     if (active) {
       const TreeParams p = tree_params();
+      const int w = wave();
+      int place = __builtin_amdgcn_readfirstlane(sh.run[w]);
+      if (!cells) place = 2 * place + (first ? 1 : 0);
+      const int lane = tree_tid() & 63, c = lane & 31, hf = lane >> 5;
       const float L = l_part + __shfl_xor(l_part, 32, 64);
       const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
       const int64_t row = (int64_t)it.first * p.H + m0 + c;
@@ -531,16 +863,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
           p.lse[row] = L > 0.f || L != L ? (m_run * p.sl + __log2f(L)) * 0.6931471805599453f
                                          : -INFINITY;
       } else {
-        float* part = tree_part(p, run, t_lo == 0, w);
+        float* part = tree_part(p, place);
         unroll<64>([&](auto uc) {
           constexpr int u = uc, i = 4 * u;
-          reinterpret_cast<f32x4*>(part)[64 * u + lane] =
+          reinterpret_cast<f32x4*>(part + w * kTreePartWave)[64 * u + lane] =
               (f32x4){hw_read<i>() * inv, hw_read<i + 1>() * inv, hw_read<i + 2>() * inv,
                       hw_read<i + 3>() * inv};
         });
         if (hf == 0) {
-          part[64 * 64 * 4 + c] = m_run * p.sl;
-          part[64 * 64 * 4 + 32 + c] = L;
+          part += p.part_waves * kTreePartWave;
+          part[32 * w + c] = m_run * p.sl;
+          part[32 * p.part_waves + 32 * w + c] = L;
         }
       }
     }
@@ -552,35 +885,62 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
 // o = sum w_i o_i / sum w_i, the pieces in the order of the keys.
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
   const int lane = threadIdx.x & 63;
-  const int unit = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6);  // (group, wave, dim tile)
+  const int unit = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6);  // (group, wave, tile of O^T)
   const int t = unit & 15, w = (unit >> 4) & 3;
   const int c = lane & 31, hf = lane >> 5;
-  const TreeItem it = tree_find(p, unit >> 6, true);
+  const TreePlan plan = {(int)p.plan[0], p.plan[1]};
+  const TreeItem it = tree_find(p, plan, unit >> 6, true);
   if (it.r < 0) return;
-  const int M = it.n * p.H, m0 = it.g * kTreeRows + 32 * w;
+  const int M = it.n * p.H, ro = 32 * w, m0 = it.g * kTreeRows + ro;
   if (m0 >= M) return;
-  const int64_t per = tree_per(tree_line(p));
-  const int w0 = (int)(it.start / per), w1 = (int)((it.start + it.tiles - 1) / per);
-  if (w0 == w1) return;  // not cut
+  // the pieces' partials: the first at k0, the others from k1 on, `step` apart
+  int64_t k0, k1;
+  int n, step;
+  if (plan.kt > 0) {
+    n = (it.tiles + it.cell - 1) / it.cell;
+    k0 = it.start;
+    step = it.step;
+    k1 = k0 + step;
+  } else {
+    const int64_t w0 = it.start / plan.per, w1 = (it.start + it.tiles - 1) / plan.per;
+    n = (int)(w1 - w0) + 1;
+    k0 = 2 * w0 + 1;
+    k1 = 2 * w0 + 2;
+    step = 2;
+  }
+  if (n == 1) return;  // not cut
   float m = -INFINITY, l = 0.f;
   f32x4 acc[4];
 #pragma unroll
   for (int a = 0; a < 4; a++) acc[a] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  for (int k = w0; k <= w1; k++) {
-    const float* part = tree_part(p, k, k == w0, w);
-    const float mi = part[64 * 64 * 4 + c], li = part[64 * 64 * 4 + 32 + c];
-    const bool some = li > 0.f || li != li;
-    const float mn = some ? fmaxf(m, mi) : m;
-    const float f = l > 0.f || l != l ? __builtin_amdgcn_exp2f(m - mn) : 0.f;
-    const float g = some ? __builtin_amdgcn_exp2f(mi - mn) * li : 0.f;
-    m = mn;
-    l = l * f + g;
+  // kMergeAt pieces at a time, their loads issued together
+  constexpr int kMergeAt = 4;
+  for (int i0 = 0; i0 < n; i0 += kMergeAt) {
+    float mi[kMergeAt], li[kMergeAt];
+    f32x4 x[kMergeAt][4];
 #pragma unroll
-    for (int a = 0; a < 4; a++) {
-      const f32x4 x = reinterpret_cast<const f32x4*>(part)[64 * (4 * t + a) + lane];
+    for (int i = 0; i < kMergeAt; i++) {
+      const int q = min(i0 + i, n - 1);
+      const float* part = tree_part(p, q == 0 ? k0 : k1 + (int64_t)(q - 1) * step);
+      const float* ml = part + p.part_waves * kTreePartWave + ro + c;
+      mi[i] = ml[0];
+      li[i] = i0 + i < n ? ml[32 * p.part_waves] : 0.f;
 #pragma unroll
-      for (int r = 0; r < 4; r++)
-        acc[a][r] = acc[a][r] * f + (some ? x[r] * g : 0.f);
+      for (int a = 0; a < 4; a++)
+        x[i][a] = reinterpret_cast<const f32x4*>(part + w * kTreePartWave)[64 * (4 * t + a) + lane];
+    }
+#pragma unroll
+    for (int i = 0; i < kMergeAt; i++) {
+      const bool some = li[i] > 0.f || li[i] != li[i];
+      const float mn = some ? fmaxf(m, mi[i]) : m;
+      const float f = l > 0.f || l != l ? __builtin_amdgcn_exp2f(m - mn) : 0.f;
+      const float g = some ? __builtin_amdgcn_exp2f(mi[i] - mn) * li[i] : 0.f;
+      m = mn;
+      l = l * f + g;
+#pragma unroll
+      for (int a = 0; a < 4; a++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) acc[a][r] = acc[a][r] * f + (some ? x[i][a][r] * g : 0.f);
     }
   }
   if (m0 + c >= M) return;
@@ -612,7 +972,7 @@ using namespace mi355dsa;
 
 extern "C" size_t mi355_dsa_mla_tree_workspace_size(int64_t n_tok, int n_head) {
   if (n_tok <= 0 || n_head <= 0) return 0;
-  return (size_t)2 * kTreeWGs * tree_part_waves(n_tok, n_head) * kTreePartWave * sizeof(float);
+  return (size_t)2 * kTreeWGs * tree_part_waves(n_tok, n_head) * (kTreePartWave + 64) * sizeof(float) + 16;
 }
 
 extern "C" int mi355_dsa_mla_tree_attention(
@@ -649,20 +1009,26 @@ extern "C" int mi355_dsa_mla_tree_attention(
   p.lse = lse;
   p.part = reinterpret_cast<float*>(workspace);
   p.part_waves = tree_part_waves(n_tok, n_head);
+  p.plan = reinterpret_cast<int64_t*>(p.part + (size_t)2 * kTreeWGs * p.part_waves * (kTreePartWave + 64));
   p.R = n_req;
   p.T = (int)n_tok;
   p.H = n_head;
   p.max_blocks = max_blocks;
   p.page_size = page_size;
-  p.page_shift = (page_size & (page_size - 1)) == 0 ? ilog2_pow2(page_size) : -1;
+  // ceil(2^(31 + k) / page_size) with 2^k >= page_size > 2^(k - 1): the product of a
+  // position below 2^31 exceeds the quotient by less than 2^-31 of a position's share
+  const int k = ilog2_pow2(page_size);
+  p.page_shift = 31 + k;
+  p.page_mul = (uint32_t)((((uint64_t)1 << (31 + k)) + page_size - 1) / page_size);
   p.n_kv_rows = n_kv_rows;
   p.sl = (scale == 0.f ? 1.f : fabsf(scale)) * 1.4426950408889634f;
   p.q_sign = scale == 0.f ? 0.f : scale < 0.f ? -1.f : 1.f;
   hipStream_t st = as_stream(stream);
   auto kern = kv_fp8 ? mla_tree_kernel<true> : mla_tree_kernel<false>;
-  int rc = reserve_lds(reinterpret_cast<const void*>(kern), sizeof(TreeSmem), "mla_tree");
+  const size_t lds = kv_fp8 ? sizeof(TreeSmem<true>) : sizeof(TreeSmem<false>);
+  int rc = reserve_lds(reinterpret_cast<const void*>(kern), lds, "mla_tree");
   if (rc != MI355_DSA_OK) return rc;
-  kern<<<kTreeWGs, kTreeThreads, sizeof(TreeSmem), st>>>(p);
+  kern<<<kTreeWGs, kTreeThreads, lds, st>>>(p);
   DSA_LAUNCH_CHECK("mla_tree");
   const int64_t units = tree_max_groups(n_tok, n_head, n_req) * 64;
   tree_merge_kernel<<<dim3((unsigned)(units / 4)), 256, 0, st>>>(p);
