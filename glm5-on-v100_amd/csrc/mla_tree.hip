@@ -99,7 +99,9 @@ struct TreeSmem {
   int32_t blk[kTreePages];      // cache blocks of the segment, -1: none
   uint32_t dirty[kTreeWaves];
   int gap;  // some block of the segment is missing
-  int run[kTreeWaves];  // the workgroup's, parked over the loops
+  // of each wave, over the loops: first row, rows and group of the request, place of
+  // its partial (-1: o is written)
+  u32x4 item[kTreeWaves];
 };
 static_assert(sizeof(TreeSmem<false>) <= 160 * 1024 && sizeof(TreeSmem<true>) <= 160 * 1024,
               "one workgroup per CU");
@@ -149,11 +151,12 @@ __device__ __forceinline__ int64_t shfl64(int64_t v, int src) {
   return ((int64_t)__builtin_amdgcn_readlane((int)(v >> 32), src) << 32) |
          (uint32_t)__builtin_amdgcn_readlane((int)v, src);
 }
-// inclusive sums over the lanes
-__device__ __forceinline__ int64_t scan64(int64_t v) {
+// inclusive sums over the lanes, of which the first n hold something
+__device__ __forceinline__ int64_t scan64(int64_t v, int n) {
   const int lane = tree_tid() & 63;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
+    if (m >= n) break;
     const int64_t u = __shfl_up(v, m, 64);
     if (lane >= m) v += u;
   }
@@ -175,7 +178,7 @@ __device__ __forceinline__ TreePlan tree_plan(const TreeParams& p) {
   int64_t line = 0;
   for (int r0 = 0; r0 < p.R; r0 += 64) {
     const TreeReq q = tree_req(p, r0 + lane);
-    line += shfl64(scan64((int64_t)q.groups * q.tiles), 63);
+    line += shfl64(scan64((int64_t)q.groups * q.tiles, p.R - r0), min(p.R - r0, 64) - 1);
   }
   TreePlan pl;
   pl.per = max((int64_t)kTreeMinTiles, (line + kTreeWGs - 1) / kTreeWGs);
@@ -187,7 +190,7 @@ __device__ __forceinline__ TreePlan tree_plan(const TreeParams& p) {
     for (int r0 = 0; r0 < p.R; r0 += 64) {
       const TreeReq q = tree_req(p, r0 + lane);
       const int n = kt >= q.tiles ? 1 : (q.tiles + (int)kt - 1) / (int)kt;
-      units += shfl64(scan64((int64_t)q.groups * n), 63);
+      units += shfl64(scan64((int64_t)q.groups * n, p.R - r0), min(p.R - r0, 64) - 1);
     }
     if (units <= kTreeWGs) {
       pl.kt = (int)min(kt, (int64_t)INT32_MAX);
@@ -224,9 +227,9 @@ __device__ __forceinline__ TreeItem tree_find(const TreeParams& p, const TreePla
     }
     const int64_t cost = (int64_t)q.groups * (pl.kt > 0 ? n : q.tiles);  // units, or tiles
     const int64_t size = by_group ? q.groups : cost;
-    const int64_t incl = base + scan64(size);
+    const int64_t incl = base + scan64(size, p.R - r0);
     const uint64_t hit = __ballot(at < incl && size > 0);
-    const int64_t lsum = line + scan64(cost);
+    const int64_t lsum = line + scan64(cost, p.R - r0);
     if (hit) {
       const int k = __builtin_ctzll(hit);
       it.r = r0 + k;
@@ -282,7 +285,7 @@ __device__ __forceinline__ void tree_dma_raw(const uint8_t* row, uint8_t* raw, i
   dma16_at<0>(src, raw);
   dma16_at<64>(src, raw + 1024);
   dma16_at<128>(src, raw + 2048);
-  dma16_at<192>(src, raw + 3072);
+  dma16_at<192>(src, raw + 3 * 1024);
   dma4(row + kValueDim + 4 * (l & 3), raw + 4096);
 }
 // Addresses of a conversion.  In a tile quad q holds blocks 2 q and 2 q + 1; lane j of
@@ -472,7 +475,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
 
   // neighbouring runs on one XCD (workgroups go round the eight of them)
   const int run = (int)(blockIdx.x & 7) * (kTreeWGs / 8) + (int)(blockIdx.x >> 3);
-  sh.run[w] = run;
   TreePlan plan = tree_plan(p);
   if (run == 0 && threadIdx.x == 0) {  // for the merge
     p.plan[0] = plan.kt;
@@ -515,8 +517,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
     const bool cells = plan.kt > 0;
     const int t_lo = cells ? it.part * it.cell : (int)(at - it.start);
     const int t_hi = (int)min((int64_t)it.tiles, (int64_t)t_lo + (cells ? it.cell : left));
-    const bool whole = t_lo == 0 && t_hi == it.tiles;
-    const bool first = t_lo == 0;
+    {
+      const bool whole = t_lo == 0 && t_hi == it.tiles;
+      const int place = whole ? -1 : cells ? run : 2 * run + (t_lo == 0 ? 1 : 0);
+      sh.item[w] = (u32x4){(uint32_t)it.first, (uint32_t)M, (uint32_t)it.g, (uint32_t)place};
+    }
     at += t_hi - t_lo;
     left = cells ? 0 : left - (t_hi - t_lo);
     const int k_hi = min(t_hi * kTreeTile, it.len);
@@ -797,7 +802,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
               }
               if constexpr (u == 8) dma16_at<64>(src, raw + 1024);
               if constexpr (u == 16) dma16_at<128>(src, raw + 2048);
-              if constexpr (u == 24) dma16_at<192>(src, raw + 3072);
+              if constexpr (u == 24) dma16_at<192>(src, raw + 3 * 1024);
             }
             if constexpr (u == 20) row_begin(i + (FP8 ? 5 : 4));
             if constexpr (u == 26) {
@@ -829,12 +834,16 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
     if (active) {
       const TreeParams p = tree_params();
       const int w = wave();
-      int place = __builtin_amdgcn_readfirstlane(sh.run[w]);
-      if (!cells) place = 2 * place + (first ? 1 : 0);
+      const u32x4 item = sh.item[w];
+      const int first = __builtin_amdgcn_readfirstlane((int)item[0]);
+      const int M = __builtin_amdgcn_readfirstlane((int)item[1]);
+      const int m0 = __builtin_amdgcn_readfirstlane((int)item[2]) * kTreeRows + 32 * w;
+      const int place = __builtin_amdgcn_readfirstlane((int)item[3]);
+      const bool whole = place < 0;
       const int lane = tree_tid() & 63, c = lane & 31, hf = lane >> 5;
       const float L = l_part + __shfl_xor(l_part, 32, 64);
       const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-      const int64_t row = (int64_t)it.first * p.H + m0 + c;
+      const int64_t row = (int64_t)first * p.H + m0 + c;
       hw_settle();
       if (whole) {
         const bool mine = m0 + c < M;
