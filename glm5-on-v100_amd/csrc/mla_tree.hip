@@ -648,7 +648,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
       int up = 0;           // O has to be scaled
       TreeFrag<A> kf, vf;
       TreeAddr kb;
-      auto mask = [&](int tile) {
+      auto mask = [&](f32x16& s, int tile) {
         const bool draft = is_draft(tile);
         if (!gaps && !draft && (tile + 1) * kTreeTile <= keys) return;
         hw_settle();
@@ -683,7 +683,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
         kb = tree_addr(lds0 + ka0, 0);
         tree_kfirst(kf, kb);
         tree_qk(s, qf, kf, kb, [](auto) {});
-        mask(0);
+        mask(s, 0);
         hw_settle();
         asm volatile("" : "+v"(s));
         mt = fmaxf(s[0], s[1]);
@@ -694,7 +694,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
         kb = tree_addr(lds0 + s1 + ka0, 0);
         tree_kfirst(kf, kb);
       }
-      if constexpr (FP8) lds_barrier();  // rope of tile 0 is done with
+      lds_barrier();  // rope of tile 0 and the flags of its cleaning are done with
       int row = row_of(FP8 ? 4 : 3);  // of tile i + 4, or i + 3
       int rope_row = FP8 ? row_of(3) : 0;
 #pragma unroll 1
@@ -774,14 +774,16 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
           };
           if (more) tree_qk(sn, qf, kf, kb, side);
           else unroll<36>(side);
-          s = sn;
-          if (more) mask(i + 1);
+          if (more) mask(sn, i + 1);
           float m2 = -INFINITY;
           constexpr int kLast = 31 - A;  // the last V operand is read here
           tree_pv(pb, vf, vb, [&](auto uc) {
             constexpr int u = uc;
-            if constexpr (u == 3) asm volatile("" : "+v"(s));  // S is complete
-            if constexpr (u >= 4 && u < 12) m2 = fmaxf(fmaxf(m2, s[2 * (u - 4)]), s[2 * (u - 4) + 1]);
+            // S is complete: the MFMAs since hide its last ones.  No use above this.
+            if constexpr (u == 3) asm volatile("" : "+v"(sn));
+            if constexpr (u >= 4 && u < 12)
+              m2 = fmaxf(fmaxf(m2, sn[2 * (u - 4)]), sn[2 * (u - 4) + 1]);
+            if constexpr (u == 15) s = sn;
             if constexpr (u == 13) mt = xor32_max(m2);
             if constexpr (u == 14) {
               up = 0;
