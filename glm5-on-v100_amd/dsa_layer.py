@@ -39,6 +39,13 @@ reach), which on a 64k causal prefill takes the logits from 36 % to 45 % of
 the fp16 MFMA peak (fewer, fuller launches; 2048 is level, larger is slower
 once the buffer leaves the 256 MB MALL).
 
+Verification of drafted trees (verify_tree) takes the step's tensors as the
+projections leave them, not yet rotated, and attends densely, as the few rows of
+a draft and their request's whole context are one matrix product for all heads:
+rotary positions of q and k_pe with the latent rows written in the same launch
+(rope_concat_and_cache_mla), the indexer's key rotated and stored, step 3, tree
+attention, step 5.
+
 All buffers come from torch's caching allocator; nothing here synchronises
 the host except the per-sub-chunk causal reach, which the reference also reads
 on the host (memoized per chunk, :774-789) and which callers can pass in.
@@ -49,7 +56,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import _cache_ops, _lib, _sm70_ops
+from . import _cache_ops, _lib, _sm70_ops, mla_tree, rope
 from .ops import _check, _stream
 
 KT = 64  # key tile the prefill logits launch is rounded to (sparse_attn_indexer.py:753)
@@ -383,6 +390,51 @@ class DsaLayer:
                       int(slot.dtype == torch.int64), ikc.data_ptr(), int(ik_fp8), ik_rows,
                       ik.data_ptr(), islot.data_ptr(), hist.data_ptr(), hist.numel(), _stream(q))
         return ql, hist
+
+    # -- verification of drafted trees --------------------------------------
+    def verify_tree(self, q: torch.Tensor, kv_c: torch.Tensor, k_pe: torch.Tensor,
+                    positions: torch.Tensor, table: torch.Tensor, slot_mapping: torch.Tensor,
+                    block_table: torch.Tensor, seq_lens: torch.Tensor,
+                    cu_seqlens_q: torch.Tensor, tree_mask: torch.Tensor,
+                    idx_k: torch.Tensor | None = None,
+                    interleaved: bool = True) -> torch.Tensor:
+        """Every request's tree of drafted tokens in one step.  q [T, H, P + 64] fp16,
+        kv_c [T, 512] and k_pe [T, 64], not rotated; positions [T] are the tokens'
+        places in the text (context length + depth in the tree, mla_tree.tree_masks),
+        table their rotary table.  slot_mapping [T] (< 0: not written) names the rows of
+        the cache positions seq_lens[r] - n .. seq_lens[r] - 1 in the order of the
+        request's n tokens, cu_seqlens_q[r] .. cu_seqlens_q[r + 1] - 1; tree_mask as in
+        mla_tree.tree_attention.  idx_k [T, 128], if given, is rotated over its first 64
+        dims (half layout) and written to the indexer cache.  q, k_pe and idx_k stay as
+        they are.  Returns out [T, H * V], zero for tokens of no request."""
+        T = slot_mapping.numel()
+        _check(q.dim() == 3 and q.shape == (T, self.w.n_heads, self.w.nope_dim + 64),
+               "q must be [T, H, P + 64], a slot for each token")
+        _check(q.dtype == torch.float16, "q must be fp16")
+        _check(positions.shape == (T,), "positions must be [T]")
+        fused = kv_c.dtype == torch.float16  # else (bf16) q is rotated in a launch of its own
+        qr = _cache_ops.rope_concat_and_cache_mla(
+            positions, table, kv_c, k_pe, self.latent_cache, slot_mapping, self.kv_dtype,
+            interleaved, q if fused else None, self.w.nope_dim)
+        rest = [] if fused else [q]
+        if idx_k is not None:
+            _check(idx_k.shape == (T, 128), "idx_k must be [T, 128]")
+            rest.append(idx_k)
+        if rest:
+            done = rope.apply_rotary(rest, positions, table,
+                                     ([] if fused else [self.w.nope_dim]) + [0] * (idx_k is not None),
+                                     ([] if fused else [interleaved]) + [False] * (idx_k is not None))
+            if not fused:
+                qr = done[0]
+            if idx_k is not None:
+                self.store_index_key(done[-1], slot_mapping)
+        H = self.w.n_heads
+        o = torch.zeros(T, H, 512, dtype=torch.float16, device=q.device)
+        lse = torch.full((T, H), float("-inf"), dtype=torch.float32, device=q.device)
+        mla_tree.tree_attention(q_latent(qr, self.w), self.latent_cache, block_table, seq_lens,
+                                cu_seqlens_q, tree_mask, self.w.scale, o, lse)
+        self.last_idx, self.last_o, self.last_lse = None, o, lse
+        return v_up(o, self.w)
 
     # -- prefill ------------------------------------------------------------
     def prefill_topk(self, idx_q: torch.Tensor, idx_w: torch.Tensor, bounds: list[int],
