@@ -197,7 +197,9 @@ __device__ __forceinline__ TreePlan tree_plan(const TreeParams& p) {
       break;
     }
     if (kt >= most) break;
-    kt = min(most, kt + max((int64_t)1, kt * (min(units, (int64_t)2 * kTreeWGs) - kTreeWGs) / (2 * kTreeWGs)));
+    // by what the count is over, an eighth of the way at least: few steps
+    const int64_t over = kt * (min(units, (int64_t)2 * kTreeWGs) - kTreeWGs) / (2 * kTreeWGs);
+    kt = min(most, kt + max(max((int64_t)1, (most - pl.per) / 8), over));
   }
   return pl;
 }
