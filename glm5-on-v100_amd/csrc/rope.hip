@@ -9,10 +9,11 @@
 
 namespace mi355dsa {
 
+template <bool PIECES>
 __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
   int k = 0;
   while (k + 1 < a.n_parts && (int)blockIdx.x >= a.first[k + 1]) k++;
-  rotary_block(a, a.part[k], (int)blockIdx.x - a.first[k]);
+  rotary_block<PIECES>(a, a.part[k], (int)blockIdx.x - a.first[k]);
 }
 
 // The rope piece of lane l (lanes 8 apart hold the same one), rotated.
@@ -42,10 +43,10 @@ struct RopeCacheArgs {
 };
 
 // Workgroups [0, kv_blocks): the cache rows, one wave a token; the others q.
-template <bool FP8, bool BF16>
+template <bool FP8, bool BF16, bool PIECES>
 __global__ void __launch_bounds__(256) rope_concat_cache_mla_kernel(RopeCacheArgs a) {
   if ((int)blockIdx.x >= a.kv_blocks) {
-    rotary_block_t<BF16 ? 1 : 0>(a.rot, a.rot.part[0], (int)blockIdx.x - a.kv_blocks);
+    rotary_block_t<BF16 ? 1 : 0, PIECES>(a.rot, a.rot.part[0], (int)blockIdx.x - a.kv_blocks);
     return;
   }
   const int lane = threadIdx.x & 63;
@@ -310,7 +311,10 @@ extern "C" int mi355_dsa_rotary(const mi355_dsa_rotary_part* parts, int n_parts,
   }
   a.n_parts = n_parts;
   a.first[n_parts] = (int)n;
-  rotary_kernel<<<dim3((unsigned)n), 256, 0, as_stream(stream)>>>(a);
+  bool pieces = true;
+  for (int i = 0; i < n_parts; i++) pieces &= a.part[i].vec != 0;
+  auto kern = pieces ? rotary_kernel<true> : rotary_kernel<false>;
+  kern<<<dim3((unsigned)n), 256, 0, as_stream(stream)>>>(a);
   DSA_LAUNCH_CHECK("rotary");
   return MI355_DSA_OK;
 }
@@ -356,9 +360,14 @@ extern "C" int mi355_dsa_rope_concat_and_cache_mla(
   a.kv_blocks = (int)kv_blocks;
   const dim3 grid((unsigned)(kv_blocks + q_blocks));
   hipStream_t st = as_stream(stream);
-  if (!kv_fp8) rope_concat_cache_mla_kernel<false, false><<<grid, 256, 0, st>>>(a);
-  else if (in_bf16) rope_concat_cache_mla_kernel<true, true><<<grid, 256, 0, st>>>(a);
-  else rope_concat_cache_mla_kernel<true, false><<<grid, 256, 0, st>>>(a);
+  const bool pieces = a.rot.n_parts == 0 || a.rot.part[0].vec;
+  auto kern = !kv_fp8  ? pieces ? rope_concat_cache_mla_kernel<false, false, true>
+                                : rope_concat_cache_mla_kernel<false, false, false>
+              : in_bf16 ? pieces ? rope_concat_cache_mla_kernel<true, true, true>
+                                 : rope_concat_cache_mla_kernel<true, true, false>
+              : pieces  ? rope_concat_cache_mla_kernel<true, false, true>
+                        : rope_concat_cache_mla_kernel<true, false, false>;
+  kern<<<grid, 256, 0, st>>>(a);
   DSA_LAUNCH_CHECK(what);
   return MI355_DSA_OK;
 }
