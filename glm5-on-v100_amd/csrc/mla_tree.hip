@@ -1001,7 +1001,10 @@ extern "C" int mi355_dsa_mla_tree_attention(
   DSA_CHECK((int64_t)max_blocks * page_size < ((int64_t)1 << 30), "mla_tree: block table too wide");
   DSA_CHECK(isfinite(scale), "mla_tree: scale must be finite");
   if (n_tok == 0 || n_req == 0) return MI355_DSA_OK;
-  DSA_CHECK(n_tok * n_head < ((int64_t)1 << 30), "mla_tree: too many rows");
+  DSA_CHECK(n_tok < ((int64_t)1 << 30) && n_tok * n_head < ((int64_t)1 << 30),
+            "mla_tree: too many rows");
+  const int64_t units = tree_max_groups(n_tok, n_head, n_req) * 64;  // of the merge
+  DSA_CHECK(units <= INT32_MAX, "mla_tree: too many rows");
   DSA_CHECK(o && lse && q && kv_cache && seq_lens && cu_seqlens_q && tree_mask &&
                 (block_table || max_blocks == 0),
             "null pointer argument");
@@ -1043,7 +1046,6 @@ extern "C" int mi355_dsa_mla_tree_attention(
   if (rc != MI355_DSA_OK) return rc;
   kern<<<kTreeWGs, kTreeThreads, lds, st>>>(p);
   DSA_LAUNCH_CHECK("mla_tree");
-  const int64_t units = tree_max_groups(n_tok, n_head, n_req) * 64;
   tree_merge_kernel<<<dim3((unsigned)(units / 4)), 256, 0, st>>>(p);
   DSA_LAUNCH_CHECK("mla_tree merge");
   return MI355_DSA_OK;

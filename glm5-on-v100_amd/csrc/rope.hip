@@ -212,6 +212,8 @@ __global__ void __launch_bounds__(256) gather_latent_kernel(GatherArgs a) {
   }
 }
 
+constexpr int64_t kMaxTokens = (int64_t)1 << 40;  // the grids' sizes are computed in 64 bits
+
 // Fills the kernel's form of a caller's part; the number of its workgroups in
 // *blocks.  `what` names the entry point.
 static int rotary_part(const mi355_dsa_rotary_part& s, int rot, int64_t n_tok, const char* what,
@@ -295,6 +297,7 @@ extern "C" int mi355_dsa_rotary(const mi355_dsa_rotary_part* parts, int n_parts,
   DSA_CHECK(n_parts >= 0 && n_parts <= kRotaryParts, "rotary: 0 to %d tensors, got %d", kRotaryParts,
             n_parts);
   DSA_CHECK(n_tok >= 0, "rotary: n_tok must be >= 0");
+  DSA_CHECK(n_tok <= kMaxTokens, "rotary: too many tokens");
   if (n_tok == 0 || n_parts == 0) return MI355_DSA_OK;
   DSA_CHECK(parts, "rotary: null pointer argument");
   RotaryArgs a{};
@@ -327,6 +330,7 @@ extern "C" int mi355_dsa_rope_concat_and_cache_mla(
   clear_error();
   const char* what = "rope_concat_and_cache_mla";
   DSA_CHECK(n_tok >= 0 && n_rows >= 0, "n_tok and n_rows must be >= 0");
+  DSA_CHECK(n_tok <= kMaxTokens, "%s: too many tokens", what);
   if (n_tok == 0) return MI355_DSA_OK;
   DSA_CHECK(kv_cache && kv_c && k_pe && slot_mapping, "null pointer argument");
   DSA_CHECK(aligned_to(kv_cache, 16) && aligned_to(kv_c, 16) && aligned_to(k_pe, 16),
@@ -380,6 +384,7 @@ extern "C" int mi355_dsa_gather_latent_cache(void* out, int64_t out_stride, int 
                                              int n_req, void* stream) {
   clear_error();
   DSA_CHECK(total >= 0 && n_rows >= 0 && max_blocks >= 0 && n_req >= 0, "gather_latent_cache: bad sizes");
+  DSA_CHECK(total <= kMaxTokens, "gather_latent_cache: too many rows");
   DSA_CHECK(page_size > 0, "page size must be > 0");
   DSA_CHECK(out_dtype >= 0 && out_dtype <= 2,
             "gather_latent_cache: dtype must be 0 (fp16), 1 (bf16) or 2 (fp32)");
