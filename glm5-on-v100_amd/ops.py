@@ -78,6 +78,9 @@ def _stream(t: torch.Tensor) -> int:
 
 
 _current_device = torch.cuda.current_device
+# the handle alone: building the Stream object around it takes 1 us
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 def _launch(name: str, dev: torch.device, *args) -> None:
@@ -85,7 +88,7 @@ def _launch(name: str, dev: torch.device, *args) -> None:
     device made current where it is not: entering torch.cuda.device costs more than
     the check (3 of the 25 us of a short call)."""
     i = dev.index
-    stream = torch.cuda.current_stream(i).cuda_stream
+    stream = _raw_stream(i)
     if i == _current_device():
         _lib.call(name, *args, stream)
     else:
