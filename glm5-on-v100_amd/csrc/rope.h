@@ -196,7 +196,8 @@ __device__ __forceinline__ void rotary_unit(const RotaryPart& p, int rot, const 
 // Items i, i + 256, .. below hi of a token without pieces: one pair, or one plain
 // element, each.  Four at a time, their loads before their stores (items do not share
 // elements), so that a wave waits for memory once and not for each of them (1537
-// tokens x 17 heads of 100 fp32, 21 MB: 11.3 -> 9.2 us; 4.2 us at the copy rate).
+// tokens x 17 heads of 100 fp32, 21 MB: 11.3 -> 9.2 us, 8.6 in a graph; 4.2 at the
+// rate of a copy).
 template <int DT>
 __device__ __forceinline__ void rotary_single(const RotaryPart& p, int rot, const float* row,
                                               const uint8_t* x, uint8_t* out, int i, int hi) {
