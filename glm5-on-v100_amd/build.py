@@ -76,6 +76,78 @@ def _usage(asm: str, symbol: str, key: str) -> int:
     raise RuntimeError(f"{symbol}: no metadata")
 
 
+def _registers(text: str) -> set[str]:
+    """The vector and accumulation registers that operands name."""
+    found = set()
+    for bank, lo, hi in re.findall(r"\b([av])\[(\w+):(\w+)\]", text):
+        found |= {f"{bank}{i}" for i in range(int(lo, 0), int(hi, 0) + 1)}
+    return found | set(re.findall(r"\b[av]\d+\b", text))
+
+
+# Wait states, as in the instruction set's table of required software waits: of an
+# MFMA's result before anything but an accumulating MFMA touches it (the longest
+# case, 16 passes), and of a vector result before an MFMA reads it.
+_MFMA_TO_USE, _VALU_TO_MFMA = 19, 2
+
+
+def check_waits(lines: list[str], kernel: str) -> None:
+    """Raises if, on any path, an instruction follows an MFMA or an MFMA a vector
+    instruction too closely for the registers they share.  The compiler adds these waits
+    only for MFMAs that it placed itself, not for those of inline asm."""
+    code, label = [], {}
+    for line in lines:
+        text = line.split(";")[0].strip()
+        if re.fullmatch(r"\.LBB\w+:", text):
+            label[text[:-1]] = len(code)
+        elif text and not text.startswith(".") and not text.endswith(":"):
+            code.append(text)
+
+    def operands(i):
+        return [x.strip() for x in code[i].partition(" ")[2].split(",")]
+
+    def follow(start, states, visit):
+        """visit(i) for the instructions within `states` wait states; True ends a path."""
+        paths, seen = [(start, states)], {}
+        while paths:
+            i, left = paths.pop()
+            while left > 0 and i < len(code) and seen.get(i, 0) < left:
+                seen[i] = left
+                text = code[i]
+                if visit(i) or text.startswith("s_endpgm"):
+                    break
+                # an MFMA waits for the one before it, 8 passes
+                left -= int(text.split()[1]) + 1 if text.startswith("s_nop") else \
+                    8 if text.startswith("v_mfma") else 1
+                to = re.match(r"s_c?branch\w*\s+(\.LBB\w+)", text)
+                if to:
+                    paths.append((label[to.group(1)], left))
+                    if text.startswith("s_branch"):
+                        break
+                i += 1
+
+    for i, text in enumerate(code):
+        if not text.startswith("v_") or " " not in text:
+            continue
+        result, mfma = _registers(operands(i)[0]), text.startswith("v_mfma")
+
+        def after_mfma(k):
+            if code[k].startswith("v_mfma"):
+                d, a, b = operands(k)[:3]
+                if _registers(f"{a} {b}") & result:
+                    raise RuntimeError(f"{kernel}: no wait between {text} and {code[k]}")
+                return bool(_registers(d) & result)  # accumulated, or a new result
+            if _registers(code[k]) & result:
+                raise RuntimeError(f"{kernel}: no wait between {text} and {code[k]}")
+            return False
+
+        def after_valu(k):
+            if code[k].startswith("v_mfma") and _registers(" ".join(operands(k)[1:])) & result:
+                raise RuntimeError(f"{kernel}: no wait between {text} and {code[k]}")
+            return False
+
+        follow(i + 1, _MFMA_TO_USE if mfma else _VALU_TO_MFMA, after_mfma if mfma else after_valu)
+
+
 def check_kernels(asm: str, own_agprs: list[str], no_spills: list[str] = []) -> None:
     """Raises unless no kernel of either list spills or uses scratch memory, and
     every kernel of `own_agprs` is as its inline asm needs it: at most 256 other
@@ -113,7 +185,10 @@ def _compile(src: str) -> str:
         raise RuntimeError(f"hipcc failed for {src}:\n{r.stdout}\n{r.stderr}")
     if checked:
         with open(asm_path(name)) as f:
-            check_kernels(f.read(), OWN_AGPRS.get(name, []), NO_SPILLS.get(name, []))
+            asm = f.read()
+        check_kernels(asm, OWN_AGPRS.get(name, []), NO_SPILLS.get(name, []))
+        for kernel in OWN_AGPRS.get(name, []):
+            check_waits(_body(asm, kernel)[1], kernel)
     return obj
 
 
