@@ -61,7 +61,9 @@ __host__ __device__ constexpr int tree_slots(bool fp8) { return fp8 ? 3 : 4; }
 constexpr int kTreePages = 2048;    // block-table entries resolved at a time
 constexpr int kTreeMaxDraft = 64;   // tokens of a request that a mask can name
 constexpr int kTreeWGs = 256;       // runs of the line: one workgroup per CU
-constexpr int kTreeMinTiles = 2;    // tiles of a run at least
+// Tiles of a run at least.  us of 4 tokens x 16 heads for 2, 3, 4: 500 keys 20.4 / 20.2 /
+// 22.4, 8000 30.9 / 29.1 / 28.7; of 8 x 64 over 500: 28.4 / 26.5 / 27.2.
+constexpr int kTreeMinTiles = 3;
 constexpr int kTreeBlocks = kLatentDim / 32;                   // 64-byte blocks of an fp16 row
 constexpr int kTreeSlotBytes = kTreeBlocks * kTreeTile * 64;   // 36864
 // fp8 rows as they are, on their way: bytes of a wave's share of a tile (twice)
@@ -69,6 +71,10 @@ constexpr int kTreeRaw = 64 * 64 + 256;
 // LDS reads ahead of their MFMA; fp8 rows leave no registers for a third
 __host__ __device__ constexpr int tree_ahead(bool fp8) { return fp8 ? 2 : 3; }
 constexpr float kTreeLazyMax = 8.f; // log2 that scores may exceed the running maximum by
+// Units of the merge (64 a group) up to which 8 waves share one.  us with a wave and with
+// 8 a unit: 1 group over 8000 keys 50 / 29, over 180000 107 / 65; 8 groups 378 / 379; 32
+// groups with 8 pieces each 176 / 188.
+constexpr int kTreeMergeUnits = 16 * 64;
 constexpr int kTreePartWave = 64 * 64 * 4;  // floats of a wave's O^T in a partial
 
 struct TreeParams {
@@ -895,10 +901,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
 
 // Joins the pieces of the groups that runs cut: wave = 32 rows of a group x 32
 // dims, in the partials' own order.  m = max m_i (log2 units), w_i = 2^(m_i - m) l_i,
-// o = sum w_i o_i / sum w_i, the pieces in the order of the keys.
-__global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
-  const int lane = threadIdx.x & 63;
-  const int unit = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6);  // (group, wave, tile of O^T)
+// o = sum w_i o_i / sum w_i, the pieces in the order of the keys.  S waves of a
+// workgroup share the pieces of a unit: a lone group has up to 256 of them, one after
+// the other a memory latency for every four.
+template <int S>
+__global__ void __launch_bounds__(S == 1 ? 256 : 64 * S) tree_merge_kernel(TreeParams p) {
+  static_assert(S == 1 || S == 8, "each of 8 waves writes 2 of the lane's 16 values");
+  __shared__ float part_acc[S == 1 ? 1 : S][16][64], part_m[S == 1 ? 1 : S][64], part_l[S == 1 ? 1 : S][64];
+  const int lane = threadIdx.x & 63, wv = (int)(threadIdx.x >> 6);
+  const int unit = S == 1 ? (int)blockIdx.x * 4 + wv : (int)blockIdx.x;  // (group, wave, tile of O^T)
   const int t = unit & 15, w = (unit >> 4) & 3;
   const int c = lane & 31, hf = lane >> 5;
   const TreePlan plan = {(int)p.plan[0], p.plan[1]};
@@ -928,16 +939,17 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
   for (int a = 0; a < 4; a++) acc[a] = (f32x4){0.f, 0.f, 0.f, 0.f};
   // kMergeAt pieces at a time, their loads issued together
   constexpr int kMergeAt = 4;
-  for (int i0 = 0; i0 < n; i0 += kMergeAt) {
+  const int lo = S == 1 ? 0 : n * wv / S, hi = S == 1 ? n : n * (wv + 1) / S;
+  for (int i0 = lo; i0 < hi; i0 += kMergeAt) {
     float mi[kMergeAt], li[kMergeAt];
     f32x4 x[kMergeAt][4];
 #pragma unroll
     for (int i = 0; i < kMergeAt; i++) {
-      const int q = min(i0 + i, n - 1);
+      const int q = min(i0 + i, hi - 1);
       const float* part = tree_part(p, q == 0 ? k0 : k1 + (int64_t)(q - 1) * step);
       const float* ml = part + p.part_waves * kTreePartWave + ro + c;
       mi[i] = ml[0];
-      li[i] = i0 + i < n ? ml[32 * p.part_waves] : 0.f;
+      li[i] = i0 + i < hi ? ml[32 * p.part_waves] : 0.f;
 #pragma unroll
       for (int a = 0; a < 4; a++)
         x[i][a] = reinterpret_cast<const f32x4*>(part + w * kTreePartWave)[64 * (4 * t + a) + lane];
@@ -956,9 +968,38 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
         for (int r = 0; r < 4; r++) acc[a][r] = acc[a][r] * f + (some ? x[i][a][r] * g : 0.f);
     }
   }
+  const int64_t row = (int64_t)it.first * p.H + m0 + c;
+  if constexpr (S > 1) {
+#pragma unroll
+    for (int a = 0; a < 16; a++) part_acc[wv][a][lane] = acc[a / 4][a % 4];
+    part_m[wv][lane] = m;
+    part_l[wv][lane] = l;
+    __syncthreads();
+    float x = 0.f, y = 0.f;  // values 2 wv and + 1
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < S; i++) {
+      const float li = part_l[i][lane];
+      const bool some = li > 0.f || li != li;
+      const float mi = part_m[i][lane], mn = some ? fmaxf(m, mi) : m;
+      const float f = l > 0.f || l != l ? __builtin_amdgcn_exp2f(m - mn) : 0.f;
+      const float g = some ? __builtin_amdgcn_exp2f(mi - mn) : 0.f;
+      m = mn;
+      l = l * f + (some ? li * g : 0.f);
+      x = x * f + (some ? part_acc[i][2 * wv][lane] * g : 0.f);
+      y = y * f + (some ? part_acc[i][2 * wv + 1][lane] * g : 0.f);
+    }
+    if (m0 + c >= M) return;
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    *reinterpret_cast<f16x2*>(p.o + row * kValueDim + 32 * t + 8 * (wv >> 1) + 4 * hf + 2 * (wv & 1)) =
+        (f16x2){(f16)(x * inv), (f16)(y * inv)};
+    if (t == 0 && hf == 0 && wv == 0)
+      p.lse[row] = l > 0.f || l != l ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY;
+    return;
+  }
   if (m0 + c >= M) return;
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  const int64_t row = (int64_t)it.first * p.H + m0 + c;
 #pragma unroll
   for (int a = 0; a < 4; a++) {
     f16x4 v;
@@ -1046,7 +1087,9 @@ extern "C" int mi355_dsa_mla_tree_attention(
   if (rc != MI355_DSA_OK) return rc;
   kern<<<kTreeWGs, kTreeThreads, lds, st>>>(p);
   DSA_LAUNCH_CHECK("mla_tree");
-  tree_merge_kernel<<<dim3((unsigned)(units / 4)), 256, 0, st>>>(p);
+  // few groups have many pieces each
+  if (units <= kTreeMergeUnits) tree_merge_kernel<8><<<dim3((unsigned)units), 512, 0, st>>>(p);
+  else tree_merge_kernel<1><<<dim3((unsigned)(units / 4)), 256, 0, st>>>(p);
   DSA_LAUNCH_CHECK("mla_tree merge");
   return MI355_DSA_OK;
 }
