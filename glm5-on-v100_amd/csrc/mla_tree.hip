@@ -276,7 +276,8 @@ __device__ __forceinline__ float* tree_part(const TreeParams& p, int64_t k) {
 // In LDS a tile is block-major: block b (32 dims, 64 bytes) of key r at 2048 b +
 // 64 r, its 16-byte piece i at i ^ ((r >> 2) & 3): the QK reads (one piece of 32
 // keys per half-wave) and the transpose reads cover the banks without conflicts.
-// Wave w brings blocks 9 (w / 2) .. +8 of keys 16 (w % 2) .. +15, four lanes a key.
+// Of fp16 rows wave w brings blocks 9 (w / 2) .. +8 of keys 16 (w % 2) .. +15, four
+// lanes a key.
 __device__ __align__(16) const uint8_t kTreeZeroRow[kLatentDim * 2] = {};
 
 __device__ __forceinline__ void tree_dma_rope(const uint8_t* row, uint8_t* slot, int w) {
@@ -621,7 +622,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
       // instructions is spread over the steps (a wave alone on its SIMD waits for
       // each), and the first operands of a product are read in the one before it.
       auto is_draft = [&](int tile) { return seg_lo + tile * kTreeTile + kTreeTile > draft0; };
-      // slots of the tiles i .. i + 3, bytes
+      // slots of the tiles i .. i + 3 (fp8: i + 2), bytes
       int s0 = 0, s1 = kTreeSlotBytes, s2 = 2 * kTreeSlotBytes, s3 = FP8 ? 0 : 3 * kTreeSlotBytes;
       uint32_t dirty = 0;
       if constexpr (FP8) {
