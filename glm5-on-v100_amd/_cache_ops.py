@@ -53,8 +53,10 @@ def rope_concat_and_cache_mla(positions: torch.Tensor, table: torch.Tensor, kv_c
     table [positions, 64] (rope.rotary_table); T = slot_mapping.numel() tokens,
     positions [T]; q [T, H, D] of kv_c's type, its dims [q_offset, q_offset + 64)
     rotated into q_out (q itself for in place; allocated if not given).  k_pe is
-    not changed.  A token with a negative slot writes no row, its q is rotated all
-    the same; one with a position outside the table is not rotated.  Valid slots
+    not changed.  The 64 rope values of an fp8_ds_mla row are stored in k_pe's type, as
+    the writer alone does; gather_latent_cache takes that type, sparse, dense and tree
+    attention read fp16 (for bf16 tensors see DsaLayer.store, which stores fp16).
+    A token with a negative slot writes no row, its q is rotated all the same; one with a position outside the table is not rotated.  Valid slots
     must be distinct.  Returns q_out, or None without q."""
     _check(kv_cache_dtype in ("auto", "fp8_ds_mla"),
            f"rope_concat_and_cache_mla: unsupported kv_cache_dtype {kv_cache_dtype!r}")

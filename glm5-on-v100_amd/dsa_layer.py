@@ -104,6 +104,14 @@ def _rows8(x: torch.Tensor) -> torch.Tensor:
     return x if ok else x.contiguous()
 
 
+def _rope_bits(k_pe: torch.Tensor) -> torch.Tensor:
+    """k_pe as the latent rows of this layer hold it.  Everything that attends to them
+    reads their 64 rope values as fp16 (q is fp16), while the writers store a value's 16
+    bits as they are: bf16 values are rounded to fp16 here (exact for 2^-14 <= |x| <=
+    65504) and keep bf16's name for the writer, which takes one type for the row."""
+    return k_pe.to(torch.float16).view(torch.bfloat16) if k_pe.dtype == torch.bfloat16 else k_pe
+
+
 def head_proj(out: torch.Tensor, x: torch.Tensor, wt: torch.Tensor, tail: int) -> None:
     """out[t, h, :N] = x[t, h, :K] @ wt[h].T, out[t, h, N:N+tail] = x[t, h, K:K+tail];
     x [T, H, >= K + tail], wt [H, N, K], out [T, H, >= N + tail] (fp16)."""
@@ -164,7 +172,8 @@ class DsaLayer:
 
     def store_latent(self, kv_c: torch.Tensor, k_pe: torch.Tensor,
                      slot_mapping: torch.Tensor) -> None:
-        _cache_ops.concat_and_cache_mla(kv_c, k_pe, self.latent_cache, slot_mapping,
+        """The rows' rope values are stored as fp16, whatever k_pe's type."""
+        _cache_ops.concat_and_cache_mla(kv_c, _rope_bits(k_pe), self.latent_cache, slot_mapping,
                                         self.kv_dtype, self._one)
 
     def store_index_key(self, idx_k: torch.Tensor, slot_mapping: torch.Tensor) -> None:
@@ -316,7 +325,7 @@ class DsaLayer:
             ok = x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0
             return x if ok else x.contiguous()
 
-        kv_c, k_pe = rows16(kv_c[:B]), rows16(k_pe[:B])
+        kv_c, k_pe = rows16(kv_c[:B]), rows16(_rope_bits(k_pe[:B]))
         ik = idx_k[:B].to(torch.float16).contiguous()
         slot = slot_mapping.contiguous()
         islot = slot.to(torch.int32)
@@ -371,7 +380,7 @@ class DsaLayer:
             ok = x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0
             return x if ok else x.contiguous()
 
-        kv_c, k_pe = rows16(kv_c[:B]), rows16(k_pe[:B])
+        kv_c, k_pe = rows16(kv_c[:B]), rows16(_rope_bits(k_pe[:B]))
         ik = idx_k[:B].to(torch.float16).contiguous()
         slot = slot_mapping.contiguous()
         islot = slot.to(torch.int32)
@@ -405,27 +414,31 @@ class DsaLayer:
         the cache positions seq_lens[r] - n .. seq_lens[r] - 1 in the order of the
         request's n tokens, cu_seqlens_q[r] .. cu_seqlens_q[r + 1] - 1; tree_mask as in
         mla_tree.tree_attention.  idx_k [T, 128], if given, is rotated over its first 64
-        dims (half layout) and written to the indexer cache.  q, k_pe and idx_k stay as
-        they are.  Returns out [T, H * V], zero for tokens of no request."""
+        dims (half layout) and written to the indexer cache.  kv_c and k_pe may be bf16
+        where the rows are fp8_ds_mla (the rope values are stored as fp16).  q, k_pe and
+        idx_k stay as they are.  Returns out [T, H * V], zero for tokens of no request."""
         T = slot_mapping.numel()
         _check(q.dim() == 3 and q.shape == (T, self.w.n_heads, self.w.nope_dim + 64),
                "q must be [T, H, P + 64], a slot for each token")
         _check(q.dtype == torch.float16, "q must be fp16")
         _check(positions.shape == (T,), "positions must be [T]")
-        fused = kv_c.dtype == torch.float16  # else (bf16) q is rotated in a launch of its own
-        qr = _cache_ops.rope_concat_and_cache_mla(
-            positions, table, kv_c, k_pe, self.latent_cache, slot_mapping, self.kv_dtype,
-            interleaved, q if fused else None, self.w.nope_dim)
-        rest = [] if fused else [q]
+        P = self.w.nope_dim
         if idx_k is not None:
             _check(idx_k.shape == (T, 128), "idx_k must be [T, 128]")
-            rest.append(idx_k)
-        if rest:
-            done = rope.apply_rotary(rest, positions, table,
-                                     ([] if fused else [self.w.nope_dim]) + [0] * (idx_k is not None),
-                                     ([] if fused else [interleaved]) + [False] * (idx_k is not None))
-            if not fused:
+        if kv_c.dtype == torch.float16:
+            qr = _cache_ops.rope_concat_and_cache_mla(positions, table, kv_c, k_pe,
+                                                      self.latent_cache, slot_mapping,
+                                                      self.kv_dtype, interleaved, q, P)
+            xs, offs, inter = [], [], []
+        else:  # bf16: rotated in k_pe's type, stored as fp16
+            xs, offs, inter = [q, k_pe[:T]], [P, 0], [interleaved] * 2
+        if idx_k is not None:
+            xs, offs, inter = xs + [idx_k], offs + [0], inter + [False]
+        if xs:
+            done = rope.apply_rotary(xs, positions, table, offs, inter)
+            if kv_c.dtype != torch.float16:
                 qr = done[0]
+                self.store_latent(kv_c, done[1], slot_mapping)
             if idx_k is not None:
                 self.store_index_key(done[-1], slot_mapping)
         H = self.w.n_heads

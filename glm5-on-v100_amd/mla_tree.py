@@ -44,7 +44,7 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
     i of its tree_mask (int64 [T]) is set, its own bit included; at most 64 drafted
     tokens of a request can be seen.  kv_cache [n_blocks, page, 576] fp16 or
     [n_blocks, page, 656] uint8 (fp8_ds_mla, read as the fp16 values that
-    gather_latent_cache gives); block_table int32 [R, max_blocks], seq_lens int32 [R].
+    gather_latent_cache gives; the 64 rope values must have been written as fp16); block_table int32 [R, max_blocks], seq_lens int32 [R].
 
     Returns o [T, H, 512] fp16 and lse [T, H] fp32; a row that sees nothing has
     o = 0 and lse = -inf.  Rows of no request (behind the last one) are not
