@@ -40,11 +40,13 @@ the fp16 MFMA peak (fewer, fuller launches; 2048 is level, larger is slower
 once the buffer leaves the 256 MB MALL).
 
 Verification of drafted trees (verify_tree) takes the step's tensors as the
-projections leave them, not yet rotated, and attends densely, as the few rows of
-a draft and their request's whole context are one matrix product for all heads:
-rotary positions of q and k_pe with the latent rows written in the same launch
-(rope_concat_and_cache_mla), the indexer's key rotated and stored, step 3, tree
-attention, step 5.
+projections leave them, not yet rotated, and accepts drafts by the outputs that
+decode would give: rotary positions of q and k_pe with the latent rows written in
+the same launch (rope_concat_and_cache_mla), the indexer's key rotated and stored,
+step 3, the attention, step 5.  Where the block table holds at most topk positions
+the selection keeps every key and the attention is tree attention, one matrix
+product of all heads of a draft and their request's context; in longer tables it is
+steps 2 and 4, each drafted token with its own selection out of what it sees.
 
 All buffers come from torch's caching allocator; nothing here synchronises
 the host except the per-sub-chunk causal reach, which the reference also reads
@@ -405,8 +407,9 @@ class DsaLayer:
                     positions: torch.Tensor, table: torch.Tensor, slot_mapping: torch.Tensor,
                     block_table: torch.Tensor, seq_lens: torch.Tensor,
                     cu_seqlens_q: torch.Tensor, tree_mask: torch.Tensor,
-                    idx_k: torch.Tensor | None = None,
-                    interleaved: bool = True) -> torch.Tensor:
+                    idx_k: torch.Tensor | None = None, interleaved: bool = True,
+                    idx_q: torch.Tensor | None = None,
+                    idx_w: torch.Tensor | None = None) -> torch.Tensor:
         """Every request's tree of drafted tokens in one step.  q [T, H, P + 64] fp16,
         kv_c [T, 512] and k_pe [T, 64], not rotated; positions [T] are the tokens'
         places in the text (context length + depth in the tree, mla_tree.tree_masks),
@@ -415,16 +418,26 @@ class DsaLayer:
         request's n tokens, cu_seqlens_q[r] .. cu_seqlens_q[r + 1] - 1; tree_mask as in
         mla_tree.tree_attention.  idx_k [T, 128], if given, is rotated over its first 64
         dims (half layout) and written to the indexer cache.  kv_c and k_pe may be bf16
-        where the rows are fp8_ds_mla (the rope values are stored as fp16).  q, k_pe and
-        idx_k stay as they are.  Returns out [T, H * V], zero for tokens of no request."""
+        where the rows are fp8_ds_mla (the rope values are stored as fp16).  A block table
+        of more than topk positions needs idx_q [T, 32, 128], rotated as idx_k is, and
+        idx_w [T, 32]: every token attends to the topk of its visible positions that the
+        indexer chooses, as in decode (last_idx), with the indexer's keys in the cache or
+        given as idx_k.  q, k_pe, idx_k and idx_q stay as they are.  Returns out [T, H * V], zero for tokens of no request."""
         T = slot_mapping.numel()
         _check(q.dim() == 3 and q.shape == (T, self.w.n_heads, self.w.nope_dim + 64),
                "q must be [T, H, P + 64], a slot for each token")
         _check(q.dtype == torch.float16, "q must be fp16")
         _check(positions.shape == (T,), "positions must be [T]")
-        P = self.w.nope_dim
+        P, R = self.w.nope_dim, block_table.shape[0]
+        choose = R > 0 and block_table.shape[1] * self.latent_cache.shape[-2] > self.topk
         if idx_k is not None:
             _check(idx_k.shape == (T, 128), "idx_k must be [T, 128]")
+        if choose:
+            _check(idx_q is not None and idx_w is not None,
+                   f"the block table has more than topk = {self.topk} positions: idx_q and idx_w "
+                   "are needed")
+            _check(idx_q.shape == (T, 32, 128) and idx_w.shape == (T, 32),
+                   "idx_q must be [T, 32, 128] and idx_w [T, 32]")
         if kv_c.dtype == torch.float16:
             qr = _cache_ops.rope_concat_and_cache_mla(positions, table, kv_c, k_pe,
                                                       self.latent_cache, slot_mapping,
@@ -434,20 +447,60 @@ class DsaLayer:
             xs, offs, inter = [q, k_pe[:T]], [P, 0], [interleaved] * 2
         if idx_k is not None:
             xs, offs, inter = xs + [idx_k], offs + [0], inter + [False]
+        if choose:
+            xs, offs, inter = xs + [idx_q], offs + [0], inter + [False]
         if xs:
             done = rope.apply_rotary(xs, positions, table, offs, inter)
             if kv_c.dtype != torch.float16:
                 qr = done[0]
                 self.store_latent(kv_c, done[1], slot_mapping)
             if idx_k is not None:
-                self.store_index_key(done[-1], slot_mapping)
+                self.store_index_key(done[-2 if choose else -1], slot_mapping)
+        ql = q_latent(qr, self.w)
+        if choose:
+            idx, bt, sl = self._tree_topk(done[-1], idx_w, block_table, seq_lens, cu_seqlens_q,
+                                          tree_mask)
+            o, lse, out = self._attention(ql, idx, bt, sl)
+            lse = lse.masked_fill((idx < 0).all(1, keepdim=True), float("-inf"))
+            self.last_idx, self.last_o, self.last_lse = idx, o, lse
+            return out
         H = self.w.n_heads
         o = torch.zeros(T, H, 512, dtype=torch.float16, device=q.device)
         lse = torch.full((T, H), float("-inf"), dtype=torch.float32, device=q.device)
-        mla_tree.tree_attention(q_latent(qr, self.w), self.latent_cache, block_table, seq_lens,
-                                cu_seqlens_q, tree_mask, self.w.scale, o, lse)
+        mla_tree.tree_attention(ql, self.latent_cache, block_table, seq_lens, cu_seqlens_q,
+                                tree_mask, self.w.scale, o, lse)
         self.last_idx, self.last_o, self.last_lse = None, o, lse
         return v_up(o, self.w)
+
+    def _tree_topk(self, idx_q, idx_w, block_table, seq_lens, cu_seqlens_q, tree_mask):
+        """The topk of each token's visible positions by the indexer's scores, ascending,
+        -1 where there is none; with the block-table row and length of each token."""
+        T, R, dev = idx_q.shape[0], block_table.shape[0], idx_q.device
+        max_kv = block_table.shape[1] * self.idx_k_cache.shape[1]
+        t = torch.arange(T, dtype=torch.int32, device=dev)
+        r = torch.searchsorted(cu_seqlens_q, t, right=True) - 1
+        live = (r >= 0) & (r < R)  # a request's token
+        r = r.clamp(0, R - 1)
+        n = cu_seqlens_q[r + 1] - cu_seqlens_q[r]
+        sl = torch.where(live, seq_lens[r], 0).to(torch.int32)
+        bt = block_table.index_select(0, r)
+        score = torch.empty(T, max_kv, dtype=torch.float32, device=dev)
+        _sm70_ops.sm70_indexer_logits(score, idx_q.to(torch.float16).contiguous(),
+                                      self.idx_k_cache, idx_w.to(torch.float16).contiguous(), bt,
+                                      sl, None)
+        # the columns of the request's drafted tokens: those that the token does not see
+        W = min(T, max_kv)
+        first = (sl - n).long()  # position of drafted token 0
+        col = first.clamp(0, max_kv - W)[:, None] + torch.arange(W, device=dev)
+        d = col - first[:, None]
+        bit = (tree_mask[:, None] >> d.clamp(0, mla_tree.MAX_DRAFT - 1)) & 1
+        hide = (d >= 0) & (d < n[:, None]) & ((bit == 0) | (d >= mla_tree.MAX_DRAFT))
+        score.scatter_(1, col, score.gather(1, col).masked_fill(hide, float("-inf")))
+        idx = torch.empty(T, self.topk, dtype=torch.int32, device=dev)
+        ws = torch.empty(1 << 20, dtype=torch.uint8, device=dev)
+        _sm70_ops.persistent_topk(score, sl.view(T, 1), idx, ws, self.topk, max_kv)
+        hidden = score.gather(1, idx.clamp_min(0).long()) == float("-inf")
+        return idx.masked_fill_(hidden, -1), bt, sl
 
     # -- prefill ------------------------------------------------------------
     def prefill_topk(self, idx_q: torch.Tensor, idx_w: torch.Tensor, bounds: list[int],
