@@ -197,7 +197,6 @@ def asm_path(name: str) -> str:
     return os.path.join(BUILD_DIR, name.replace(".hip", f"-hip-amdgcn-amd-amdhsa-{ARCH}.s"))
 
 
-TESTKIT_SRC = os.path.join(PKG_DIR, "..", "tests", "hip", "quant_exhaustive.hip")
 TESTKIT_LIB = os.path.join(PKG_DIR, "..", "tests", "hip", "libdsa_testkit.so")
 
 
@@ -205,10 +204,11 @@ def build_testkit(verbose: bool = True) -> str:
     """Builds the test-only kernels (tests/hip/*.hip) into
     tests/hip/libdsa_testkit.so; the product library does not contain them."""
     tmp = TESTKIT_LIB + ".tmp"
-    cmd = [hipcc(), *compile_flags(), "-shared", TESTKIT_SRC, "-o", tmp]
+    sources = sorted(glob.glob(os.path.join(os.path.dirname(TESTKIT_LIB), "*.hip")))
+    cmd = [hipcc(), *compile_flags(), "-shared", *sources, "-o", tmp]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"hipcc failed for {TESTKIT_SRC}:\n{r.stdout}\n{r.stderr}")
+        raise RuntimeError(f"hipcc failed for {sources}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, TESTKIT_LIB)
     if verbose:
         print(f"built {os.path.normpath(TESTKIT_LIB)}", flush=True)

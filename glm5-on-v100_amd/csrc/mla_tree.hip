@@ -48,22 +48,17 @@
 
 #include "capi_internal.h"
 #include "dsa_common.h"
+#include "mla_tree_plan.h"
 #include "mla_waves.h"
 
 namespace mi355dsa {
 
 constexpr int kTreeWaves = 4;
 constexpr int kTreeThreads = 64 * kTreeWaves;
-constexpr int kTreeRows = 128;      // (token, head) rows of a group
-constexpr int kTreeTile = 32;       // keys
 // key tiles in LDS
 __host__ __device__ constexpr int tree_slots(bool fp8) { return fp8 ? 3 : 4; }
 constexpr int kTreePages = 2048;    // block-table entries resolved at a time
 constexpr int kTreeMaxDraft = 64;   // tokens of a request that a mask can name
-constexpr int kTreeWGs = 256;       // runs of the line: one workgroup per CU
-// Tiles of a run at least.  us of 4 tokens x 16 heads for 2, 3, 4: 500 keys 20.4 / 20.2 /
-// 22.4, 8000 30.9 / 29.1 / 28.7; of 8 x 64 over 500: 28.4 / 26.5 / 27.2.
-constexpr int kTreeMinTiles = 3;
 constexpr int kTreeBlocks = kLatentDim / 32;                   // 64-byte blocks of an fp16 row
 constexpr int kTreeSlotBytes = kTreeBlocks * kTreeTile * 64;   // 36864
 // fp8 rows as they are, on their way: bytes of a wave's share of a tile (twice)
@@ -77,26 +72,6 @@ constexpr float kTreeLazyMax = 8.f; // log2 that scores may exceed the running m
 constexpr int kTreeMergeUnits = 16 * 64;
 constexpr int kTreePartWave = 64 * 64 * 4;  // floats of a wave's O^T in a partial
 
-struct TreeParams {
-  const f16* q;
-  const uint8_t* kv;
-  const int32_t* bt;
-  const int32_t* seq_lens;
-  const int32_t* cu;
-  const int64_t* mask;
-  f16* o;
-  float* lse;
-  float* part;  // [2 kTreeWGs] of part_waves x kTreePartWave, m [32 part_waves], l likewise
-  int part_waves;
-  int64_t* plan;  // [2] of the workspace
-  int R, T, H;
-  int max_blocks, page_size;
-  uint32_t page_mul, page_shift;  // x / page_size = x * page_mul >> page_shift for x < 2^31
-  int64_t n_kv_rows;
-  float sl;      // |scale| log2 e (log2 e where scale is 0)
-  float q_sign;  // -1, 0 or 1: sign of scale
-};
-
 template <bool FP8>
 struct TreeSmem {
   uint8_t ring[tree_slots(FP8)][kTreeSlotBytes];
@@ -108,6 +83,9 @@ struct TreeSmem {
   // of each wave, over the loops: first row, rows and group of the request, place of
   // its partial (-1: o is written)
   u32x4 item[kTreeWaves];
+  // .. the plan, and the place that it goes on from
+  TreePlan plan[kTreeWaves];
+  int64_t at[kTreeWaves];
 };
 static_assert(sizeof(TreeSmem<false>) <= 160 * 1024 && sizeof(TreeSmem<true>) <= 160 * 1024,
               "one workgroup per CU");
@@ -125,146 +103,6 @@ __device__ __forceinline__ TreeParams tree_params() {
 #endif
 }
 
-// threadIdx.x, not known to be the same from use to use: what follows from it is
-// computed where it is used, instead of a register for each over the tile loop.
-__device__ __forceinline__ int tree_tid() {
-  int t = threadIdx.x;
-  asm volatile("" : "+v"(t));
-  return t;
-}
-
-// ---- the line of tiles ----
-struct TreeReq {
-  int first, n;  // token rows
-  int len;       // positions that can be visible
-  int groups, tiles;
-};
-__device__ __forceinline__ TreeReq tree_req(const TreeParams& p, int r) {
-  TreeReq q = {0, 0, 0, 0, 0};
-  if (r < p.R) {
-    const int a = min(max(p.cu[r], 0), p.T), b = min(max(p.cu[r + 1], a), p.T);
-    q.first = a;
-    q.n = b - a;
-    const int64_t width = (int64_t)p.max_blocks * p.page_size;
-    q.len = max(0, p.seq_lens[r]);
-    if (q.len > width) q.len = (int)width;
-    q.groups = (int)(((int64_t)q.n * p.H + kTreeRows - 1) / kTreeRows);
-    q.tiles = max(1, (q.len + kTreeTile - 1) / kTreeTile);  // no key: one empty tile
-  }
-  return q;
-}
-__device__ __forceinline__ int64_t shfl64(int64_t v, int src) {
-  return ((int64_t)__builtin_amdgcn_readlane((int)(v >> 32), src) << 32) |
-         (uint32_t)__builtin_amdgcn_readlane((int)v, src);
-}
-// inclusive sums over the lanes, of which the first n hold something
-__device__ __forceinline__ int64_t scan64(int64_t v, int n) {
-  const int lane = tree_tid() & 63;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    if (m >= n) break;
-    const int64_t u = __shfl_up(v, m, 64);
-    if (lane >= m) v += u;
-  }
-  return v;
-}
-struct TreePlan {
-  int kt;       // tiles of a cell at most; 0: equal runs of the line
-  int64_t per;  // tiles of a run of the line
-};
-// Groups of one request that work on the same keys at the same time share them in
-// the XCD's L2; apart, each fetches them for itself, more than memory gives (one
-// request of 8 groups at 180k, fp16 rows: 430 us with a group per XCD).  So requests
-// are cut into cells of kt tiles, the groups of a cell next to each other, kt the
-// smallest found that needs no more than one workgroup per CU.  Where that leaves
-// more than a fifth of the workgroups' time unused (many groups, uneven lengths),
-// the workgroups take equal runs of the line instead.
-__device__ __forceinline__ TreePlan tree_plan(const TreeParams& p) {
-  const int lane = tree_tid() & 63;
-  int64_t line = 0;
-  for (int r0 = 0; r0 < p.R; r0 += 64) {
-    const TreeReq q = tree_req(p, r0 + lane);
-    line += shfl64(scan64((int64_t)q.groups * q.tiles, p.R - r0), min(p.R - r0, 64) - 1);
-  }
-  TreePlan pl;
-  pl.per = max((int64_t)kTreeMinTiles, (line + kTreeWGs - 1) / kTreeWGs);
-  const int64_t most = max((int64_t)kTreeMinTiles, line / (kTreeWGs * 4 / 5));
-  int64_t kt = pl.per;
-  pl.kt = 0;
-  while (true) {
-    int64_t units = 0;
-    for (int r0 = 0; r0 < p.R; r0 += 64) {
-      const TreeReq q = tree_req(p, r0 + lane);
-      const int n = kt >= q.tiles ? 1 : (q.tiles + (int)kt - 1) / (int)kt;
-      units += shfl64(scan64((int64_t)q.groups * n, p.R - r0), min(p.R - r0, 64) - 1);
-    }
-    if (units <= kTreeWGs) {
-      pl.kt = (int)min(kt, (int64_t)INT32_MAX);
-      break;
-    }
-    if (kt >= most) break;
-    // by what the count is over, an eighth of the way at least: few steps
-    const int64_t over = kt * (min(units, (int64_t)2 * kTreeWGs) - kTreeWGs) / (2 * kTreeWGs);
-    kt = min(most, kt + max(max((int64_t)1, (most - pl.per) / 8), over));
-  }
-  return pl;
-}
-struct TreeItem {
-  int r;          // request, -1: none
-  int first, n, len, tiles;
-  int g;          // group
-  int cell;       // cells: tiles of one (the request's cells are alike)
-  int64_t start;  // of the group on the line; cells: the group's first unit
-  int step;       // cells: units from one cell of the group to its next
-  int part;       // cells: which one
-};
-// The group (by_group: the at-th one) or the piece of one at place `at`: of the line,
-// or unit `at` of the cells, which stand request by request, cell by cell, group by
-// group.
-__device__ __forceinline__ TreeItem tree_find(const TreeParams& p, const TreePlan& pl, int64_t at,
-                                              bool by_group) {
-  TreeItem it = {-1, 0, 0, 0, 1, 0, 1, 0, 1, 0};
-  int64_t base = 0, line = 0;
-  for (int r0 = 0; r0 < p.R; r0 += 64) {
-    const TreeReq q = tree_req(p, r0 + (tree_tid() & 63));
-    int cell = q.tiles, n = 1;
-    if (pl.kt > 0 && q.tiles > pl.kt) {
-      n = (q.tiles + pl.kt - 1) / pl.kt;
-      cell = (q.tiles + n - 1) / n;
-      n = (q.tiles + cell - 1) / cell;
-    }
-    const int64_t cost = (int64_t)q.groups * (pl.kt > 0 ? n : q.tiles);  // units, or tiles
-    const int64_t size = by_group ? q.groups : cost;
-    const int64_t incl = base + scan64(size, p.R - r0);
-    const uint64_t hit = __ballot(at < incl && size > 0);
-    const int64_t lsum = line + scan64(cost, p.R - r0);
-    if (hit) {
-      const int k = __builtin_ctzll(hit);
-      it.r = r0 + k;
-      it.first = __builtin_amdgcn_readlane(q.first, k);
-      it.n = __builtin_amdgcn_readlane(q.n, k);
-      it.len = __builtin_amdgcn_readlane(q.len, k);
-      it.tiles = __builtin_amdgcn_readlane(q.tiles, k);
-      it.cell = __builtin_amdgcn_readlane(cell, k);
-      const int groups = __builtin_amdgcn_readlane(q.groups, k);
-      const int in = (int)(at - shfl64(incl - size, k));
-      const int64_t from = shfl64(lsum - cost, k);
-      if (pl.kt > 0) {
-        it.part = by_group ? 0 : in / groups;
-        it.g = in - it.part * groups;
-        it.start = from + it.g;
-        it.step = groups;
-      } else {
-        it.g = by_group ? in : in / it.tiles;
-        it.start = from + (int64_t)it.g * it.tiles;
-      }
-      return it;
-    }
-    base = shfl64(incl, 63);
-    line = shfl64(lsum, 63);
-  }
-  return it;
-}
 // Partial k of the workspace.  Of the line, a run's first group, cut from an earlier
 // run, has place 2 run, and a group that begins in the run 2 run + 1; a cell has its
 // unit's number.
@@ -482,20 +320,23 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
   TreeSmem<FP8>& sh = *reinterpret_cast<TreeSmem<FP8>*>(smem_raw);
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-  // neighbouring runs on one XCD (workgroups go round the eight of them)
-  const int run = (int)(blockIdx.x & 7) * (kTreeWGs / 8) + (int)(blockIdx.x >> 3);
-  TreePlan plan = tree_plan(p);
-  if (run == 0 && threadIdx.x == 0) {  // for the merge
-    p.plan[0] = plan.kt;
-    p.plan[1] = plan.per;
+  // neighbouring runs on one XCD (workgroups go round the eight of them); computed where
+  // it is used, as what follows from the wave is
+  auto my_run = []() {
+    int b = blockIdx.x;
+    asm volatile("" : "+s"(b));
+    return (b & 7) * (kTreeWGs / 8) + (b >> 3);
+  };
+  {
+    const TreePlan plan = tree_plan(p);
+    const int run = my_run();
+    if (run == 0 && threadIdx.x == 0) {  // for the merge
+      p.plan[0] = plan.kt;
+      p.plan[1] = plan.per;
+    }
+    sh.plan[w] = plan;
+    sh.at[w] = run * plan.per;
   }
-  int64_t at = run;
-  int left = 1;  // cells: one unit; tiles of the run from there on
-  if (plan.kt == 0) {
-    at = run * plan.per;
-    left = (int)min(plan.per, (int64_t)INT32_MAX);
-  }
-
   // LDS addresses within a slot
   uint32_t ka0, va0;
   {
@@ -516,23 +357,26 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
     return x;
   };
 
-  while (left > 0) {
+  while (true) {
     const TreeParams p = tree_params();
+    const int mine = wave(), run = my_run();
+    const TreePlan plan = {__builtin_amdgcn_readfirstlane(sh.plan[mine].kt),
+                           tree_uniform(sh.plan[mine].per)};
+    int64_t at = tree_uniform(sh.at[mine]);
+    if (at >= (run + 1) * plan.per) break;
     const TreeItem it = tree_find(p, plan, at, false);
     if (it.r < 0) break;  // past the last one
     const int M = it.n * p.H;  // rows of the request
-    const int m0 = it.g * kTreeRows + 32 * w;
+    const int m0 = it.g * kTreeRows + 32 * mine;
     const bool active = m0 < M;
     const bool cells = plan.kt > 0;
-    const int t_lo = cells ? it.part * it.cell : (int)(at - it.start);
-    const int t_hi = (int)min((int64_t)it.tiles, (int64_t)t_lo + (cells ? it.cell : left));
+    const auto [t_lo, t_hi] = tree_take(plan, it, at, (run + 1) * plan.per);
+    sh.at[mine] = at;
     {
       const bool whole = t_lo == 0 && t_hi == it.tiles;
       const int place = whole ? -1 : cells ? run : 2 * run + (t_lo == 0 ? 1 : 0);
-      sh.item[w] = (u32x4){(uint32_t)it.first, (uint32_t)M, (uint32_t)it.g, (uint32_t)place};
+      sh.item[mine] = (u32x4){(uint32_t)it.first, (uint32_t)M, (uint32_t)it.g, (uint32_t)place};
     }
-    at += t_hi - t_lo;
-    left = cells ? 0 : left - (t_hi - t_lo);
     const int k_hi = min(t_hi * kTreeTile, it.len);
     const int draft0 = max(0, p.seq_lens[it.r]) - it.n;  // position of drafted token 0
 
@@ -545,7 +389,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
 #pragma unroll
       for (int s = 0; s < kLatentDim / 16; s++)
         qf[s] = *reinterpret_cast<const f16x8*>(qrow + 16 * s + 8 * hf);
-      sh.see[32 * w + c] = (uint64_t)p.mask[it.first + (uint32_t)m / (uint32_t)p.H];
+      sh.see[32 * wave() + c] = (uint64_t)p.mask[it.first + (uint32_t)m / (uint32_t)p.H];
       const f16 sg = (f16)p.q_sign;
       const f16x8 sg8 = {sg, sg, sg, sg, sg, sg, sg, sg};
 #pragma unroll
@@ -567,7 +411,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
       seg += ntiles;
       const int keys = min(ntiles * kTreeTile, k_hi - seg_lo);  // of the segment
       __syncthreads();  // blk and the ring are free
-      if (threadIdx.x == 0) sh.gap = 0;
+      if (tree_tid() == 0) sh.gap = 0;
       __syncthreads();
       {
         const int n = page_of(seg_lo + keys - 1) - pg0 + 1;
