@@ -34,6 +34,9 @@ int reserve_lds(const void* kernel, size_t bytes, const char* what);
 constexpr int kArriveRows = 64;
 uint32_t* arrive_slot(hipStream_t st);
 
+// Threads of a grid's dimension at most: HIP refuses a launch of 2^32 and more.
+constexpr int64_t kMaxThreads = UINT32_MAX;
+
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 inline bool aligned_to(const void* p, uintptr_t a) {

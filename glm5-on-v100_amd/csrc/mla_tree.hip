@@ -890,7 +890,7 @@ extern "C" int mi355_dsa_mla_tree_attention(
   DSA_CHECK(n_tok < ((int64_t)1 << 30) && n_tok * n_head < ((int64_t)1 << 30),
             "mla_tree: too many rows");
   const int64_t units = tree_max_groups(n_tok, n_head, n_req) * 64;  // of the merge
-  DSA_CHECK(units <= INT32_MAX, "mla_tree: too many rows");
+  DSA_CHECK((units + 3) / 4 <= kMaxThreads / 256, "mla_tree: too many rows");
   DSA_CHECK(o && lse && q && kv_cache && seq_lens && cu_seqlens_q && tree_mask &&
                 (block_table || max_blocks == 0),
             "null pointer argument");

@@ -310,7 +310,7 @@ extern "C" int mi355_dsa_rotary(const mi355_dsa_rotary_part* parts, int n_parts,
     if (rc != MI355_DSA_OK) return rc;
     a.first[i] = (int)n;
     n += blocks;
-    DSA_CHECK(n <= INT32_MAX, "rotary: too many tokens");
+    DSA_CHECK(n <= kMaxThreads / 256, "rotary: too many tokens");
   }
   a.n_parts = n_parts;
   a.first[n_parts] = (int)n;
@@ -360,7 +360,7 @@ extern "C" int mi355_dsa_rope_concat_and_cache_mla(
   a.kv = reinterpret_cast<uint8_t*>(kv_cache);
   a.n_rows = n_rows;
   const int64_t kv_blocks = (n_tok + 3) / 4;
-  DSA_CHECK(kv_blocks + q_blocks <= INT32_MAX, "too many tokens");
+  DSA_CHECK(kv_blocks + q_blocks <= kMaxThreads / 256, "%s: too many tokens", what);
   a.kv_blocks = (int)kv_blocks;
   const dim3 grid((unsigned)(kv_blocks + q_blocks));
   hipStream_t st = as_stream(stream);
@@ -397,7 +397,7 @@ extern "C" int mi355_dsa_gather_latent_cache(void* out, int64_t out_stride, int 
             "gather_latent_cache: out rows of at least 576 values, 16-byte aligned");
   DSA_CHECK(aligned_to(out, 16) && aligned_to(kv_cache, 16), "out / kv_cache misaligned");
   const int64_t blocks = (total + 4 * kGatherRows - 1) / (4 * kGatherRows);
-  DSA_CHECK(blocks <= INT32_MAX, "gather_latent_cache: too many rows");
+  DSA_CHECK(blocks <= kMaxThreads / 256, "gather_latent_cache: too many rows");
   GatherArgs a{};
   a.kv = reinterpret_cast<const uint8_t*>(kv_cache);
   a.n_rows = n_rows;
