@@ -14,7 +14,7 @@ import torch
 
 from . import rope
 from ._sm70_ops import _op
-from .ops import DSMLA_ROW_BYTES, _check, _contig, _launch
+from .ops import DSMLA_ROW_BYTES, _check, _contig, _launch, _rows16
 
 
 def concat_and_cache_mla(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache: torch.Tensor,
@@ -85,12 +85,7 @@ def rope_concat_and_cache_mla(positions: torch.Tensor, table: torch.Tensor, kv_c
     else:
         _check(q_out is None, "q_out without q")
 
-    def rows16(x):
-        ok = x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 \
-            and x.stride(0) >= x.size(1)
-        return x if ok else x.contiguous()
-
-    kv_c, k_pe, slot_mapping = rows16(kv_c), rows16(k_pe), _contig(slot_mapping)
+    kv_c, k_pe, slot_mapping = _rows16(kv_c), _rows16(k_pe), _contig(slot_mapping)
     _launch("mi355_dsa_rope_concat_and_cache_mla", kv_c.device, kv_cache.data_ptr(), fp8, n_rows,
             kv_c.data_ptr(), kv_c.stride(0), k_pe.data_ptr(), k_pe.stride(0),
             kv_c.dtype == torch.bfloat16, T, slot_mapping.data_ptr(),

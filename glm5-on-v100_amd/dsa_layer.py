@@ -59,7 +59,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _cache_ops, _lib, _sm70_ops, mla_tree, rope
-from .ops import _check, _stream
+from .ops import _check, _rows16, _stream
 
 KT = 64  # key tile the prefill logits launch is rounded to (sparse_attn_indexer.py:753)
 
@@ -98,14 +98,6 @@ class DsaLayerWeights:
         return self.W_UV.shape[2]
 
 
-def _rows8(x: torch.Tensor) -> torch.Tensor:
-    """x with unit last stride, 16-byte aligned, token / head strides that
-    are multiples of 8 elements (what the kernel loads 16 B at a time)."""
-    ok = (x.stride(2) == 1 and x.stride(1) % 8 == 0 and x.stride(0) % 8 == 0
-          and x.data_ptr() % 16 == 0)
-    return x if ok else x.contiguous()
-
-
 def _rope_bits(k_pe: torch.Tensor) -> torch.Tensor:
     """k_pe as the latent rows of this layer hold it.  Everything that attends to them
     reads their 64 rope values as fp16 (q is fp16), while the writers store a value's 16
@@ -134,7 +126,7 @@ def q_latent(q: torch.Tensor, w: DsaLayerWeights) -> torch.Tensor:
     """q [T, H, P + 64] -> [T, H, 576] fp16: bmm(q_nope, W_UK_T) | q_pe
     (triton_mla.py:413-418), one launch."""
     _check(q.dim() == 3 and q.shape[2] == w.nope_dim + 64, "q must be [T, H, P + 64]")
-    q = _rows8(q)
+    q = _rows16(q)
     out = torch.empty(q.shape[0], q.shape[1], 576, dtype=torch.float16, device=q.device)
     head_proj(out, q, w.uk_t, 64)
     return out
@@ -145,7 +137,7 @@ def v_up(o: torch.Tensor, w: DsaLayerWeights) -> torch.Tensor:
     (triton_mla.py:486-492), one launch."""
     T, H, _ = o.shape
     out = torch.empty(T, H * w.v_dim, dtype=torch.float16, device=o.device)
-    head_proj(out.view(T, H, w.v_dim), _rows8(o), w.uv_t, 0)
+    head_proj(out.view(T, H, w.v_dim), _rows16(o), w.uv_t, 0)
     return out
 
 
@@ -320,14 +312,10 @@ class DsaLayer:
         spec: (bt [B, max_blocks], sl [B]) that the launch fills from bt / sl,
         which are then per request (mi355_dsa_decode_layer_indexer_spec)."""
         B, H = q.shape[0], q.shape[1]
-        q = _rows8(q)
+        q = _rows16(q)
         ql = torch.empty(B, H, 576, dtype=torch.float16, device=q.device)
 
-        def rows16(x):
-            ok = x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0
-            return x if ok else x.contiguous()
-
-        kv_c, k_pe = rows16(kv_c[:B]), rows16(_rope_bits(k_pe[:B]))
+        kv_c, k_pe = _rows16(kv_c[:B]), _rows16(_rope_bits(k_pe[:B]))
         ik = idx_k[:B].to(torch.float16).contiguous()
         slot = slot_mapping.contiguous()
         islot = slot.to(torch.int32)
@@ -374,15 +362,11 @@ class DsaLayer:
         """mi355_dsa_decode_layer_prologue: q_latent (returned), the latent
         and indexer-K cache writes, and a cleared histogram (returned)."""
         B, H = q.shape[0], q.shape[1]
-        q = _rows8(q)
+        q = _rows16(q)
         ql = torch.empty(B, H, 576, dtype=torch.float16, device=q.device)
         hist = torch.empty(B, 4096, dtype=torch.int32, device=q.device)
 
-        def rows16(x):
-            ok = x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0
-            return x if ok else x.contiguous()
-
-        kv_c, k_pe = rows16(kv_c[:B]), rows16(_rope_bits(k_pe[:B]))
+        kv_c, k_pe = _rows16(kv_c[:B]), _rows16(_rope_bits(k_pe[:B]))
         ik = idx_k[:B].to(torch.float16).contiguous()
         slot = slot_mapping.contiguous()
         islot = slot.to(torch.int32)

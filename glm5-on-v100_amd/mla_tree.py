@@ -75,7 +75,9 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
            and out.device == q.device, "out must be contiguous fp16 [tokens, heads, 512]")
     _check(lse.dtype == torch.float32 and lse.shape == (T, H) and lse.is_contiguous()
            and lse.device == q.device, "lse must be contiguous fp32 [tokens, heads]")
-    q, block_table, seq_lens = _contig(q), _contig(block_table), _contig(seq_lens)
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    block_table, seq_lens = _contig(block_table), _contig(seq_lens)
     cu_seqlens_q, tree_mask = _contig(cu_seqlens_q), _contig(tree_mask)
     need = _lib.lib().mi355_dsa_mla_tree_workspace_size(T, H)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)

@@ -100,6 +100,17 @@ def _contig(t: torch.Tensor) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _rows16(x: torch.Tensor) -> torch.Tensor:
+    """x of 16-bit values, or a copy, as the kernels load it 16 bytes at a time: the last
+    dim dense, the other strides multiples of 8 elements (and rows that do not overlap),
+    the start 16-byte aligned.  contiguous() would not do: a tensor of one row counts as
+    contiguous wherever it starts and whatever its row stride."""
+    st = x.stride()
+    ok = st[-1] == 1 and x.data_ptr() % 16 == 0 and st[0] >= x.size(-1) \
+        and (st[0] | st[-2]) % 8 == 0  # two or three dims
+    return x if ok else x.clone(memory_format=torch.contiguous_format)
+
+
 def _out_ok(t: torch.Tensor, name: str) -> None:
     _check(t.is_contiguous(), f"{name} must be contiguous")
 
@@ -392,11 +403,7 @@ def concat_and_cache_mla_impl(kv_c, k_pe, kv_cache, slot_mapping, kv_cache_dtype
     if n_tok == 0:
         return
 
-    def rows16(x):
-        ok = (x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0)
-        return x if ok else x.contiguous()
-
-    kv_c, k_pe, slot_mapping = rows16(kv_c), rows16(k_pe), _contig(slot_mapping)
+    kv_c, k_pe, slot_mapping = _rows16(kv_c), _rows16(k_pe), _contig(slot_mapping)
     with torch.cuda.device(kv_c.device):
         _lib.call("mi355_dsa_concat_and_cache_mla", kv_cache.data_ptr(), int(fp8), n_rows,
                   kv_c.data_ptr(), kv_c.stride(0), k_pe.data_ptr(), k_pe.stride(0),
