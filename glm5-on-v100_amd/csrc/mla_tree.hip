@@ -17,7 +17,8 @@
 //   * S^T = K Q^T, v_mfma_f32_32x32x16: 32 keys x 32 rows over 576 dims, Q in 144
 //     registers;
 //   * softmax per row: lane (row c, half) holds 16 of its 32 scores; the running
-//     maximum is moved, and O scaled, only where a score exceeds it by 2^8 or more;
+//     maximum is moved, and O scaled, only where a score exceeds it by 2^8 or more, and
+//     weights stand 2^6 above it, so that they use fp16's range from 2^14 down;
 //   * O^T += V^T P^T: 512 dims x 32 rows in 256 accumulation registers; the S^T
 //     accumulator layout (keys 8 a + 4 half + r) is P^T's operand layout, so P stays
 //     in registers; V^T comes from transpose LDS reads in that order.
@@ -66,6 +67,10 @@ constexpr int kTreeRaw = 64 * 64 + 256;
 // LDS reads ahead of their MFMA; fp8 rows leave no registers for a third
 __host__ __device__ constexpr int tree_ahead(bool fp8) { return fp8 ? 2 : 3; }
 constexpr float kTreeLazyMax = 8.f; // log2 that scores may exceed the running maximum by
+// Weights are 2^(s - m + kTreeLift), at most 2^14 in fp16: keys far lighter than the
+// running maximum lose bits below 2^-20 of it and vanish below 2^-31, where at 2^(s - m)
+// 184320 keys of 2^-25 each, 0.5 % of the sum, were in l and not in O.
+constexpr float kTreeLift = 6.f;
 // Units of the merge (64 a group) up to which 8 waves share one.  us with a wave and with
 // 8 a unit: 1 group over 8000 keys 50 / 29, over 180000 107 / 65; 8 groups 378 / 379; 32
 // groups with 8 pieces each 176 / 188.
@@ -530,7 +535,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
           l_part *= alpha;
           if (first) up = 0;  // O is zero
         }
-        ml = m_run * p.sl;
+        ml = __builtin_fmaf(m_run, p.sl, -kTreeLift);
       };
       if (active) {
         kb = tree_addr(lds0 + ka0, 0);
@@ -724,8 +729,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
           }
         });
         if (mine && hf == 0)
-          p.lse[row] = L > 0.f || L != L ? (m_run * p.sl + __log2f(L)) * 0.6931471805599453f
-                                         : -INFINITY;
+          p.lse[row] = L > 0.f || L != L
+                           ? (__builtin_fmaf(m_run, p.sl, -kTreeLift) + __log2f(L)) * 0.6931471805599453f
+                           : -INFINITY;
       } else {
         float* part = tree_part(p, place);
         unroll<64>([&](auto uc) {
@@ -736,7 +742,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
         });
         if (hf == 0) {
           part += p.part_waves * kTreePartWave;
-          part[32 * w + c] = m_run * p.sl;
+          part[32 * w + c] = __builtin_fmaf(m_run, p.sl, -kTreeLift);
           part[32 * p.part_waves + 32 * w + c] = L;
         }
       }
