@@ -291,11 +291,12 @@ __device__ __forceinline__ float tree_pick(uint32_t keys, int e, float a, float 
 }
 
 // A tile with drafted tokens, which not every row sees: 0 * inf would reach the
-// rows that do not.  Key rows that hold an infinity or NaN become zeros in LDS,
-// and their keys bits of the returned mask (to every wave, after a barrier): the
-// scores of the rows that see them are made NaN instead.  Wave w looks after
+// rows that do not.  Drafted key rows that hold an infinity or NaN become zeros in
+// LDS, and their keys bits of the returned mask (to every wave, after a barrier): the
+// scores of the rows that see them are made NaN instead.  The tile's keys before
+// `first` are context, seen by all rows, and stay as they are.  Wave w looks after
 // keys 8 w .. +7, eight lanes a key.
-__device__ __forceinline__ uint32_t tree_clean(uint32_t* flags, uint8_t* slot, int w) {
+__device__ __forceinline__ uint32_t tree_clean(uint32_t* flags, uint8_t* slot, int w, int first) {
   const int lane = tree_tid() & 63;
   // the lane's pieces: places q = lane % 8 + 8 i of the key's 72, four to a block
   uint8_t* const key = slot + 64 * (8 * w + (lane >> 3)) + 16 * (lane & 3) + 2048 * ((lane >> 2) & 1);
@@ -306,7 +307,7 @@ __device__ __forceinline__ uint32_t tree_clean(uint32_t* flags, uint8_t* slot, i
     for (int k = 0; k < 4; k++)
       bad |= (x[k] & 0x7c00u) == 0x7c00u || (x[k] & 0x7c000000u) == 0x7c000000u;
   }
-  const uint64_t lanes = __ballot(bad);
+  const uint64_t lanes = __ballot(bad && 8 * w + (lane >> 3) >= first);
   uint32_t keys = 0;
 #pragma unroll
   for (int k = 0; k < 8; k++) keys |= ((lanes >> (8 * k)) & 0xff) != 0 ? 1u << k : 0u;
@@ -497,7 +498,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
         asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
       }
       lds_barrier();  // tiles 0 and 1 are in
-      if (is_draft(0)) dirty = tree_clean(sh.dirty, sh.ring[0], wave());
+      if (is_draft(0)) dirty = tree_clean(sh.dirty, sh.ring[0], wave(), draft0 - seg_lo);
 
       constexpr int A = tree_ahead(FP8);
       f32x16 s;             // scores of tile i, then their exponentials
@@ -560,7 +561,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
         const bool more = i + 1 < ntiles;
         // tile i + 1 is in, and every wave is done with tile i - 1, in whose place
         // tile i + 3 goes
-        if (more && is_draft(i + 1)) dirty = tree_clean(sh.dirty, sh.ring[0] + s1, wave());
+        if (more && is_draft(i + 1))
+          dirty = tree_clean(sh.dirty, sh.ring[0] + s1, wave(), draft0 - seg_lo - (i + 1) * kTreeTile);
         uint8_t* const raw = sh.raw[FP8 ? i & 1 : 0][FP8 ? w : 0];
         // fp8: the wave's share of tile i + 2 has landed
         if constexpr (FP8) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
