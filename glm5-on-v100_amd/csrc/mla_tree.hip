@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
       constexpr int A = tree_ahead(FP8);
       f32x16 s;             // scores of tile i, then their exponentials
       float mt = 0.f;       // the largest score
-      float ml = 0.f, alpha = 1.f;  // of the exponents; of O
+      float alpha = 1.f;    // of O
       int up = 0;           // O has to be scaled
       TreeFrag<A> kf, vf;
       TreeAddr kb;
@@ -536,7 +536,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
           l_part *= alpha;
           if (first) up = 0;  // O is zero
         }
-        ml = __builtin_fmaf(m_run, p.sl, -kTreeLift);
       };
       if (active) {
         kb = tree_addr(lds0 + ka0, 0);
@@ -587,8 +586,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
             unroll<64>([&](auto k) { hw_scale<4 * k>(alpha); });
           }
           f16x8 pb[2];
-          // stages of the exponential of element e
-          auto arg = [&](int e) { s[e] = __builtin_fmaf(s[e], p.sl, -ml); };
+          // stages of the exponential of element e; from the difference of the scores, which
+          // is 0 for the largest whatever its size (s sl - m sl is off by the rounding of
+          // m sl: P was infinite from scores of 2^25 on; 0.5 % of the time with few groups)
+          auto arg = [&](int e) { s[e] = __builtin_fmaf(s[e] - m_run, p.sl, kTreeLift); };
           auto ex = [&](int e) { s[e] = __builtin_amdgcn_exp2f(s[e]); };
           auto sum = [&](int e) {
             l_part += s[e];
@@ -893,7 +894,7 @@ extern "C" int mi355_dsa_mla_tree_attention(
   DSA_CHECK(page_size > 0, "page size must be > 0");
   DSA_CHECK(n_kv_rows < ((int64_t)1 << 31), "cache has too many rows");
   DSA_CHECK((int64_t)max_blocks * page_size < ((int64_t)1 << 30), "mla_tree: block table too wide");
-  DSA_CHECK(isfinite(scale), "mla_tree: scale must be finite");
+  DSA_CHECK(isfinite(scale * 1.4426950408889634f), "mla_tree: scale must be finite, also times log2 e");
   if (n_tok == 0 || n_req == 0) return MI355_DSA_OK;
   DSA_CHECK(n_tok < ((int64_t)1 << 30) && n_tok * n_head < ((int64_t)1 << 30),
             "mla_tree: too many rows");
