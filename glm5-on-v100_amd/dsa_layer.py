@@ -412,6 +412,8 @@ class DsaLayer:
                "q must be [T, H, P + 64], a slot for each token")
         _check(q.dtype == torch.float16, "q must be fp16")
         _check(positions.shape == (T,), "positions must be [T]")
+        # the rest of what later launches would refuse: none may follow a written cache
+        mla_tree._check_trees(T, block_table, seq_lens, cu_seqlens_q, tree_mask, q.device)
         P, R = self.w.nope_dim, block_table.shape[0]
         choose = R > 0 and block_table.shape[1] * self.latent_cache.shape[-2] > self.topk
         if idx_k is not None:
@@ -422,6 +424,11 @@ class DsaLayer:
                    "are needed")
             _check(idx_q.shape == (T, 32, 128) and idx_w.shape == (T, 32),
                    "idx_q must be [T, 32, 128] and idx_w [T, 32]")
+            _check(idx_w.device == q.device, "idx_w must be on q's GPU")
+        for x in (idx_k, idx_q if choose else None):
+            _check(x is None or (x.dtype in rope._DTYPE_CODE and x.device == q.device
+                                 and x.stride(-1) == 1),
+                   "idx_k and idx_q must be fp16, bf16 or fp32 on q's GPU, the last dim contiguous")
         if kv_c.dtype == torch.float16:
             qr = _cache_ops.rope_concat_and_cache_mla(positions, table, kv_c, k_pe,
                                                       self.latent_cache, slot_mapping,

@@ -33,6 +33,21 @@ def tree_masks(parents) -> tuple[list[int], list[int]]:
     return mask, depth
 
 
+def _check_trees(n_tok: int, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                 cu_seqlens_q: torch.Tensor, tree_mask: torch.Tensor, dev: torch.device) -> None:
+    _check(block_table.dim() == 2 and block_table.dtype == torch.int32,
+           "block_table must be int32 [requests, max_blocks]")
+    R = block_table.size(0)
+    _check(seq_lens.dim() == 1 and seq_lens.dtype == torch.int32 and seq_lens.size(0) == R,
+           "seq_lens must be int32 [requests]")
+    _check(cu_seqlens_q.dim() == 1 and cu_seqlens_q.dtype == torch.int32
+           and cu_seqlens_q.size(0) == R + 1, "cu_seqlens_q must be int32 [requests + 1]")
+    _check(tree_mask.dim() == 1 and tree_mask.dtype == torch.int64 and tree_mask.size(0) == n_tok,
+           "tree_mask must be int64 [tokens]")
+    _check(block_table.device == dev and seq_lens.device == dev and cu_seqlens_q.device == dev
+           and tree_mask.device == dev, "all tensors must be on one GPU")
+
+
 def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor,
                    seq_lens: torch.Tensor, cu_seqlens_q: torch.Tensor, tree_mask: torch.Tensor,
                    scale: float, out: torch.Tensor | None = None,
@@ -55,18 +70,8 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
     fp8, n_rows = _latent_rows(kv_cache)
     T, H = q.size(0), q.size(1)
     _check(H > 0, "n_head must be > 0")
-    _check(block_table.dim() == 2 and block_table.dtype == torch.int32,
-           "block_table must be int32 [requests, max_blocks]")
+    _check_trees(T, block_table, seq_lens, cu_seqlens_q, tree_mask, q.device)
     R = block_table.size(0)
-    _check(seq_lens.dim() == 1 and seq_lens.dtype == torch.int32 and seq_lens.size(0) == R,
-           "seq_lens must be int32 [requests]")
-    _check(cu_seqlens_q.dim() == 1 and cu_seqlens_q.dtype == torch.int32
-           and cu_seqlens_q.size(0) == R + 1, "cu_seqlens_q must be int32 [requests + 1]")
-    _check(tree_mask.dim() == 1 and tree_mask.dtype == torch.int64 and tree_mask.size(0) == T,
-           "tree_mask must be int64 [tokens]")
-    _check(block_table.device == q.device and seq_lens.device == q.device
-           and cu_seqlens_q.device == q.device and tree_mask.device == q.device,
-           "all tensors must be on one GPU")
     if out is None:
         out = torch.empty(T, H, 512, dtype=torch.float16, device=q.device)
     if lse is None:
