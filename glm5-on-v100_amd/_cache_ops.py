@@ -82,6 +82,7 @@ def rope_concat_and_cache_mla(positions: torch.Tensor, table: torch.Tensor, kv_c
     if q is not None:
         _check(q.dtype == kv_c.dtype, "q must have kv_c's type")
         part, q_out = rope._part(q, q_out, q_offset, interleaved, T, kv_c.device)
+        part = part if q.shape[-2] else None  # no head
     else:
         _check(q_out is None, "q_out without q")
 

@@ -125,6 +125,7 @@ def apply_rotary(xs, positions: torch.Tensor, table: torch.Tensor, offsets=0, in
     positions = _table_args(positions, table)
     T, dev = positions.shape[0], table.device
     parts = [_part(x, o, a, i, T, dev) for x, o, a, i in zip(xl, ol, offs, inter)]
-    _launch("mi355_dsa_rotary", dev, b"".join([p[0] for p in parts]), n, positions.data_ptr(),
+    some = [p for p, y in parts if y.shape[-2]]  # tensors of no head need no work
+    _launch("mi355_dsa_rotary", dev, b"".join(some), len(some), positions.data_ptr(),
             positions.dtype == torch.int64, T, table.data_ptr(), table.shape[0], table.shape[1])
     return parts[0][1] if single else [p[1] for p in parts]
