@@ -2,6 +2,7 @@
 // every token written in the same launch, and the latent cache read back.
 #include <float.h>
 #include <stddef.h>
+#include <stdlib.h>
 
 #include "cache_write.h"
 #include "capi_internal.h"
@@ -308,6 +309,12 @@ extern "C" int mi355_dsa_rotary(const mi355_dsa_rotary_part* parts, int n_parts,
     int64_t blocks = 0;
     rc = rotary_part(parts[i], rot_dim, n_tok, "rotary", &a.part[i], &blocks);
     if (rc != MI355_DSA_OK) return rc;
+    // one tensor's two parts may be rotated in place, the same elements may not be twice
+    for (int j = 0; j < i; j++)
+      DSA_CHECK(parts[i].out != parts[j].out ||
+                    (a.part[i].inplace && a.part[j].inplace &&
+                     abs(parts[i].offset - parts[j].offset) >= rot_dim),
+                "rotary: two tensors of a call are written to the same place");
     a.first[i] = (int)n;
     n += blocks;
     DSA_CHECK(n <= kMaxThreads / 256, "rotary: too many tokens");

@@ -111,7 +111,8 @@ def apply_rotary(xs, positions: torch.Tensor, table: torch.Tensor, offsets=0, in
     4 (a step's q, k_pe and the indexer's q and k) with one offset and layout
     each, rotated in one launch.  outs: tensors to write, xs themselves for in
     place (only the rotated part moves then); otherwise they must not overlap
-    xs.  A token whose position is outside the table (a padded one, -1) is not
+    xs, and no two of them may hold the same elements (of two places in one tensor,
+    both in place, the rotated parts).  A token whose position is outside the table (a padded one, -1) is not
     rotated.  Returns what was written, a tensor or a list as xs."""
     single = isinstance(xs, torch.Tensor)
     xl = [xs] if single else xs

@@ -100,7 +100,8 @@ int mi355_dsa_concat_and_cache_mla(void* kv_cache, int kv_fp8, int64_t n_rows,
  * copied; with out == x (and the same strides) they are not touched, otherwise
  * out must not overlap x.  Strides in elements, the last dim dense.  A token
  * whose position is outside [0, max_pos) is not rotated.  positions: int64
- * (pos_i64 = 1) or int32 [n_tok].  Up to 4 parts share one launch.
+ * (pos_i64 = 1) or int32 [n_tok].  Up to 4 parts share one launch; no two may
+ * write the same elements.
  * It has no counterpart in the reference, which takes rotated tensors.
  */
 typedef struct {
