@@ -12,9 +12,9 @@ from __future__ import annotations
 
 import torch
 
-from . import rope
+from . import ops, rope
 from ._sm70_ops import _op
-from .ops import DSMLA_ROW_BYTES, _check, _contig, _launch, _rows16
+from .ops import DSMLA_ROW_BYTES, _check, _contig, _launch, _no_grad, _rows16, _traced
 
 
 def concat_and_cache_mla(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache: torch.Tensor,
@@ -58,6 +58,19 @@ def rope_concat_and_cache_mla(positions: torch.Tensor, table: torch.Tensor, kv_c
     attention read fp16 (for bf16 tensors see DsaLayer.store, which stores fp16).
     A token with a negative slot writes no row, its q is rotated all the same; one with a position outside the table is not rotated.  Valid slots
     must be distinct.  Returns q_out, or None without q."""
+    _no_grad(kv_c, k_pe, q)
+    if not _traced(kv_c):
+        return _rope_write(positions, table, kv_c, k_pe, kv_cache, slot_mapping, kv_cache_dtype,
+                           interleaved, q, q_offset, q_out)
+    if q is not None and q_out is None:
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    ops.op("rope_concat_and_cache_mla")(positions, table, kv_c, k_pe, kv_cache, slot_mapping,
+                                        kv_cache_dtype, interleaved, q, q_offset, q_out)
+    return q_out
+
+
+def _rope_write(positions, table, kv_c, k_pe, kv_cache, slot_mapping, kv_cache_dtype, interleaved,
+                q, q_offset, q_out):
     _check(kv_cache_dtype in ("auto", "fp8_ds_mla"),
            f"rope_concat_and_cache_mla: unsupported kv_cache_dtype {kv_cache_dtype!r}")
     fp8, n_rows = _latent_rows(kv_cache)
@@ -110,6 +123,15 @@ def gather_latent_cache(kv_cache: torch.Tensor, block_table: torch.Tensor,
     written, they stay as they were in a given out).  dtype fp16, bf16 or fp32;
     pe_dtype: the type that the 64 rope values of fp8_ds_mla rows were written in.
     A position whose row does not resolve reads as zeros."""
+    if _traced(kv_cache):
+        if out is None:
+            out = torch.empty(total, 576, dtype=dtype, device=kv_cache.device)
+        ops.op("gather_latent_cache")(out, kv_cache, block_table, cu_seqlens, starts, dtype, pe_dtype)
+        return out
+    return _gather(out, kv_cache, block_table, cu_seqlens, total, starts, dtype, pe_dtype)
+
+
+def _gather(out, kv_cache, block_table, cu_seqlens, total, starts, dtype, pe_dtype):
     fp8, n_rows = _latent_rows(kv_cache)
     _check(kv_cache.is_cuda and block_table.device == kv_cache.device
            and cu_seqlens.device == kv_cache.device
@@ -141,3 +163,19 @@ def gather_latent_cache(kv_cache: torch.Tensor, block_table: torch.Tensor,
             n_rows, kv_cache.size(-2), block_table.data_ptr(), block_table.size(1),
             cu_seqlens.data_ptr(), starts.data_ptr() if starts is not None else None, R)
     return out
+
+
+def _op_rope_write(*args):
+    _rope_write(*args)
+
+
+def _op_gather(out, kv_cache, block_table, cu_seqlens, starts, dtype, pe_dtype):
+    _gather(out, kv_cache, block_table, cu_seqlens, out.size(0), starts, dtype, pe_dtype)
+
+
+ops.define("rope_concat_and_cache_mla(Tensor positions, Tensor table, Tensor kv_c, Tensor k_pe, "
+           "Tensor(a!) kv_cache, Tensor slot_mapping, str kv_cache_dtype, bool interleaved, "
+           "Tensor? q, int q_offset, Tensor(b!)? q_out) -> ()", _op_rope_write)
+ops.define("gather_latent_cache(Tensor(a!) out, Tensor kv_cache, Tensor block_table, "
+           "Tensor cu_seqlens, Tensor? starts, ScalarType dtype, ScalarType pe_dtype) -> ()",
+           _op_gather)

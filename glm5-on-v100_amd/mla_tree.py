@@ -11,9 +11,9 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib
+from . import _lib, ops
 from ._cache_ops import _latent_rows
-from .ops import _check, _contig, _launch
+from .ops import _check, _contig, _launch, _no_grad, _traced
 
 MAX_DRAFT = 64  # drafted tokens of a request that a mask can name
 
@@ -64,6 +64,19 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
     Returns o [T, H, 512] fp16 and lse [T, H] fp32; a row that sees nothing has
     o = 0 and lse = -inf.  Rows of no request (behind the last one) are not
     written: they stay as they were in a given out / lse."""
+    _no_grad(q, kv_cache)
+    _check(q.dim() == 3, "q must be [tokens, heads, 576]")
+    T, H = q.shape[:2]
+    if out is None:
+        out = torch.empty(T, H, 512, dtype=torch.float16, device=q.device)
+    if lse is None:
+        lse = torch.empty(T, H, dtype=torch.float32, device=q.device)
+    run = ops.op("mla_tree_attention") if _traced(q) else _attention
+    run(out, lse, q, kv_cache, block_table, seq_lens, cu_seqlens_q, tree_mask, scale)
+    return out, lse
+
+
+def _attention(out, lse, q, kv_cache, block_table, seq_lens, cu_seqlens_q, tree_mask, scale):
     _check(q.is_cuda and kv_cache.device == q.device, "q and kv_cache must be on the GPU")
     _check(q.dtype == torch.float16, "q must be fp16")
     _check(q.dim() == 3 and q.size(2) == 576, "q must be [tokens, heads, 576]")
@@ -72,10 +85,6 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
     _check(H > 0, "n_head must be > 0")
     _check_trees(T, block_table, seq_lens, cu_seqlens_q, tree_mask, q.device)
     R = block_table.size(0)
-    if out is None:
-        out = torch.empty(T, H, 512, dtype=torch.float16, device=q.device)
-    if lse is None:
-        lse = torch.empty(T, H, dtype=torch.float32, device=q.device)
     _check(out.dtype == torch.float16 and out.shape == (T, H, 512) and out.is_contiguous()
            and out.device == q.device, "out must be contiguous fp16 [tokens, heads, 512]")
     _check(lse.dtype == torch.float32 and lse.shape == (T, H) and lse.is_contiguous()
@@ -90,4 +99,8 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
             T, H, kv_cache.data_ptr(), fp8, n_rows, kv_cache.size(-2), block_table.data_ptr(),
             block_table.size(1), seq_lens.data_ptr(), cu_seqlens_q.data_ptr(), R,
             tree_mask.data_ptr(), scale, ws.data_ptr(), need)
-    return out, lse
+
+
+ops.define("mla_tree_attention(Tensor(a!) o, Tensor(b!) lse, Tensor q, Tensor kv_cache, "
+           "Tensor block_table, Tensor seq_lens, Tensor cu_seqlens_q, Tensor tree_mask, "
+           "float scale) -> ()", _attention)

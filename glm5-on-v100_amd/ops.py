@@ -487,6 +487,27 @@ _registered = {}
 CACHE_OPS = ("concat_and_cache_mla",)
 
 
+def define(schema: str, impl) -> None:
+    """Adds an op without a counterpart in the reference (rope.py, _cache_ops.py and
+    mla_tree.py define theirs when the package is imported).  Their Python functions call
+    the kernel directly (a dispatch costs half of a short call) and the op where they are
+    traced."""
+    name = schema.partition("(")[0]
+    SCHEMAS[name], IMPLS[name] = schema, impl
+
+
+def _traced(t: torch.Tensor) -> bool:
+    """Whether a call on t is recorded (torch.compile, fake tensors) instead of run."""
+    return torch.compiler.is_compiling() or type(t) is not torch.Tensor
+
+
+def _no_grad(*tensors: torch.Tensor | None) -> None:
+    """Refuses tensors whose gradient the call would lose without a word."""
+    if torch.is_grad_enabled():
+        _check(not any(t is not None and t.requires_grad for t in tensors),
+               "there is no backward pass: call under torch.no_grad() or on detached tensors")
+
+
 def register(namespace: str | None = None, names=None) -> str:
     """Registers the ops `names` (default: every op) in `namespace`
     (idempotent per namespace); returns the namespace."""

@@ -13,8 +13,8 @@ import math
 
 import torch
 
-from . import _lib
-from .ops import _check, _launch
+from . import _lib, ops
+from .ops import _check, _launch, _no_grad, _traced
 
 _DTYPE_CODE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 MAX_TENSORS = 4  # of one launch
@@ -123,10 +123,29 @@ def apply_rotary(xs, positions: torch.Tensor, table: torch.Tensor, offsets=0, in
     ol = [None] * n if outs is None else [outs] if isinstance(outs, torch.Tensor) else outs
     _check(len(offs) == n and len(inter) == n and len(ol) == n,
            "apply_rotary: one offset, layout and out for each tensor")
+    _no_grad(*xl)
+    if _traced(positions):
+        ol = [torch.empty_like(x, memory_format=torch.contiguous_format) if o is None else o
+              for x, o in zip(xl, ol)]
+        ops.op("apply_rotary")(ol, xl, positions, table, offs, inter)
+    else:
+        ol = _rotary(ol, xl, positions, table, offs, inter)
+    return ol[0] if single else ol
+
+
+def _rotary(ol, xl, positions, table, offs, inter) -> list[torch.Tensor]:
     positions = _table_args(positions, table)
     T, dev = positions.shape[0], table.device
     parts = [_part(x, o, a, i, T, dev) for x, o, a, i in zip(xl, ol, offs, inter)]
     some = [p for p, y in parts if y.shape[-2]]  # tensors of no head need no work
     _launch("mi355_dsa_rotary", dev, b"".join(some), len(some), positions.data_ptr(),
             positions.dtype == torch.int64, T, table.data_ptr(), table.shape[0], table.shape[1])
-    return parts[0][1] if single else [p[1] for p in parts]
+    return [p[1] for p in parts]
+
+
+def _op_rotary(*args):
+    _rotary(*args)
+
+
+ops.define("apply_rotary(Tensor(a!)[] outs, Tensor[] xs, Tensor positions, Tensor table, "
+           "int[] offsets, bool[] interleaved) -> ()", _op_rotary)
