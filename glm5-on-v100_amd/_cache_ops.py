@@ -71,8 +71,8 @@ def rope_concat_and_cache_mla(positions: torch.Tensor, table: torch.Tensor, kv_c
 
 def _rope_write(positions, table, kv_c, k_pe, kv_cache, slot_mapping, kv_cache_dtype, interleaved,
                 q, q_offset, q_out):
-    _check(kv_cache_dtype in ("auto", "fp8_ds_mla"),
-           f"rope_concat_and_cache_mla: unsupported kv_cache_dtype {kv_cache_dtype!r}")
+    if kv_cache_dtype not in ("auto", "fp8_ds_mla"):
+        raise RuntimeError(f"rope_concat_and_cache_mla: unsupported kv_cache_dtype {kv_cache_dtype!r}")
     fp8, n_rows = _latent_rows(kv_cache)
     _check(fp8 == (kv_cache_dtype == "fp8_ds_mla"),
            "kv_cache's type is not that of kv_cache_dtype")
@@ -95,7 +95,7 @@ def _rope_write(positions, table, kv_c, k_pe, kv_cache, slot_mapping, kv_cache_d
     if q is not None:
         _check(q.dtype == kv_c.dtype, "q must have kv_c's type")
         part, q_out = rope._part(q, q_out, q_offset, interleaved, T, kv_c.device)
-        part = part if q.shape[-2] else None  # no head
+        part = part or None  # no head
     else:
         _check(q_out is None, "q_out without q")
 

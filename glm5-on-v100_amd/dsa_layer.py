@@ -469,11 +469,12 @@ class DsaLayer:
         T, R, dev = idx_q.shape[0], block_table.shape[0], idx_q.device
         max_kv = block_table.shape[1] * self.idx_k_cache.shape[1]
         t = torch.arange(T, dtype=torch.int32, device=dev)
-        r = torch.searchsorted(cu_seqlens_q, t, right=True) - 1
+        cu = cu_seqlens_q.clamp(0, T)
+        r = torch.searchsorted(cu, t, right=True) - 1
         live = (r >= 0) & (r < R)  # a request's token
         r = r.clamp(0, R - 1)
-        n = cu_seqlens_q[r + 1] - cu_seqlens_q[r]
-        sl = torch.where(live, seq_lens[r], 0).to(torch.int32)
+        n = cu[r + 1] - cu[r]
+        sl = torch.where(live, seq_lens[r], 0).clamp_min(0)
         bt = block_table.index_select(0, r)
         score = torch.empty(T, max_kv, dtype=torch.float32, device=dev)
         _sm70_ops.sm70_indexer_logits(score, idx_q.to(torch.float16).contiguous(),

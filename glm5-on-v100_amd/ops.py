@@ -2,7 +2,8 @@
 
 Schemas are the reference's, verbatim (patches/glm5-v100-sm70-glue.patch:
 494-565; persistent_topk from its call sites, reference/
-sparse_attn_indexer.py:632-639 and :873-880).  Each op validates its tensors
+sparse_attn_indexer.py:632-639 and :873-880); rope.py, _cache_ops.py and
+mla_tree.py define those that the reference lacks.  Each op validates its tensors
 the way the reference's TORCH_CHECKs do (same conditions, RuntimeError),
 then calls the C ABI on the current stream.  Only the CUDA (= HIP on ROCm)
 dispatch key has a kernel: CPU tensors raise, there is no silent fallback.
@@ -78,6 +79,7 @@ def _stream(t: torch.Tensor) -> int:
 
 
 _current_device = torch.cuda.current_device
+_is_compiling, _grad_enabled = torch.compiler.is_compiling, torch.is_grad_enabled
 # the handle alone: building the Stream object around it takes 1 us
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
                       lambda i: torch.cuda.current_stream(i).cuda_stream)
@@ -498,14 +500,16 @@ def define(schema: str, impl) -> None:
 
 def _traced(t: torch.Tensor) -> bool:
     """Whether a call on t is recorded (torch.compile, fake tensors) instead of run."""
-    return torch.compiler.is_compiling() or type(t) is not torch.Tensor
+    return _is_compiling() or type(t) is not torch.Tensor
 
 
 def _no_grad(*tensors: torch.Tensor | None) -> None:
     """Refuses tensors whose gradient the call would lose without a word."""
-    if torch.is_grad_enabled():
-        _check(not any(t is not None and t.requires_grad for t in tensors),
-               "there is no backward pass: call under torch.no_grad() or on detached tensors")
+    if _grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("there is no backward pass: call under torch.no_grad() or on "
+                                   "detached tensors")
 
 
 def register(namespace: str | None = None, names=None) -> str:

@@ -73,7 +73,8 @@ def rotary_table(rot_dim: int, max_positions: int, base: float = 10000.0,
 
 def _part(x: torch.Tensor, out: torch.Tensor | None, offset: int, interleaved: bool, n_tok: int,
           dev: torch.device):
-    """(packed mi355_dsa_rotary_part, out) of x [T, H, D] or [T, D]; out allocated if None."""
+    """(packed mi355_dsa_rotary_part, out) of x [T, H, D] or [T, D]; out allocated if None.
+    Nothing is packed of a tensor of no head."""
     shape, code = x.shape, _DTYPE_CODE.get(x.dtype)
     _check(len(shape) in (2, 3) and shape[0] == n_tok,
            "apply_rotary: tensors are [tokens, heads, dim] or [tokens, dim]")
@@ -89,6 +90,8 @@ def _part(x: torch.Tensor, out: torch.Tensor | None, offset: int, interleaved: b
     _check((xs[-1] == 1 and os[-1] == 1) or shape[-1] <= 1,
            "apply_rotary: the last dim must be contiguous")
     heads = shape[1] if len(xs) == 3 else 1
+    if heads == 0:
+        return b"", out
     return _lib.ROTARY_PART.pack(out.data_ptr(), x.data_ptr(), os[0], os[-2], xs[0], xs[-2], heads,
                                  shape[-1], offset, code, interleaved), out
 
@@ -117,7 +120,8 @@ def apply_rotary(xs, positions: torch.Tensor, table: torch.Tensor, offsets=0, in
     single = isinstance(xs, torch.Tensor)
     xl = [xs] if single else xs
     n = len(xl)
-    _check(1 <= n <= MAX_TENSORS, f"apply_rotary: 1 to {MAX_TENSORS} tensors")
+    if not 1 <= n <= MAX_TENSORS:
+        raise RuntimeError(f"apply_rotary: 1 to {MAX_TENSORS} tensors")
     offs = [offsets] * n if isinstance(offsets, int) else offsets
     inter = [interleaved] * n if isinstance(interleaved, bool) else interleaved
     ol = [None] * n if outs is None else [outs] if isinstance(outs, torch.Tensor) else outs
@@ -137,9 +141,10 @@ def _rotary(ol, xl, positions, table, offs, inter) -> list[torch.Tensor]:
     positions = _table_args(positions, table)
     T, dev = positions.shape[0], table.device
     parts = [_part(x, o, a, i, T, dev) for x, o, a, i in zip(xl, ol, offs, inter)]
-    some = [p for p, y in parts if y.shape[-2]]  # tensors of no head need no work
-    _launch("mi355_dsa_rotary", dev, b"".join(some), len(some), positions.data_ptr(),
-            positions.dtype == torch.int64, T, table.data_ptr(), table.shape[0], table.shape[1])
+    packed = b"".join([p[0] for p in parts])
+    _launch("mi355_dsa_rotary", dev, packed, len(packed) // _lib.ROTARY_PART.size,
+            positions.data_ptr(), positions.dtype == torch.int64, T, table.data_ptr(),
+            table.shape[0], table.shape[1])
     return [p[1] for p in parts]
 
 
