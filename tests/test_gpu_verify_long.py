@@ -146,6 +146,35 @@ def test_trees(pkg, lib, dev, H, extra, fp8):
     assert bool((L.last_lse[T:] == -torch.inf).all())
 
 
+def test_lengths_past_the_table_and_below_nothing(pkg, lib, dev):
+    """A length past the table: its positions are seen, the drafted tokens have none; a
+    negative one: nothing is seen; offsets past the tokens end with them."""
+    g = torch.Generator().manual_seed(12)
+    H, ctx, counts = 16, [477, 100, 200], [3, 2, 2]
+    bt = torch.randperm(90, generator=g).int().view(3, 30)
+    L = layer(pkg, dev, H, False)
+    fill(L, ctx, bt, dev, g)
+    a, m = step(ctx, counts, bt, H, dev, g), meta(ctx, counts, bt, dev)
+    m["seq_lens"] = torch.tensor([500, -7, 202], dtype=torch.int32, device=dev)
+    m["cu_seqlens_q"] = torch.tensor([0, 3, 5, 9], dtype=torch.int32, device=dev)  # 7 tokens
+    a["slot_mapping"][:5] = -1
+    mask = torch.tensor([1, 3, 5, 1, 3, 1, 3], device=dev)
+    pos = torch.full((7,), -1, device=dev)
+    out = L.verify_tree(positions=pos, table=pkg.rope.rotary_table(64, 8, device=dev), tree_mask=mask,
+                        **a, **m)
+    keys = L.idx_k_cache.flatten(0, 1).double().cpu()
+    for t in range(7):
+        r = [0, 0, 0, 1, 1, 2, 2][t]
+        j = t - [0, 3, 5][r]
+        see = [list(range(480)), [], list(range(200)) + [200 + i for i in range(j + 1)]][r]
+        at = slots(bt, r, see) if see else torch.zeros(0, dtype=torch.long)
+        s = (a["idx_q"][t].double().cpu() @ keys[at].T).clamp_min(0).T @ a["idx_w"][t].double().cpu()
+        pick = sorted(sorted(range(len(see)), key=lambda i: (-float(s[i]), see[i]))[:TOPK])
+        assert [i for i in L.last_idx[t].tolist() if i >= 0] == [see[i] for i in pick], t
+    assert bool((out[3:5] == 0).all()) and bool((L.last_lse[3:5] == -torch.inf).all())
+    assert bool((out[:3] != 0).any()) and bool((out[5:] != 0).any())
+
+
 def test_captured(pkg, lib, dev):
     """Captured once, replayed with other lengths and inputs and eager work between."""
     g = torch.Generator().manual_seed(9)
