@@ -26,7 +26,7 @@ def concat_and_cache_mla(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache: torch
     "auto": kv_cache fp16 [n_blocks, page, 576] = [kv_c | k_pe].
     "fp8_ds_mla": kv_cache uint8 [n_blocks, page, 656]: 512 e4m3 bytes with a
     max(amax/448, FLT_MIN) scale per 128-dim tile, the 4 fp32 scales, then the
-    64 16-bit RoPE values.  `scale` is unused by both (vLLM reads it only for
+    64 16-bit RoPE values in k_pe's type (sparse attention reads fp16).  `scale` is unused by both (vLLM reads it only for
     per-tensor fp8 caches)."""
     _op("concat_and_cache_mla")(kv_c, k_pe, kv_cache, slot_mapping, kv_cache_dtype, scale)
 
@@ -54,8 +54,8 @@ def rope_concat_and_cache_mla(positions: torch.Tensor, table: torch.Tensor, kv_c
     positions [T]; q [T, H, D] of kv_c's type, its dims [q_offset, q_offset + 64)
     rotated into q_out (q itself for in place; allocated if not given).  k_pe is
     not changed.  The 64 rope values of an fp8_ds_mla row are stored in k_pe's type, as
-    the writer alone does; gather_latent_cache takes that type, sparse, dense and tree
-    attention read fp16 (for bf16 tensors see DsaLayer.store, which stores fp16).
+    the writer alone does: gather_latent_cache and mla_tree.tree_attention take that type
+    (pe_dtype), sparse and dense attention read fp16 (DsaLayer stores fp16 for them).
     A token with a negative slot writes no row, its q is rotated all the same; one with a position outside the table is not rotated.  Valid slots
     must be distinct.  Returns q_out, or None without q."""
     _no_grad(kv_c, k_pe, q)

@@ -50,7 +50,8 @@ def compile_flags() -> list[str]:
 # those that hold values in accumulation registers named in inline asm, which
 # the compiler does not know to be in use.
 OWN_AGPRS = {"sparse_mla.hip": ["mla_hw_f16_kernel"],
-             "mla_tree.hip": ["mla_tree_kernelILb0E", "mla_tree_kernelILb1E"]}
+             "mla_tree.hip": ["mla_tree_kernelILb0E", "mla_tree_kernelILb1ELb0E",
+                              "mla_tree_kernelILb1ELb1E"]}
 # Kernels that must not spill: a reload in a loop waits for all of the wave's
 # memory operations, gathers in flight included.
 NO_SPILLS = {"sparse_mla.hip": ["sparse_mla_prefill_fp8_ws_kernel", "sparse_mla_few_kernelILb0E"],

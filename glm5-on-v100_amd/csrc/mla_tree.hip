@@ -128,6 +128,20 @@ __device__ __forceinline__ void tree_dma_rope(const uint8_t* row, uint8_t* slot,
   dma16(row + kValueDim + 16 + 64 * (w >> 1) + 16 * ((lane & 3) ^ ((lane >> 4) & 3)),
         slot + 2048 * (16 + (w >> 1)) + 1024 * (w & 1));
 }
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+// The wave's share of a tile's rope values, come as bf16, to fp16 in place: 16 bytes a
+// lane, once they have landed and before the barrier that hands the tile over.
+__device__ __forceinline__ void tree_rope_f16(uint32_t slot, int w) {
+  const uint32_t at = slot + 2048 * (16 + (w >> 1)) + 1024 * (w & 1) + 16 * (tree_tid() & 63);
+  u32x4 x = *(const lds_u32x4*)at;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const f16x2 h = {(f16)__builtin_bit_cast(float, x[i] << 16),
+                     (f16)__builtin_bit_cast(float, x[i] & 0xffff0000u)};
+    x[i] = __builtin_bit_cast(uint32_t, h);
+  }
+  *(lds_u32x4*)at = x;
+}
 // fp8_ds_mla rows: a wave's share of a tile, 256 e4m3 values of 16 keys (quads
 // 4 (w / 2) .. +3 of 64 dims; lane j of a key's four has 16 of each quad) and the keys'
 // scales, comes by LDS-DMA as it is, to be converted by the wave that fetched it.
@@ -320,7 +334,8 @@ __device__ __forceinline__ uint32_t tree_clean(uint32_t* flags, uint8_t* slot, i
   return __builtin_amdgcn_readfirstlane(flags[0] | flags[1] << 8 | flags[2] << 16 | flags[3] << 24);
 }
 
-template <bool FP8>
+// PE_BF16: the rope values of the (fp8) rows are bf16
+template <bool FP8, bool PE_BF16>
 __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   TreeSmem<FP8>& sh = *reinterpret_cast<TreeSmem<FP8>*>(smem_raw);
@@ -487,6 +502,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
           if (k == 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
         asm volatile("s_waitcnt vmcnt(5)" ::: "memory");
+        if constexpr (PE_BF16) {
+          tree_rope_f16(lds0, ww);
+          tree_rope_f16(lds0 + kTreeSlotBytes, ww);
+        }
       } else {
 #pragma unroll 1
         for (int k = 0; k < 3; k++) {
@@ -573,6 +592,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
             tree_convert_all(lds_at(raw), lds0 + s2, ww);
             tree_dma_raw(src, raw, ww);
             asm volatile("s_waitcnt vmcnt(11)" ::: "memory");
+            if constexpr (PE_BF16) tree_rope_f16(lds0 + s2, ww);
           } else {
             unroll<9>([&](auto k) { tree_dma1<k>(src, sh.ring[0] + s3 + dlds); });
             asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
@@ -677,6 +697,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mla_tree_kernel(TreeParams p)
               // after the barrier
               if constexpr (FP8) asm volatile("s_waitcnt vmcnt(11)" ::: "memory");
               else asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
+              if constexpr (PE_BF16) tree_rope_f16(lds0 + s2, wave());
               lds_barrier();
               kb = tree_addr(lds0 + s2 + ka0, 0);
               tree_kfirst(kf, kb);
@@ -891,6 +912,7 @@ extern "C" int mi355_dsa_mla_tree_attention(
   clear_error();
   DSA_CHECK(n_tok >= 0 && n_req >= 0 && n_head > 0, "mla_tree: bad sizes");
   DSA_CHECK(max_blocks >= 0 && n_kv_rows >= 0, "bad sizes");
+  DSA_CHECK(kv_fp8 >= 0 && kv_fp8 <= 2, "mla_tree: kv_fp8 must be 0, 1 or 2");
   DSA_CHECK(page_size > 0, "page size must be > 0");
   DSA_CHECK(n_kv_rows < ((int64_t)1 << 31), "cache has too many rows");
   DSA_CHECK((int64_t)max_blocks * page_size < ((int64_t)1 << 30), "mla_tree: block table too wide");
@@ -935,7 +957,9 @@ extern "C" int mi355_dsa_mla_tree_attention(
   p.sl = (scale == 0.f ? 1.f : fabsf(scale)) * 1.4426950408889634f;
   p.q_sign = scale == 0.f ? 0.f : scale < 0.f ? -1.f : 1.f;
   hipStream_t st = as_stream(stream);
-  auto kern = kv_fp8 ? mla_tree_kernel<true> : mla_tree_kernel<false>;
+  auto kern = !kv_fp8       ? mla_tree_kernel<false, false>
+              : kv_fp8 == 2 ? mla_tree_kernel<true, true>
+                            : mla_tree_kernel<true, false>;
   const size_t lds = kv_fp8 ? sizeof(TreeSmem<true>) : sizeof(TreeSmem<false>);
   int rc = reserve_lds(reinterpret_cast<const void*>(kern), lds, "mla_tree");
   if (rc != MI355_DSA_OK) return rc;

@@ -51,7 +51,7 @@ def _check_trees(n_tok: int, block_table: torch.Tensor, seq_lens: torch.Tensor,
 def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor,
                    seq_lens: torch.Tensor, cu_seqlens_q: torch.Tensor, tree_mask: torch.Tensor,
                    scale: float, out: torch.Tensor | None = None,
-                   lse: torch.Tensor | None = None):
+                   lse: torch.Tensor | None = None, pe_dtype: torch.dtype = torch.float16):
     """q [T, H, 576] fp16 (q_latent form); request r's drafted tokens are the rows
     cu_seqlens_q[r] .. cu_seqlens_q[r + 1] - 1 (int32 [R + 1]), n of them, already
     written to the cache at positions seq_lens[r] - n .. seq_lens[r] - 1.  Token j
@@ -72,15 +72,18 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
     if lse is None:
         lse = torch.empty(T, H, dtype=torch.float32, device=q.device)
     run = ops.op("mla_tree_attention") if _traced(q) else _attention
-    run(out, lse, q, kv_cache, block_table, seq_lens, cu_seqlens_q, tree_mask, scale)
+    run(out, lse, q, kv_cache, block_table, seq_lens, cu_seqlens_q, tree_mask, scale, pe_dtype)
     return out, lse
 
 
-def _attention(out, lse, q, kv_cache, block_table, seq_lens, cu_seqlens_q, tree_mask, scale):
+def _attention(out, lse, q, kv_cache, block_table, seq_lens, cu_seqlens_q, tree_mask, scale,
+               pe_dtype):
     _check(q.is_cuda and kv_cache.device == q.device, "q and kv_cache must be on the GPU")
     _check(q.dtype == torch.float16, "q must be fp16")
     _check(q.dim() == 3 and q.size(2) == 576, "q must be [tokens, heads, 576]")
     fp8, n_rows = _latent_rows(kv_cache)
+    _check(pe_dtype in ((torch.float16, torch.bfloat16) if fp8 else (torch.float16,)),
+           "pe_dtype must be fp16, or bf16 for fp8_ds_mla rows")
     T, H = q.size(0), q.size(1)
     _check(H > 0, "n_head must be > 0")
     _check_trees(T, block_table, seq_lens, cu_seqlens_q, tree_mask, q.device)
@@ -96,11 +99,11 @@ def _attention(out, lse, q, kv_cache, block_table, seq_lens, cu_seqlens_q, tree_
     need = _lib.lib().mi355_dsa_mla_tree_workspace_size(T, H)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     _launch("mi355_dsa_mla_tree_attention", q.device, out.data_ptr(), lse.data_ptr(), q.data_ptr(),
-            T, H, kv_cache.data_ptr(), fp8, n_rows, kv_cache.size(-2), block_table.data_ptr(),
-            block_table.size(1), seq_lens.data_ptr(), cu_seqlens_q.data_ptr(), R,
-            tree_mask.data_ptr(), scale, ws.data_ptr(), need)
+            T, H, kv_cache.data_ptr(), 2 if pe_dtype == torch.bfloat16 else fp8, n_rows,
+            kv_cache.size(-2), block_table.data_ptr(), block_table.size(1), seq_lens.data_ptr(),
+            cu_seqlens_q.data_ptr(), R, tree_mask.data_ptr(), scale, ws.data_ptr(), need)
 
 
 ops.define("mla_tree_attention(Tensor(a!) o, Tensor(b!) lse, Tensor q, Tensor kv_cache, "
            "Tensor block_table, Tensor seq_lens, Tensor cu_seqlens_q, Tensor tree_mask, "
-           "float scale) -> ()", _attention)
+           "float scale, ScalarType pe_dtype) -> ()", _attention)
