@@ -26,8 +26,8 @@ def concat_and_cache_mla(kv_c: torch.Tensor, k_pe: torch.Tensor, kv_cache: torch
     "auto": kv_cache fp16 [n_blocks, page, 576] = [kv_c | k_pe].
     "fp8_ds_mla": kv_cache uint8 [n_blocks, page, 656]: 512 e4m3 bytes with a
     max(amax/448, FLT_MIN) scale per 128-dim tile, the 4 fp32 scales, then the
-    64 16-bit RoPE values in k_pe's type (sparse attention reads fp16).  `scale` is unused by both (vLLM reads it only for
-    per-tensor fp8 caches)."""
+    64 16-bit RoPE values in k_pe's type (sparse attention reads fp16).
+    `scale` is unused by both (vLLM reads it only for per-tensor fp8 caches)."""
     _op("concat_and_cache_mla")(kv_c, k_pe, kv_cache, slot_mapping, kv_cache_dtype, scale)
 
 
@@ -56,8 +56,9 @@ def rope_concat_and_cache_mla(positions: torch.Tensor, table: torch.Tensor, kv_c
     not changed.  The 64 rope values of an fp8_ds_mla row are stored in k_pe's type, as
     the writer alone does: gather_latent_cache and mla_tree.tree_attention take that type
     (pe_dtype), sparse and dense attention read fp16 (DsaLayer stores fp16 for them).
-    A token with a negative slot writes no row, its q is rotated all the same; one with a position outside the table is not rotated.  Valid slots
-    must be distinct.  Returns q_out, or None without q."""
+    A token with a negative slot writes no row, its q is rotated all the same; one with a
+    position outside the table is not rotated.  Valid slots must be distinct.  Returns
+    q_out, or None without q."""
     _no_grad(kv_c, k_pe, q)
     if not _traced(kv_c):
         return _rope_write(positions, table, kv_c, k_pe, kv_cache, slot_mapping, kv_cache_dtype,

@@ -425,6 +425,8 @@ class DsaLayer:
             _check(idx_q.shape == (T, 32, 128) and idx_w.shape == (T, 32),
                    "idx_q must be [T, 32, 128] and idx_w [T, 32]")
             _check(idx_w.device == q.device, "idx_w must be on q's GPU")
+            page = self.idx_k_cache.shape[1]
+            _check(page & (page - 1) == 0, "indexer cache page size must be a power of two")
         for x in (idx_k, idx_q if choose else None):
             _check(x is None or (x.dtype in rope._DTYPE_CODE and x.device == q.device
                                  and x.stride(-1) == 1),
