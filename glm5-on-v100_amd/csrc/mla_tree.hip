@@ -29,14 +29,16 @@
 // products.
 //
 // What bounds it: the clock under the matrix cores' power.  One request of 1024 rows
-// over 184320 fp16 keys (411 GFLOP): 375 us, 1.10 PFLOP/s; on zeros, at full clock,
-// 298 us; an fp16 library product of 16384^3 reaches 1.31 PFLOP/s on this card.
-// 16 requests of 2560 rows over 32768 fp8 keys (2924 GFLOP): 3.0 ms, 0.97 PFLOP/s; on
-// zeros 2.57 ms: 128 conversions a wave and tile do not all hide beside MFMAs.
-// Measured against it: converting from registers (loads a tile ahead) 3.12 ms; pairs
-// of waves that share 64 rows and each take half of the dims (half of the LDS reads,
-// but scores and P exchanged through LDS, two barriers per tile) 385 us and 3.05 ms;
-// no overlap of softmax and products 430 us and 3.29 ms.
+// over 184320 fp16 keys (411 GFLOP): 381 us, 1.08 PFLOP/s; on zeros, at full clock,
+// 296 us; an fp16 library product of 16384^3 reaches 1.30 PFLOP/s on this card.
+// 16 requests of 2560 rows over 32768 fp8 keys (2924 GFLOP): 3.07 ms, 0.95 PFLOP/s; on
+// zeros 2.55 ms: 128 conversions a wave and tile do not all hide beside MFMAs, and every
+// one of a request's 20 groups converts all of its keys.
+// Measured against it (at 375 us and 3.0 ms, before scores were subtracted ahead of
+// their exponentials): converting from registers (loads a tile ahead) 3.12 ms; pairs of
+// waves that share 64 rows and each take half of the dims (half of the LDS reads, but
+// scores and P exchanged through LDS, two barriers per tile) 385 us and 3.05 ms; no
+// overlap of softmax and products 430 us and 3.29 ms.
 //
 // Division of the work: from the lengths on the device, either cells (a request's
 // keys cut in pieces, the groups of a piece side by side) or, with the key tiles of

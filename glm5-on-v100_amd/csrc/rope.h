@@ -161,8 +161,9 @@ __device__ __forceinline__ Bits<DT> bits_of(float v) {
 }
 
 // 16 bytes of an output.  NEW: it is another tensor than the input, and is stored
-// past the L2 (8192 tokens x 64 heads x 192 bf16 79.3 -> 60.0 us, 6.7 TB/s; in
-// place, where the lines are in the L2 anyway, 22.2 either way).
+// past the L2 (8192 tokens x 64 heads x 192 bf16, one input over and over, which the
+// caches partly hold: 79.3 -> 60.0 us; inputs that change 75.4 us, 5.4 TB/s; in place,
+// where the lines are in the L2 anyway, 22.2 either way).
 template <bool NEW>
 __device__ __forceinline__ void put_piece(u32x4* dst, const u32x4 v) {
   if constexpr (NEW) __builtin_nontemporal_store(v, dst);

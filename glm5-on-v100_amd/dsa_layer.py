@@ -59,7 +59,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _cache_ops, _lib, _sm70_ops, mla_tree, rope
-from .ops import _check, _rows16, _stream
+from .ops import _check, _no_grad, _rows16, _stream
 
 KT = 64  # key tile the prefill logits launch is rounded to (sparse_attn_indexer.py:753)
 
@@ -406,13 +406,15 @@ class DsaLayer:
         of more than topk positions needs idx_q [T, 32, 128], rotated as idx_k is, and
         idx_w [T, 32]: every token attends to the topk of its visible positions that the
         indexer chooses, as in decode (last_idx), with the indexer's keys in the cache or
-        given as idx_k.  q, k_pe, idx_k and idx_q stay as they are.  Returns out [T, H * V], zero for tokens of no request."""
+        given as idx_k.  q, k_pe, idx_k and idx_q stay as they are.  Returns out
+        [T, H * V], zero for tokens of no request."""
         T = slot_mapping.numel()
         _check(q.dim() == 3 and q.shape == (T, self.w.n_heads, self.w.nope_dim + 64),
                "q must be [T, H, P + 64], a slot for each token")
         _check(q.dtype == torch.float16, "q must be fp16")
         _check(positions.shape == (T,), "positions must be [T]")
         # the rest of what later launches would refuse: none may follow a written cache
+        _no_grad(q, kv_c, k_pe, idx_k, idx_q, idx_w)
         mla_tree._check_trees(T, block_table, seq_lens, cu_seqlens_q, tree_mask, q.device)
         P, R = self.w.nope_dim, block_table.shape[0]
         choose = R > 0 and block_table.shape[1] * self.latent_cache.shape[-2] > self.topk

@@ -20,6 +20,7 @@ I32 = dict(dtype=torch.int32)
     (dict(idx_k=torch.zeros(2, 64).half()), "idx_k must be"),
     (dict(idx_k=torch.zeros(2, 128, dtype=torch.float64)), "idx_k and idx_q must be"),
     (dict(idx_k=torch.zeros(2, 256).half()[:, ::2]), "idx_k and idx_q must be"),
+    (dict(idx_k=torch.zeros(2, 128).half().requires_grad_()), "no backward pass"),
     (dict(idx_k=torch.zeros(2, 128).half()), "GPU")])
 def test_refuses(pkg, kw, msg):
     m = pkg.dsa_layer
