@@ -132,7 +132,8 @@ __device__ __forceinline__ void tree_dma_rope(const uint8_t* row, uint8_t* slot,
 }
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 // The wave's share of a tile's rope values, come as bf16, to fp16 in place: 16 bytes a
-// lane, once they have landed and before the barrier that hands the tile over.
+// lane, once they have landed and before the barrier that hands the tile over (16
+// requests of 2560 rows over 32768 keys: 3 % longer than with fp16 values).
 __device__ __forceinline__ void tree_rope_f16(uint32_t slot, int w) {
   const uint32_t at = slot + 2048 * (16 + (w >> 1)) + 1024 * (w & 1) + 16 * (tree_tid() & 63);
   u32x4 x = *(const lds_u32x4*)at;

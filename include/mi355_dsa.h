@@ -157,6 +157,8 @@ int mi355_dsa_gather_latent_cache(void* out, int64_t out_stride, int out_dtype, 
  * count as the fp16 values that mi355_dsa_gather_latent_cache gives.  Scores and sums are fp32, P is rounded
  * to fp16 for the product with V.  A row that sees a drafted token whose cache
  * row holds an infinity or NaN is NaN; a row that does not is not touched by it.
+ * Context rows, which all see, count as they are (a score of -inf weighs 0).
+ * scale: any finite value whose product with log2 e is finite.
  * The workspace (16-byte aligned) carries nothing between calls.
  */
 size_t mi355_dsa_mla_tree_workspace_size(int64_t n_tok, int n_head);
