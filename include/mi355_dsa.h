@@ -154,8 +154,8 @@ int mi355_dsa_gather_latent_cache(void* out, int64_t out_stride, int out_dtype, 
  * [n_tok, n_head] (natural log); a row that sees nothing gets o = 0,
  * lse = -inf.  Rows of no request are left as they were.  kv_fp8 = 0: rows of
  * 576 fp16; 1: fp8_ds_mla rows with fp16 rope values, 2: with bf16 ones, which
- * count as the fp16 values that mi355_dsa_gather_latent_cache gives.  Scores and sums are fp32, P is rounded
- * to fp16 for the product with V.  A row that sees a drafted token whose cache
+ * count as the fp16 values that mi355_dsa_gather_latent_cache gives.  Scores
+ * and sums are fp32, P is rounded to fp16 for the product with V.  A row that sees a drafted token whose cache
  * row holds an infinity or NaN is NaN; a row that does not is not touched by it.
  * Context rows, which all see, count as they are (a score of -inf weighs 0).
  * scale: any finite value whose product with log2 e is finite.
