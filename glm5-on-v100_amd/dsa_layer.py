@@ -58,7 +58,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import _cache_ops, _lib, _sm70_ops, mla_tree, rope
+from . import _cache_ops, _lib, _sm70_ops, mla_tree, paging, rope
 from .ops import _check, _no_grad, _rows16, _stream
 
 KT = 64  # key tile the prefill logits launch is rounded to (sparse_attn_indexer.py:753)
@@ -217,9 +217,8 @@ class DsaLayer:
             spec = (torch.empty(B, bt.shape[1], dtype=torch.int32, device=q.device),
                     torch.empty(B, dtype=torch.int32, device=q.device))
         elif B != R:
-            offs = torch.arange(n, device=q.device, dtype=torch.int32)
-            sl = (sl.unsqueeze(1) - (n - 1) + offs).reshape(-1).contiguous()
-            bt = bt.repeat_interleave(n, dim=0).contiguous()
+            bt, sl = paging.token_tables(bt, sl, torch.arange(0, B + 1, n, device=q.device,
+                                                              dtype=torch.int32), B)
         if step:
             # one launch: both cache writes and the indexer logits; then the
             # top-k (leaving the layer's histogram zero) with q_latent beside it

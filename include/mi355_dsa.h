@@ -170,6 +170,65 @@ int mi355_dsa_mla_tree_attention(void* o, float* lse, const void* q, int64_t n_t
                                  size_t workspace_bytes, void* stream);
 
 /*
+ * Room for a step's tokens, in place: request r of length seq_lens[r] (int32
+ * [n_req]) gains new_tokens[r] (< 0: 0), its further pages come from the top of
+ * the stack free_pages (max_free entries, the first *free_count of them free)
+ * into block_table (int32 [n_req, max_blocks]); with pages(n) = ceil(n /
+ * page_size), the j-th page taken over the requests in order is
+ * free_pages[*free_count - 1 - j].  seq_lens and *free_count are moved on.
+ * slot_mapping and positions int32 [max_tokens]: of the tokens request by
+ * request, as new_tokens has them; -1 behind the last one.  cu_seqlens_q int32
+ * [n_req + 1]: sums of new_tokens, at most max_tokens.  granted [n_req]: 0
+ * where a request is refused -- its table, max_tokens or 2^31 positions do not
+ * hold it, or the pages asked for by it and all before it are more than there
+ * are and it needs some; then its table and length stay and its tokens have
+ * slot and position -1.  It has no counterpart in the reference, whose
+ * scheduler does it on the host.
+ */
+int mi355_dsa_extend_tables(int32_t* block_table, int32_t* seq_lens, const int32_t* new_tokens,
+                            int n_req, int max_blocks, const int32_t* free_pages,
+                            int32_t* free_count, int max_free, int page_size,
+                            int32_t* slot_mapping, int32_t* positions, int64_t max_tokens,
+                            int32_t* cu_seqlens_q, uint8_t* granted, void* stream);
+
+/*
+ * Requests cut back to new_lens (int32 [n_req]; what is not below seq_lens[r]
+ * changes nothing), in place: entries pages(new) .. pages(old) - 1 of a request
+ * become -1, those that were >= 0 go back to the stack, the j-th of m over the
+ * requests in order to free_pages[*free_count + m - 1 - j] (dropped past
+ * max_free), so that mi355_dsa_extend_tables and this leave it as it was.
+ */
+size_t mi355_dsa_truncate_tables_workspace_size(int n_req);
+int mi355_dsa_truncate_tables(int32_t* block_table, int32_t* seq_lens, const int32_t* new_lens,
+                              int n_req, int max_blocks, int32_t* free_pages, int32_t* free_count,
+                              int max_free, int page_size, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/*
+ * Per-token tables: out int32 [n_tok, cols] row t <- the first cols entries of
+ * block_table row r (rows bt_stride entries apart) and lens[t] <- max(0,
+ * seq_lens[r] - cu_seqlens_q[r + 1] + t + 1) for the request r with
+ * cu_seqlens_q[r] <= t < cu_seqlens_q[r + 1]; -1 and 0 for a row of no request.
+ * The reference expands them with tensor ops (reference/triton_mla.py:267-279,
+ * :454-466).
+ */
+int mi355_dsa_token_tables(int32_t* out, int32_t* lens, int64_t n_tok, int cols,
+                           const int32_t* block_table, int64_t bt_stride, const int32_t* seq_lens,
+                           const int32_t* cu_seqlens_q, int n_req, void* stream);
+
+/*
+ * out[g] (int32 [n_group]) <- the leading positions that requests cu_shared[g]
+ * .. cu_shared[g + 1] - 1 hold in the same pages: page_size times the leading
+ * entries in which their block-table rows agree, at most the shortest of their
+ * lengths; 0 for a group of no request.
+ */
+size_t mi355_dsa_shared_lengths_workspace_size(int n_req);
+int mi355_dsa_shared_lengths(int32_t* out, const int32_t* cu_shared, int n_group,
+                             const int32_t* block_table, const int32_t* seq_lens, int n_req,
+                             int max_blocks, int page_size, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/*
  * Dense MLA decode over a paged fp16 latent cache: for each token b and head
  * h, attention of q[b,h,:576] * scale over the cache rows of positions
  * [0, seq_lens[b]) (row(p) = bt[b, p/page]*page + p%page; a position whose
