@@ -9,10 +9,10 @@ registers it as the module `glm5_on_v100_amd` (see __graft_entry__.py or
 tests/conftest.py).
 """
 from . import (_lib, ops, _sm70_ops, _cache_ops, dsa_layer, mla_prefill, mla_tree,  # noqa: F401
-               paging, rope, synthetic)
+               paging, rope, synthetic, w4)
 
 __all__ = ["_lib", "ops", "_sm70_ops", "_cache_ops", "dsa_layer", "mla_prefill", "mla_tree",
-           "paging", "rope", "synthetic", "load_library"]
+           "paging", "rope", "synthetic", "w4", "load_library"]
 
 
 def load_library():

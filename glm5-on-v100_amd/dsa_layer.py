@@ -217,8 +217,8 @@ class DsaLayer:
             spec = (torch.empty(B, bt.shape[1], dtype=torch.int32, device=q.device),
                     torch.empty(B, dtype=torch.int32, device=q.device))
         elif B != R:
-            bt, sl = paging.token_tables(bt, sl, torch.arange(0, B + 1, n, device=q.device,
-                                                              dtype=torch.int32), B)
+            cu = torch.arange(R + 1, device=q.device, dtype=torch.int32) * n
+            bt, sl = paging.token_tables(bt, sl, cu, B)
         if step:
             # one launch: both cache writes and the indexer logits; then the
             # top-k (leaving the layer's histogram zero) with q_latent beside it

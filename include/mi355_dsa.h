@@ -562,6 +562,43 @@ int mi355_dsa_attn_fp8_dequant(void* out, const uint8_t* w, const float* s,
  */
 int mi355_dsa_attn_fp8_quantize(uint8_t* q, float* s, const void* w, int N, int K, void* stream);
 
+/*
+ * Projections with 4-bit weights: a weight of row n and column k is
+ * (code - z) * s, code 0..15, s and z (0..15) those of row n and group k / group
+ * (32, 64 or 128 columns; K a multiple of 8).  dtype: 0 fp16, 1 bf16, of x, y,
+ * the scales and the values.  They have no counterpart on the reference's path.
+ *
+ * q, 16 bytes a lane, 16-byte aligned: word i of lane 16 g + c (c < 16) of tile
+ * (n / 16, k / 128), tiles row by row with ceil(K / 128) a row, holds row
+ * 16 (n / 16) + c, columns 128 (k / 128) + 32 i + 8 g .. +7, bits 4 e .. +3 the
+ * column 2 e (e < 4) or 2 e - 7 of them.  sz: for each tile its 128 / group
+ * groups, 16 words each: the row's scale in the low half, 16 + z as a dtype
+ * number in the high half.  Rows past N have any code and a scale of any
+ * finite value.
+ */
+
+/* y [M, N] (contiguous) = x [M, K] (rows x_stride elements apart, 16-byte
+ * aligned) times the transposed weights, M <= 64: fp32 sums of unrounded
+ * weights, rounded once. */
+int mi355_dsa_w4_linear(void* y, const void* x, int64_t x_stride, const int32_t* q,
+                        const int32_t* sz, int dtype, int M, int N, int K, int group, void* stream);
+
+/* q and sz of w [N, K] (contiguous): per group, with lo <= 0 <= hi its least and
+ * largest value and 0, s = (hi - lo) / 15, z = RN(-lo / s), or (symmetric)
+ * s = max(hi / 7, -lo / 8), z = 8; s rounded to dtype and at least 2^-24 (bf16:
+ * 2^-126); code = clamp(RN(w / s) + z, 0, 15). */
+int mi355_dsa_w4_quantize(int32_t* q, int32_t* sz, const void* w, int dtype, int N, int K,
+                          int group, int symmetric, void* stream);
+
+/* q and sz of given codes uint8 [N, K] (their low four bits; 8-byte aligned),
+ * scales [N, ceil(K / group)] and zero points uint8 of that shape (null: 8). */
+int mi355_dsa_w4_pack(int32_t* q, int32_t* sz, const uint8_t* codes, const void* s,
+                      const uint8_t* z, int dtype, int N, int K, int group, void* stream);
+
+/* out [N, K] (contiguous, 16-byte aligned) = RN((code - z) * s). */
+int mi355_dsa_w4_dequant(void* out, const int32_t* q, const int32_t* sz, int dtype, int N, int K,
+                         int group, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
