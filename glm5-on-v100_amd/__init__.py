@@ -8,10 +8,10 @@ The directory name contains dashes, so it is imported through a loader that
 registers it as the module `glm5_on_v100_amd` (see __graft_entry__.py or
 tests/conftest.py).
 """
-from . import (_lib, ops, _sm70_ops, _cache_ops, dsa_layer, mla_prefill, mla_tree,  # noqa: F401
-               paging, rope, synthetic, w4)
+from . import (_lib, ops, _sm70_ops, _cache_ops, dsa_layer, mla_prefill, mla_prefix,  # noqa: F401
+               mla_tree, paging, rope, synthetic, w4)
 
-__all__ = ["_lib", "ops", "_sm70_ops", "_cache_ops", "dsa_layer", "mla_prefill", "mla_tree",
+__all__ = ["_lib", "ops", "_sm70_ops", "_cache_ops", "dsa_layer", "mla_prefill", "mla_prefix", "mla_tree",
            "paging", "rope", "synthetic", "w4", "load_library"]
 
 

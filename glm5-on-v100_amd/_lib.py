@@ -57,6 +57,10 @@ SIGNATURES = {
     "mi355_dsa_mla_tree_attention": (_c_int, [_p, _p, _p, _c_i64, _c_int, _p, _c_int, _c_i64,
                                               _c_int, _p, _c_int, _p, _p, _c_int, _p, _c_f32, _p,
                                               _c_size, _p]),
+    "mi355_dsa_mla_prefix_workspace_size": (_c_size, [_c_i64, _c_int, _c_int, _c_int]),
+    "mi355_dsa_mla_prefix_attention": (_c_int, [_p, _p, _p, _c_i64, _c_int, _p, _c_int, _c_i64,
+                                                _c_int, _p, _c_int, _p, _p, _c_int, _p, _p, _p,
+                                                _c_int, _c_f32, _p, _c_size, _p]),
     "mi355_dsa_extend_tables": (_c_int, [_p, _p, _p, _c_int, _c_int, _p, _p, _c_int, _c_int, _p,
                                          _p, _c_i64, _p, _p, _p]),
     "mi355_dsa_truncate_tables_workspace_size": (_c_size, [_c_int]),

@@ -170,6 +170,28 @@ int mi355_dsa_mla_tree_attention(void* o, float* lse, const void* q, int64_t n_t
                                  size_t workspace_bytes, void* stream);
 
 /*
+ * Attention of requests that share a prefix: mi355_dsa_mla_tree_attention (the
+ * same arguments and results) where the requests cu_shared[g] .. cu_shared[g + 1]
+ * - 1 (int32 [n_set + 1]) of set g hold their first shared_lens[g] positions
+ * (int32 [n_set]) in the same cache rows.  Those, at most the positions before
+ * the first drafted token of every request of the set, are read through the
+ * block-table row of its first request, once for all of its rows.  cu_seqlens_q
+ * and tree_mask null: one token a request (n_tok = n_req).  Rows of requests of
+ * no set are left as they were.  max_blocks * page_size < 2^24.  A shared
+ * position counts as it is, an own one whose cache row holds an infinity or NaN
+ * does not touch the rows that do not see it (those that do may get NaN for it).
+ * It has no counterpart in the reference.
+ */
+size_t mi355_dsa_mla_prefix_workspace_size(int64_t n_tok, int n_head, int n_req, int n_set);
+int mi355_dsa_mla_prefix_attention(void* o, float* lse, const void* q, int64_t n_tok, int n_head,
+                                   const void* kv_cache, int kv_fp8, int64_t n_kv_rows,
+                                   int page_size, const int32_t* block_table, int max_blocks,
+                                   const int32_t* seq_lens, const int32_t* cu_seqlens_q, int n_req,
+                                   const int64_t* tree_mask, const int32_t* cu_shared,
+                                   const int32_t* shared_lens, int n_set, float scale,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Room for a step's tokens, in place: request r of length seq_lens[r] (int32
  * [n_req]) gains new_tokens[r] (< 0: 0), its further pages come from the top of
  * the stack free_pages (max_free entries, the first *free_count of them free)
