@@ -111,8 +111,9 @@ SIGNATURES = {
     "mi355_dsa_sparse_mla_decode_noalloc": (_c_int, [_p, _p, _p, _c_int, _c_int, _p, _c_int,
                                                      _c_i64, _c_int, _p, _c_int, _p, _c_int, _p,
                                                      _c_f32, _p]),
+    "mi355_dsa_w4_linear_workspace_size": (_c_size, [_c_int, _c_int, _c_int]),
     "mi355_dsa_w4_linear": (_c_int, [_p, _p, _c_i64, _p, _p, _c_int, _c_int, _c_int, _c_int, _c_int,
-                                     _p]),
+                                     _p, _c_size, _p]),
     "mi355_dsa_w4_quantize": (_c_int, [_p, _p, _p, _c_int, _c_int, _c_int, _c_int, _c_int, _p]),
     "mi355_dsa_w4_pack": (_c_int, [_p, _p, _p, _p, _p, _c_int, _c_int, _c_int, _c_int, _p]),
     "mi355_dsa_w4_dequant": (_c_int, [_p, _p, _p, _c_int, _c_int, _c_int, _c_int, _p]),

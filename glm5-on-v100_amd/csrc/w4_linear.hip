@@ -11,10 +11,11 @@
 // 16 + z in its high half.
 //
 // A code becomes the operand 16 + c by or-ing it into the mantissa of 16 (exact in fp16
-// and bf16): two instructions a pair.  With t = sum_k x (16 + c) and X = sum_k x over a
-// group, the group's part of y is s (t - (16 + z) X), in fp32; X is one more MFMA against
-// ones.  No weight is rounded: the error is that of fp32 sums, of terms up to 31/15 as large
-// as they would be without the 16, and y's own rounding.
+// and bf16): two instructions a pair.  In fp16 a packed subtraction of 16 + z then leaves
+// c - z, exact too, and with t = sum_k x (c - z) over a group its part of y is s t, in fp32.
+// bf16 has no packed subtraction: t = sum_k x (16 + c) and X = sum_k x, one more MFMA against
+// ones, give s (t - (16 + z) X).  No weight is rounded: the error is that of fp32
+// sums (bf16: of terms up to 31/15 as large), and y's own rounding.
 #include "capi_internal.h"
 #include "dsa_common.h"
 
@@ -68,66 +69,204 @@ struct W4Params {
   const u32x4* q;      // [tiles][KB][64]
   const uint32_t* sz;  // [tiles][KB * GPB][16]
   uint16_t* y;
+  f32x4* part;  // S > 1: [S][groups of NT tiles][NT MT][64], else null
   int64_t x_stride;
-  int M, N, K, KB, tiles;
+  int M, N, K, KB, tiles, S;
 };
 
-// MT tiles of 16 rows of x, NT tiles of the weights a workgroup, whose WAVES waves take
-// turns at the blocks of 128 columns; GPB groups a block.
-template <bool BF16, int MT, int NT, int WAVES, int GPB>
-__global__ void __launch_bounds__(64 * WAVES) w4_linear_kernel(W4Params p) {
+// global_load_lds_dwordx4 and _dword: lane l's bytes at base + off land at lds + 16 l (4 l);
+// base and lds wave-uniform.  The caller waits for them by s_waitcnt vmcnt.
+__device__ __forceinline__ void w4_dma16(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+}
+__device__ __forceinline__ void w4_dma4(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("global_load_lds_dword %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+}
+__device__ __align__(16) const uint32_t kW4Zero[4] = {};
+typedef __attribute__((address_space(3))) const u32x4 lds_cu32x4;
+typedef __attribute__((address_space(3))) const uint32_t lds_cu32;
+
+// The shape of a launch for MT tiles of 16 rows of x, of which XI x 4 rows come to LDS: WAVES
+// waves a workgroup, D blocks of weights and XD blocks of x of a wave on their way.
+template <int MT, int XI>
+struct W4Shape;
+template <>
+struct W4Shape<1, 1> {
+  static constexpr int kWaves = 8, kD = 3, kXD = 3;
+};
+template <>
+struct W4Shape<1, 4> {
+  static constexpr int kWaves = 4, kD = 3, kXD = 3;
+};
+template <>
+struct W4Shape<2, 8> {
+  static constexpr int kWaves = 4, kD = 2, kXD = 1;
+};
+template <>
+struct W4Shape<4, 16> {
+  static constexpr int kWaves = 4, kD = 1, kXD = 1;
+};
+template <int MT, int XI, int NT, int GPB>
+struct W4Ring {
+  using Shape = W4Shape<MT, XI>;
+  static constexpr int kSz = (NT * GPB + 3) / 4;   // loads of a block's scales
+  static constexpr int kQ = NT * 1024 + kSz * 256;  // bytes of a block of weights
+  static constexpr int kWave = Shape::kD * kQ + Shape::kXD * XI * 1024;
+  static constexpr int kLoads = NT + kSz;
+  static constexpr int kRed = Shape::kWaves / 2 * NT * MT * 1024;  // the join of the waves
+  static constexpr int kLds = kWave * Shape::kWaves > kRed ? kWave * Shape::kWaves : kRed;
+  static_assert(kLds <= 160 * 1024, "a workgroup's LDS");
+};
+
+// NT tiles a workgroup, GPB groups a block of 128 columns.  The blocks are cut in S x WAVES
+// runs, each of one wave.  A wave brings its blocks of weights, scales and x to a ring of its
+// own in LDS (no barrier), reads a block into registers and at once sends for the one that
+// takes its place.  x, which all workgroups read, is what bounds many rows: rows of x go to
+// every workgroup, 786 KB for 64 of 6144 columns, so that NT is large there, and the
+// workgroups begin their runs at different blocks (x's rows, 12 KB apart, would ask the
+// same L2 channels; 1 us of 20).
+//
+// us with memory cold, [24576 x 6144] and [6144 x 24576]: 1 row 17.7 and 16.8 (4.6 TB/s),
+// 16 rows 18.8 and 18.1, 32 rows 21.5 and 20.3, 64 rows 30.0 and 29.8, the latter ones
+// without the join of S > 1 (2 to 4 us).  A kernel that loads x and weights into registers: 17, 21,
+// 26, 46 at the first.  By 64 rows what bounds it is x through the L2: 1.1 MB to each
+// CU, 10 TB/s in all.
+template <bool BF16, int MT, int XI, int NT, int GPB>
+__global__ void __launch_bounds__(64 * (XI == 1 ? 8 : 4)) w4_linear_kernel(W4Params p) {
+  using R = W4Ring<MT, XI, NT, GPB>;
+  constexpr int WAVES = R::Shape::kWaves, D = R::Shape::kD, XD = R::Shape::kXD;
+  static_assert(XD == D || XD == 1, "x goes with the weights, or one block ahead");
+  // fp16: the zero point comes off the codes (exact), one packed subtraction a pair; bf16
+  // has none, there X is formed
+  constexpr bool SUB = !BF16;
   constexpr int kSteps = 4 / GPB;  // MFMAs of a group
+  extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-  const int tile0 = blockIdx.x * NT;
+  const int group = blockIdx.x / p.S, slice = blockIdx.x % p.S;
+  const int tile0 = group * NT;
+  const int unit = slice * WAVES + wave, units = WAVES * p.S;
+  const int kb0 = (int)((int64_t)p.KB * unit / units);
+  const int n_kb = (int)((int64_t)p.KB * (unit + 1) / units) - kb0;
+  const int turn = n_kb > 0 ? group * 5 % n_kb : 0;
+  // the i-th block of the run; past its end (and in a run of none) some block of the matrix
+  auto nth = [&](int i) {
+    const int k = min(i, max(n_kb - 1, 0)) + turn;
+    return min(kb0 + (k >= n_kb ? k - n_kb : k), p.KB - 1);
+  };
+  const uint32_t ring = (uint32_t)(uintptr_t)smem + wave * R::kWave, xring = ring + D * R::kQ;
   f32x4 acc[NT][MT];
 #pragma unroll
   for (int j = 0; j < NT; j++)
 #pragma unroll
     for (int i = 0; i < MT; i++) acc[j][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  // rows past M repeat the last one and are not stored
-  const uint16_t* xr[MT];
-#pragma unroll
-  for (int i = 0; i < MT; i++) xr[i] = p.x + (int64_t)min(16 * i + c, p.M - 1) * p.x_stride + 8 * g;
-  const u32x4 ones = {BF16 ? 0x3f803f80u : 0x3c003c00u, BF16 ? 0x3f803f80u : 0x3c003c00u,
-                      BF16 ? 0x3f803f80u : 0x3c003c00u, BF16 ? 0x3f803f80u : 0x3c003c00u};
+  constexpr uint32_t kOne = BF16 ? 0x3f803f80u : 0x3c003c00u;
+  const u32x4 ones = {kOne, kOne, kOne, kOne};
 
-  for (int kb = wave; kb < p.KB; kb += WAVES) {
-    u32x4 q[NT], x[MT][4];
+  // In LDS the 16-byte piece k of row r of x stands at piece k ^ (r % 16), so that the
+  // reads of a piece of 16 rows cover the banks.  Rows past M repeat the last one.
+  uint32_t xo[XI], so[R::kSz];
+#pragma unroll
+  for (int j = 0; j < XI; j++) {
+    const int row = 4 * j + (lane >> 4);
+    xo[j] = (uint32_t)(min(row, p.M - 1) * (int)p.x_stride * 2 + 16 * ((lane & 15) ^ (row & 15)));
+  }
+#pragma unroll
+  for (int i = 0; i < R::kSz; i++) {
+    const int w = 64 * i + lane, t = min(w / (16 * GPB), min(NT, p.tiles - tile0) - 1);
+    so[i] = (uint32_t)(t * p.KB * GPB * 64 + (w % (16 * GPB)) * 4);
+  }
+  auto send_q = [&](int i, int slot) {
+    const int kb = nth(i);
+    const uint32_t to = ring + slot * R::kQ;
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+      w4_dma16(p.q + ((int64_t)min(tile0 + j, p.tiles - 1) * p.KB + kb) * 64, 16 * lane, to + 1024 * j);
+#pragma unroll
+    for (int e = 0; e < R::kSz; e++)
+      w4_dma4(p.sz + ((int64_t)tile0 * p.KB + kb) * GPB * 16, so[e], to + 1024 * NT + 256 * e);
+  };
+  auto send_x = [&](int i, int slot) {
+    const int kb = nth(i);
+    const uint32_t to = xring + slot * XI * 1024;
+    if ((kb + 1) * kW4Cols <= p.K) {
+#pragma unroll
+      for (int j = 0; j < XI; j++) w4_dma16(p.x + (int64_t)kb * kW4Cols, xo[j], to + 1024 * j);
+    } else {  // columns past K are zeros
+#pragma unroll
+      for (int j = 0; j < XI; j++) {
+        const int row = 4 * j + (lane >> 4), k = kb * kW4Cols + 8 * ((lane & 15) ^ (row & 15));
+        const void* src = k < p.K ? (const void*)(p.x + (int64_t)min(row, p.M - 1) * p.x_stride + k)
+                                  : (const void*)kW4Zero;
+        dma16(src, (const void*)(uintptr_t)(to + 1024 * j));
+      }
+    }
+  };
+  if (p.KB > 0) {
+    if constexpr (XD == 1) send_x(0, 0);
+#pragma unroll
+    for (int d = 0; d < D; d++) {
+      if constexpr (XD > 1) send_x(d, d);
+      send_q(d, d);
+    }
+  }
+  int slot = 0;
+#pragma unroll 1
+  for (int it = 0; it < n_kb; it++) {
+    // the block is in: what was sent after it may be on its way
+    constexpr int kLater = XD > 1 ? (D - 1) * (R::kLoads + XI) : (D > 1 ? R::kLoads : 0);
+    static_assert(kLater < 64, "vmcnt");
+    if (XD == 1 && D > 2 && it == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLater) : "memory");
+    u32x4 x[MT][4], q[NT];
     uint32_t sz[NT][GPB];
+    const uint32_t from = ring + slot * R::kQ, xfrom = xring + (XD > 1 ? slot * XI * 1024 : 0);
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+      const int row = min(16 * i + c, p.M - 1);
+#pragma unroll
+      for (int s = 0; s < 4; s++)
+        x[i][s] = *(lds_cu32x4*)(xfrom + row * 256 + 16 * ((4 * s + g) ^ (row & 15)));
+    }
 #pragma unroll
     for (int j = 0; j < NT; j++) {
-      const int64_t at = (int64_t)min(tile0 + j, p.tiles - 1) * p.KB + kb;
-      q[j] = p.q[at * 64 + lane];
+      q[j] = *(lds_cu32x4*)(from + 1024 * j + 16 * lane);
 #pragma unroll
-      for (int e = 0; e < GPB; e++) sz[j][e] = p.sz[(at * GPB + e) * 16 + c];
+      for (int e = 0; e < GPB; e++)
+        sz[j][e] = *(lds_cu32*)(from + 1024 * NT + ((j * GPB + e) * 16 + c) * 4);
     }
-    const bool whole = (kb + 1) * kW4Cols <= p.K;
-#pragma unroll
-    for (int i = 0; i < MT; i++)
-#pragma unroll
-      for (int s = 0; s < 4; s++) {
-        const int k = kb * kW4Cols + 32 * s;
-        x[i][s] = (u32x4){0u, 0u, 0u, 0u};
-        if (whole || k + 8 * g < p.K) x[i][s] = *reinterpret_cast<const u32x4*>(xr[i] + k);
-      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read: the places are free
+    if constexpr (XD > 1) send_x(it + D, slot);
+    else send_x(it + 1, 0);
+    send_q(it + D, slot);
+    slot = slot + 1 == D ? 0 : slot + 1;
 #pragma unroll
     for (int e = 0; e < GPB; e++) {
       f32x4 sum[MT];
+      if constexpr (!SUB) {
 #pragma unroll
-      for (int i = 0; i < MT; i++) {
-        sum[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < MT; i++) {
+          sum[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < kSteps; s++) sum[i] = w4_mfma<BF16>(x[i][kSteps * e + s], ones, sum[i]);
+          for (int s = 0; s < kSteps; s++) sum[i] = w4_mfma<BF16>(x[i][kSteps * e + s], ones, sum[i]);
+        }
       }
 #pragma unroll
       for (int j = 0; j < NT; j++) {
         f32x4 t[MT];
 #pragma unroll
         for (int i = 0; i < MT; i++) t[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        const f16x2 zero = __builtin_bit_cast(f16x2, (sz[j][e] >> 16) * 0x10001u);
 #pragma unroll
         for (int s = 0; s < kSteps; s++) {
-          const u32x4 b = w4_operand<BF16>(q[j][kSteps * e + s]);
+          u32x4 b = w4_operand<BF16>(q[j][kSteps * e + s]);
+          if constexpr (SUB) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const uint32_t pair = b[k];  // a bit_cast of an element itself reads the first one
+              b[k] = __builtin_bit_cast(uint32_t, (f16x2)(__builtin_bit_cast(f16x2, pair) - zero));
+            }
+          }
 #pragma unroll
           for (int i = 0; i < MT; i++) t[i] = w4_mfma<BF16>(x[i][kSteps * e + s], b, t[i]);
         }
@@ -136,35 +275,113 @@ __global__ void __launch_bounds__(64 * WAVES) w4_linear_kernel(W4Params p) {
         for (int i = 0; i < MT; i++)
 #pragma unroll
           for (int r = 0; r < 4; r++)
-            acc[j][i][r] = __builtin_fmaf(sc, __builtin_fmaf(-z, sum[i][r], t[i][r]), acc[j][i][r]);
+            acc[j][i][r] = __builtin_fmaf(
+                sc, SUB ? t[i][r] : __builtin_fmaf(-z, sum[i][r], t[i][r]), acc[j][i][r]);
       }
     }
   }
-
-  // join the waves: D layout, lane (c, g), register r: row 4 g + r of x, row c of the tile
-  __shared__ f32x4 red[WAVES][NT * MT][64];
-#pragma unroll
-  for (int j = 0; j < NT; j++)
-#pragma unroll
-    for (int i = 0; i < MT; i++) red[wave][j * MT + i][lane] = acc[j][i];
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was sent past the end
   __syncthreads();
-  for (int e = threadIdx.x; e < NT * MT * 64; e += 64 * WAVES) {
-    const int l = e & 63, i = (e >> 6) % MT, j = (e >> 6) / MT;
-    f32x4 v = red[0][e >> 6][l];
+
+  // Join the waves, half of them handing over to the other half until one is left.
+  // D layout, lane (c, g), register r: row 4 g + r of x, row c of the tile.
+  f32x4* red = reinterpret_cast<f32x4*>(smem);
 #pragma unroll
-    for (int w = 1; w < WAVES; w++) {
-      const f32x4 u = red[w][e >> 6][l];
+  for (int half = WAVES / 2; half >= 1; half /= 2) {
+    if (wave >= half && wave < 2 * half) {
 #pragma unroll
-      for (int r = 0; r < 4; r++) v[r] += u[r];
+      for (int j = 0; j < NT; j++)
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+          red[((wave - half) * NT * MT + j * MT + i) * 64 + lane] = acc[j][i];
     }
-    const int n = (tile0 + j) * kW4Rows + (l & 15);
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int j = 0; j < NT; j++)
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+          const f32x4 u = red[(wave * NT * MT + j * MT + i) * 64 + lane];
+#pragma unroll
+          for (int r = 0; r < 4; r++) acc[j][i][r] += u[r];
+        }
+    }
+    if (half > 1) __syncthreads();
+  }
+  if (wave > 0) return;
+  if (p.part != nullptr) {
+    f32x4* to = p.part + ((int64_t)slice * (gridDim.x / p.S) + group) * (NT * MT * 64);
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+      for (int i = 0; i < MT; i++) to[(j * MT + i) * 64 + lane] = acc[j][i];
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < NT; j++) {
+    const int n = (tile0 + j) * kW4Rows + c;
     if (n >= p.N) continue;
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int m = 16 * i + 4 * (l >> 4) + r;
-      if (m < p.M) p.y[(int64_t)m * p.N + n] = (uint16_t)w4_bits<BF16>(v[r]);
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int m = 16 * i + 4 * g + r;
+        if (m < p.M) p.y[(int64_t)m * p.N + n] = (uint16_t)w4_bits<BF16>(acc[j][i][r]);
+      }
+  }
+}
+
+// The sums of the S slices, in their order: a wave a tile of y
+template <bool BF16>
+__global__ void __launch_bounds__(256) w4_join_kernel(W4Params p, int MT, int units) {
+  const int unit = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int i = unit % MT, tile = unit / MT, n = tile * kW4Rows + (lane & 15);
+  if (tile >= p.tiles) return;
+  const f32x4* from = p.part + (int64_t)unit * 64 + lane;
+  f32x4 v = from[0];
+  for (int s = 1; s < p.S; s++) {
+    const f32x4 u = from[(int64_t)s * units * 64];
+#pragma unroll
+    for (int r = 0; r < 4; r++) v[r] += u[r];
+  }
+  if (n >= p.N) return;
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    const int m = 16 * i + 4 * (lane >> 4) + r;
+    if (m < p.M) p.y[(int64_t)m * p.N + n] = (uint16_t)w4_bits<BF16>(v[r]);
+  }
+}
+
+// Tiles of a workgroup and slices of K, by the time that they are expected to take: the
+// workgroups of a CU one after the other, each its blocks at the time that a block of NT tiles was
+// measured to take (us, at sizes that fill the chip), and the join (4 us with its launch).  Slices pay where N
+// alone leaves CUs idle: 64 rows at [6144 x 24576] 54 us with one, 30 and the join
+// with four; at [24576 x 6144] one is best.
+struct W4Plan {
+  int nt, s;
+};
+static int w4_row_tiles(int M) { return M <= 16 ? 1 : M <= 32 ? 2 : 4; }
+static W4Plan w4_plan(int M, int N, int K) {
+  const int tiles = (N + kW4Rows - 1) / kW4Rows, KB = (K + kW4Cols - 1) / kW4Cols;
+  const bool few = M <= 4;
+  const float base = few ? 0.022f : M <= 16 ? 0.06f : M <= 32 ? 0.08f : 0.15f;
+  const float each = few ? 0.045f : M <= 16 ? 0.052f : M <= 32 ? 0.058f : 0.076f;
+  W4Plan best = {1, 1};
+  float least = 1e30f;
+  for (const int nt : {1, 2, 3, 6}) {
+    if (few && nt > 2) break;
+    const int64_t groups = (tiles + nt - 1) / nt;
+    for (int s = 1; s <= 16 && (s == 1 || 8 * s <= KB); s *= 2) {
+      const int64_t rounds = (groups * s + 255) / 256;
+      float t = (float)rounds * (float)((KB + s - 1) / s) * (base + each * (float)nt);
+      if (s > 1) t += 4.f + (float)s * (float)w4_row_tiles(M) * (float)tiles * 2048.f / 6e6f;
+      if (t < least) {
+        least = t;
+        best = {nt, s};
+      }
     }
   }
+  return best;
 }
 
 // ---- the weights ----
@@ -302,18 +519,43 @@ __global__ void __launch_bounds__(256) w4_dequant_kernel(W4Weights p) {
   }
 }
 
-template <bool BF16, int MT, int NT, int WAVES>
-static void w4_launch_group(const W4Params& p, int gpb, hipStream_t st) {
-  const dim3 grid((unsigned)((p.tiles + NT - 1) / NT));
-  if (gpb == 1) w4_linear_kernel<BF16, MT, NT, WAVES, 1><<<grid, 64 * WAVES, 0, st>>>(p);
-  else if (gpb == 2) w4_linear_kernel<BF16, MT, NT, WAVES, 2><<<grid, 64 * WAVES, 0, st>>>(p);
-  else w4_linear_kernel<BF16, MT, NT, WAVES, 4><<<grid, 64 * WAVES, 0, st>>>(p);
+template <bool BF16, int MT, int XI, int NT, int GPB>
+static int w4_run(const W4Params& p, hipStream_t st) {
+  using R = W4Ring<MT, XI, NT, GPB>;
+  auto kern = w4_linear_kernel<BF16, MT, XI, NT, GPB>;
+  int rc = reserve_lds(reinterpret_cast<const void*>(kern), R::kLds, "w4_linear");
+  if (rc != MI355_DSA_OK) return rc;
+  const int groups = (p.tiles + NT - 1) / NT;
+  kern<<<dim3((unsigned)(groups * p.S)), 64 * R::Shape::kWaves, R::kLds, st>>>(p);
+  DSA_LAUNCH_CHECK("w4_linear");
+  if (p.S == 1) return MI355_DSA_OK;
+  const int units = groups * NT * MT;
+  w4_join_kernel<BF16><<<dim3((unsigned)((units + 3) / 4)), 256, 0, st>>>(p, MT, units);
+  DSA_LAUNCH_CHECK("w4_linear join");
+  return MI355_DSA_OK;
+}
+template <bool BF16, int MT, int XI, int NT>
+static int w4_run_gpb(const W4Params& p, int gpb, hipStream_t st) {
+  return gpb == 1   ? w4_run<BF16, MT, XI, NT, 1>(p, st)
+         : gpb == 2 ? w4_run<BF16, MT, XI, NT, 2>(p, st)
+                    : w4_run<BF16, MT, XI, NT, 4>(p, st);
+}
+template <bool BF16, int MT, int XI>
+static int w4_run_nt(const W4Params& p, int nt, int gpb, hipStream_t st) {
+  if (nt == 1) return w4_run_gpb<BF16, MT, XI, 1>(p, gpb, st);
+  if (nt == 2) return w4_run_gpb<BF16, MT, XI, 2>(p, gpb, st);
+  if constexpr (XI > 1) {
+    if (nt == 3) return w4_run_gpb<BF16, MT, XI, 3>(p, gpb, st);
+    return w4_run_gpb<BF16, MT, XI, 6>(p, gpb, st);
+  }
+  return set_error(MI355_DSA_EINVAL, "w4_linear: no such plan");
 }
 template <bool BF16>
-static void w4_launch(const W4Params& p, int gpb, hipStream_t st) {
-  if (p.M <= 16) w4_launch_group<BF16, 1, 1, 8>(p, gpb, st);
-  else if (p.M <= 32) w4_launch_group<BF16, 2, 1, 8>(p, gpb, st);
-  else w4_launch_group<BF16, 4, 1, 8>(p, gpb, st);
+static int w4_launch(const W4Params& p, int nt, int gpb, hipStream_t st) {
+  if (p.M <= 4) return w4_run_nt<BF16, 1, 1>(p, nt, gpb, st);
+  if (p.M <= 16) return w4_run_nt<BF16, 1, 4>(p, nt, gpb, st);
+  if (p.M <= 32) return w4_run_nt<BF16, 2, 8>(p, nt, gpb, st);
+  return w4_run_nt<BF16, 4, 16>(p, nt, gpb, st);
 }
 
 static int w4_check(int N, int K, int group, int dtype) {
@@ -345,9 +587,17 @@ static int64_t w4_blocks(int K) { return ((int64_t)K + kW4Cols - 1) / kW4Cols; }
 
 using namespace mi355dsa;
 
+extern "C" size_t mi355_dsa_w4_linear_workspace_size(int M, int N, int K) {
+  if (M <= 0 || M > kW4MaxM || N <= 0 || K <= 0) return 0;
+  const W4Plan plan = w4_plan(M, N, K);
+  if (plan.s == 1) return 0;
+  const int64_t groups = (w4_tiles(N) + plan.nt - 1) / plan.nt;
+  return (size_t)plan.s * groups * plan.nt * w4_row_tiles(M) * 1024;
+}
+
 extern "C" int mi355_dsa_w4_linear(void* y, const void* x, int64_t x_stride, const int32_t* q,
                                    const int32_t* sz, int dtype, int M, int N, int K, int group,
-                                   void* stream) {
+                                   void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   int rc = w4_check(N, K, group, dtype);
   if (rc != MI355_DSA_OK) return rc;
@@ -369,11 +619,19 @@ extern "C" int mi355_dsa_w4_linear(void* y, const void* x, int64_t x_stride, con
   p.K = K;
   p.KB = (int)w4_blocks(K);
   p.tiles = (int)w4_tiles(N);
-  DSA_CHECK((int64_t)p.tiles * 512 <= kMaxThreads, "w4_linear: too many rows");
-  if (dtype == 0) w4_launch<false>(p, kW4Cols / group, as_stream(stream));
-  else w4_launch<true>(p, kW4Cols / group, as_stream(stream));
-  DSA_LAUNCH_CHECK("w4_linear");
-  return MI355_DSA_OK;
+  // a few tiles' scales, and x, within 32-bit offsets; as many workgroups as a grid takes
+  DSA_CHECK(K < (1 << 24), "w4_linear: too many columns");
+  DSA_CHECK((M - 1) * x_stride < ((int64_t)1 << 29), "w4_linear: bad row stride of x");
+  DSA_CHECK((int64_t)p.tiles * 16 * 512 <= kMaxThreads, "w4_linear: too many rows");
+  const W4Plan plan = w4_plan(M, N, K);
+  const size_t need = mi355_dsa_w4_linear_workspace_size(M, N, K);
+  DSA_CHECK(need == 0 || (workspace && workspace_bytes >= need),
+            "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+  DSA_CHECK(need == 0 || aligned_to(workspace, 16), "workspace must be 16-byte aligned");
+  p.S = plan.s;
+  p.part = need ? reinterpret_cast<f32x4*>(workspace) : nullptr;
+  return dtype == 0 ? w4_launch<false>(p, plan.nt, kW4Cols / group, as_stream(stream))
+                    : w4_launch<true>(p, plan.nt, kW4Cols / group, as_stream(stream));
 }
 
 extern "C" int mi355_dsa_w4_quantize(int32_t* q, int32_t* sz, const void* w, int dtype, int N, int K,

@@ -8,7 +8,7 @@ A weight of row n and column k is (code - zero point) * scale, codes and zero po
 """
 from __future__ import annotations
 
-from typing import NamedTuple
+from dataclasses import dataclass
 
 import torch
 
@@ -19,7 +19,8 @@ MAX_ROWS = 64  # of x in w4_linear
 _DTYPE_CODE = {torch.float16: 0, torch.bfloat16: 1}
 
 
-class W4Weight(NamedTuple):
+@dataclass(frozen=True)
+class W4Weight:
     """Weights [n, k] as the kernels read them: q int32 [ceil(n / 16), ceil(k / 128), 64, 4],
     sz int32 [ceil(n / 16), ceil(k / 128) * 128 / group, 16] (mi355_dsa.h has the layout)."""
     q: torch.Tensor
@@ -29,11 +30,19 @@ class W4Weight(NamedTuple):
     group: int
     dtype: torch.dtype
 
+    def __post_init__(self):
+        _check(self.dtype in _DTYPE_CODE, "w4: fp16 or bf16 weights")
+        _check(self.group in (32, 64, 128), "w4: group must be 32, 64 or 128")
+        _check(self.k % 8 == 0, "w4: K must be a multiple of 8")
+        t, b = -(-self.n // 16), -(-self.k // 128)
+        _check(self.q.shape == (t, b, 64, 4) and self.sz.shape == (t, b * (128 // self.group), 16)
+               and self.q.dtype == torch.int32 and self.sz.dtype == torch.int32
+               and self.q.is_contiguous() and self.sz.is_contiguous()
+               and self.sz.device == self.q.device, "w4: q and sz are not of weights [n, k]")
+
 
 def _empty(n: int, k: int, group: int, dtype: torch.dtype, dev) -> W4Weight:
-    _check(dtype in _DTYPE_CODE, "w4: fp16 or bf16 weights")
     _check(group in (32, 64, 128), "w4: group must be 32, 64 or 128")
-    _check(k % 8 == 0, "w4: K must be a multiple of 8")
     t, b = -(-n // 16), -(-k // 128)
     return W4Weight(torch.empty(t, b, 64, 4, dtype=torch.int32, device=dev),
                     torch.empty(t, b * (128 // group), 16, dtype=torch.int32, device=dev),
@@ -87,21 +96,11 @@ def _pack(q, sz, codes, scales, zeros, group):
             None if z is None else z.data_ptr(), _DTYPE_CODE[s.dtype], c.size(0), c.size(1), group)
 
 
-def _check_weight(w: W4Weight) -> None:
-    want = (-(-w.n // 16), -(-w.k // 128))
-    _check(w.dtype in _DTYPE_CODE and w.group in (32, 64, 128) and w.k % 8 == 0
-           and w.q.shape == (*want, 64, 4) and w.q.dtype == torch.int32 and w.q.is_contiguous()
-           and w.sz.shape == (want[0], want[1] * (128 // w.group), 16)
-           and w.sz.dtype == torch.int32 and w.sz.is_contiguous() and w.sz.device == w.q.device,
-           "w4: not a weight that w4_quantize or w4_pack made")
-
-
 def w4_linear(x: torch.Tensor, w: W4Weight, out: torch.Tensor | None = None) -> torch.Tensor:
     """x [M, K] times the transposed weights: [M, N] in x's type (the weights'), M at most
     64 rows.  Weights enter unrounded, sums are fp32.  Prefill-sized products: w4_dequant
     and a matrix product."""
     _no_grad(x)
-    _check_weight(w)
     _check(x.dim() == 2 and x.size(1) == w.k, "x must be [M, K]")
     _check(x.dtype == w.dtype, "x must have the weights' type")
     _check(x.size(0) <= MAX_ROWS, f"w4_linear: at most {MAX_ROWS} rows, got {x.size(0)}")
@@ -118,15 +117,20 @@ def w4_linear(x: torch.Tensor, w: W4Weight, out: torch.Tensor | None = None) -> 
 def _linear(y, x, q, sz, group):
     _check(x.is_cuda and q.device == x.device and sz.device == x.device,
            "all tensors must be on one GPU")
-    if x.size(0):
+    M, K = x.shape
+    if M:
         x = _rows16(x)
+        if M * x.stride(0) >= 1 << 29:  # the kernel's offsets are 32-bit
+            x = x.contiguous()
+    N = y.size(1)
+    need = _lib.lib().mi355_dsa_w4_linear_workspace_size(M, N, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     _launch("mi355_dsa_w4_linear", x.device, y.data_ptr(), x.data_ptr(), x.stride(0), q.data_ptr(),
-            sz.data_ptr(), _DTYPE_CODE[x.dtype], x.size(0), y.size(1), x.size(1), group)
+            sz.data_ptr(), _DTYPE_CODE[x.dtype], M, N, K, group, ops._ptr(ws), need)
 
 
 def w4_dequant(w: W4Weight) -> torch.Tensor:
     """The weights as values [N, K] of their type, RN((code - zero point) * scale)."""
-    _check_weight(w)
     out = torch.empty(w.n, w.k, dtype=w.dtype, device=w.q.device)
     run = ops.op("w4_dequant") if _traced(w.q) else _dequant
     run(out, w.q, w.sz, w.group)

@@ -600,10 +600,13 @@ int mi355_dsa_attn_fp8_quantize(uint8_t* q, float* s, const void* w, int N, int 
  */
 
 /* y [M, N] (contiguous) = x [M, K] (rows x_stride elements apart, 16-byte
- * aligned) times the transposed weights, M <= 64: fp32 sums of unrounded
- * weights, rounded once. */
+ * aligned) times the transposed weights, M <= 64, K < 2^24: fp32 sums of
+ * unrounded weights, rounded once.  The workspace (16-byte aligned) carries
+ * nothing between calls; 0 bytes means none. */
+size_t mi355_dsa_w4_linear_workspace_size(int M, int N, int K);
 int mi355_dsa_w4_linear(void* y, const void* x, int64_t x_stride, const int32_t* q,
-                        const int32_t* sz, int dtype, int M, int N, int K, int group, void* stream);
+                        const int32_t* sz, int dtype, int M, int N, int K, int group,
+                        void* workspace, size_t workspace_bytes, void* stream);
 
 /* q and sz of w [N, K] (contiguous): per group, with lo <= 0 <= hi its least and
  * largest value and 0, s = (hi - lo) / 15, z = RN(-lo / s), or (symmetric)

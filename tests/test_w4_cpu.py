@@ -1,4 +1,6 @@
 """Refusals of the 4-bit projections without a GPU, and their calls under tracing."""
+from dataclasses import replace
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -12,7 +14,7 @@ def err(pkg):
 
 
 def linear(lib, **kw):
-    d = dict(y=64, x=64, stride=256, q=64, sz=64, dtype=0, M=2, N=16, K=256, group=128)
+    d = dict(y=64, x=64, stride=256, q=64, sz=64, dtype=0, M=2, N=16, K=256, group=128, ws=None, n=0)
     d.update(kw)
     return lib.mi355_dsa_w4_linear(*d.values(), None)
 
@@ -23,10 +25,21 @@ def linear(lib, **kw):
     (dict(group=256), "group must be"), (dict(dtype=2), "dtype must be"), (dict(stride=252), "stride"),
     (dict(stride=248), "stride"), (dict(x=66), "misaligned"), (dict(q=72), "misaligned"),
     (dict(sz=66), "misaligned"), (dict(N=(1 << 31) - 1, M=1), "too many rows"),
+    (dict(K=1 << 24, stride=1 << 24), "too many columns"), (dict(stride=1 << 29), "row stride"),
+    (dict(M=64, N=6144, K=24576, stride=24576), "workspace too small"),
+    (dict(M=64, N=6144, K=24576, stride=24576, ws=72, n=1 << 40), "16-byte aligned"),
     *[({k: None}, "null pointer") for k in ("y", "x", "q", "sz")]])
 def test_linear(pkg, lib, kw, msg):
     assert linear(lib, **kw) == 1 and msg in err(pkg)
     assert linear(lib, M=0, y=None) == 0 and linear(lib, N=0, q=None) == 0
+
+
+def test_workspace_sizes(lib):
+    size = lib.mi355_dsa_w4_linear_workspace_size
+    assert size(0, 16, 128) == size(1, 0, 128) == size(1, 16, 0) == size(65, 16, 128) == 0
+    assert size(64, 24576, 6144) == 0          # enough workgroups without slices
+    n = size(64, 6144, 24576)                  # slices of whole fp32 tiles
+    assert n and n % (64 * 6144 * 4) == 0
 
 
 def quant(lib, **kw):
@@ -83,8 +96,9 @@ def test_python_refusals(pkg, lib):
             W.w4_linear(x, w)
     with pytest.raises(RuntimeError, match="out must"):
         W.w4_linear(torch.zeros(2, 64, dtype=F16), w, torch.zeros(2, 21, dtype=F16))
-    with pytest.raises(RuntimeError, match="not a weight"):
-        W.w4_linear(torch.zeros(2, 64, dtype=F16), w._replace(group=64))
+    for kw in (dict(group=64), dict(n=33), dict(k=136), dict(q=w.q.float()), dict(sz=w.sz[:, ::2])):
+        with pytest.raises(RuntimeError, match="not of weights"):
+            replace(w, **kw)
 
 
 def test_traced(pkg, lib):
