@@ -24,7 +24,13 @@
 namespace mi355dsa {
 
 constexpr int kPlanThreads = 1024;
+// Requests, sets and row groups (one a thread), and positions of a block table, up to which
+// the division keeps its tables in LDS and its sums in 32 bits
+constexpr int kPlanFew = 256;
+constexpr int64_t kPlanWidth = 1 << 20;  // 256 row groups of 129 runs of 2^15 tiles: below 2^31
 
+// Inclusive sum over the workgroup's threads, and the total
+template <int NT>
 __device__ __forceinline__ int64_t plan_scan(int64_t v, int64_t* ws, int64_t* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -36,7 +42,7 @@ __device__ __forceinline__ int64_t plan_scan(int64_t v, int64_t* ws, int64_t* to
   __syncthreads();
   int64_t before = 0, all = 0;
 #pragma unroll
-  for (int i = 0; i < kPlanThreads / 64; i++) {
+  for (int i = 0; i < NT / 64; i++) {
     const int64_t x = ws[i];
     before += i < wave ? x : 0;
     all += x;
@@ -45,130 +51,215 @@ __device__ __forceinline__ int64_t plan_scan(int64_t v, int64_t* ws, int64_t* to
   *total = all;
   return before + v;
 }
-// The last i in [0, n) with x[i] <= v, x ascending
-__device__ __forceinline__ int plan_last(const int32_t* x, int n, int v) {
+template <int NT>
+__device__ __forceinline__ int plan_scan(int v, int* ws, int* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int x = (int)wave_incl_scan((uint32_t)v);
+  if (lane == 63) ws[wave] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 64; i++) {
+    const int y = ws[i];
+    before += i < wave ? y : 0;
+    all += y;
+  }
+  __syncthreads();
+  *total = all;
+  return before + x;
+}
+// The last i in [0, n) with x(i) <= v, x ascending
+template <typename F>
+__device__ __forceinline__ int plan_last(F&& x, int n, int v) {
   int lo = 0, hi = n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (x[mid] <= v) lo = mid;
+    if (x(mid) <= v) lo = mid;
     else hi = mid;
   }
   return lo;
 }
 
+template <bool FEW>
+struct PlanLds {};
+template <>
+struct PlanLds<true> {
+  int tok[kPlanFew], end[kPlanFew], len[kPlanFew], tiles[kPlanFew], upto[kPlanFew];
+  PrefixSet sets[kPlanFew];
+  int before[kPlanFew + 1], cu[kPlanFew + 1], shared[kPlanFew];
+};
+
 // One workgroup: the sets' shared positions, the requests' own tiles, the row groups and
-// the cut of their line.
-__global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(PrefixParams p) {
-  __shared__ int64_t ws[kPlanThreads / 64];
-  __shared__ PrefixRun s_cells[kTreeWGs];  // of a row group: set, cells, tiles of one
+// the cut of their line.  What bounds it is its chain of dependent steps: 5 us for 4 requests,
+// 8 for 128 (10 and 17 with all of it in global memory and 64-bit sums).
+template <bool FEW>
+__global__ void __launch_bounds__(FEW ? kPlanFew : kPlanThreads) prefix_plan_kernel(PrefixParams p) {
+  constexpr int NT = FEW ? kPlanFew : kPlanThreads;
+  typedef std::conditional_t<FEW, int, int64_t> Sum;
+  __shared__ Sum ws[NT / 64];
+  __shared__ PrefixRun s_cells[kTreeWGs];  // of a row group: set, cells, tiles of one, first place
+  __shared__ int s_units[64], s_uneven;
+  __shared__ PlanLds<FEW> l;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const TreeParams& t = p.t;
   const int64_t width = (int64_t)t.max_blocks * t.page_size;
-
-  for (int r = tid; r <= t.R; r += kPlanThreads) p.own[r] = 0;
+  auto tokens = [&](int r) {
+    if constexpr (FEW) return PrefixTokens{l.tok[r], l.end[r]};
+    else return prefix_tokens(t, r);
+  };
+  auto length = [&](int r) {
+    if constexpr (FEW) return l.len[r];
+    else return max(0, t.seq_lens[r]);
+  };
+  auto token0 = [&](int r) {  // ascending over the requests
+    if constexpr (FEW) return l.tok[r];
+    else return t.cu == nullptr ? r : t.cu[r];
+  };
+  auto upto = [&](int r) -> Sum {  // own tiles of the requests before r
+    if (r == 0) return 0;
+    if constexpr (FEW) return l.upto[r - 1];
+    else return p.reqs[r - 1].upto;
+  };
+  PrefixSet* sets;
+  int* before;
+  const int32_t *cu_shared, *shared;
+  if constexpr (FEW) {
+    sets = l.sets;
+    before = l.before;
+    cu_shared = l.cu;
+    shared = l.shared;
+    if (tid < t.R) {
+      const PrefixTokens k = prefix_tokens(t, tid);
+      l.tok[tid] = k.a;
+      l.end[tid] = k.b;
+      l.len[tid] = max(0, t.seq_lens[tid]);
+      l.tiles[tid] = 0;
+    }
+    if (tid <= p.S) l.cu[tid] = p.cu_shared[tid];
+    if (tid == 0) l.cu[p.S] = p.cu_shared[p.S];
+    if (tid < p.S) l.shared[tid] = p.shared[tid];
+  } else {
+    sets = p.sets;
+    before = p.before;
+    cu_shared = p.cu_shared;
+    shared = p.shared;
+    for (int r = tid; r < t.R; r += NT) p.reqs[r] = {};
+  }
   __syncthreads();
-  for (int s = wave; s < p.S; s += kPlanThreads / 64) {
-    const int lead = min(max(p.cu_shared[s], 0), t.R), end = min(max(p.cu_shared[s + 1], lead), t.R);
+  for (int s = wave; s < p.S; s += NT / 64) {
+    const int lead = min(max(cu_shared[s], 0), t.R), end = min(max(cu_shared[s + 1], lead), t.R);
     // what every token sees: positions before the first drafted one
     int ctx = INT32_MAX;
     for (int r = lead + lane; r < end; r += 64) {
-      const PrefixTokens k = prefix_tokens(t, r);
-      if (k.b > k.a) ctx = min(ctx, max(0, t.seq_lens[r]) - (k.b - k.a));
+      const PrefixTokens k = tokens(r);
+      if (k.b > k.a) ctx = min(ctx, length(r) - (k.b - k.a));
     }
     ctx = wave_min_i32(ctx);
     int P = 0;
-    if (ctx != INT32_MAX) P = (int)min((int64_t)max(0, min(p.shared[s], ctx)), width);
+    if (ctx != INT32_MAX) P = (int)min((int64_t)max(0, min(shared[s], ctx)), width);
     for (int r = lead + lane; r < end; r += 64) {
-      const PrefixTokens k = prefix_tokens(t, r);
-      const int64_t len = min((int64_t)max(0, t.seq_lens[r]), width);
-      p.own[r + 1] = k.b > k.a && len > P ? prefix_tiles(len - P) : 0;
+      const PrefixTokens k = tokens(r);
+      const int len = (int)min((int64_t)length(r), width);
+      const int tiles = k.b > k.a && len > P ? prefix_tiles(len - P) : 0;
+      if constexpr (FEW) l.tiles[r] = tiles;
+      else p.reqs[r].tiles = tiles;
     }
     if (lane == 0) {
       int first = 0, last = 0;
       if (lead < end) {
-        first = prefix_tokens(t, lead).a;
-        last = max(first, prefix_tokens(t, end - 1).b);
+        first = tokens(lead).a;
+        last = max(first, tokens(end - 1).b);
       }
-      p.sets[s] = {first, (last - first) * t.H, P, lead, end};
+      sets[s] = {first, (last - first) * t.H, P, lead, end};
     }
   }
   __syncthreads();
-  int64_t total = 0, carry = 0;
-  for (int s0 = 0; s0 < p.S; s0 += kPlanThreads) {
-    const int s = s0 + tid;
-    const int64_t n = s < p.S ? ((int64_t)p.sets[s].M + kTreeRows - 1) / kTreeRows : 0;
-    const int64_t upto = carry + plan_scan(n, ws, &total);
-    if (s < p.S) p.before[s] = (int)min(upto - n, (int64_t)INT32_MAX);
-    carry += total;
-  }
-  const int n_groups = (int)min(carry, (int64_t)p.most);  // more only if sets overlap
-  if (tid == 0) p.before[p.S] = n_groups;
-  carry = 0;
-  for (int r0 = 0; r0 < t.R; r0 += kPlanThreads) {
+  Sum total, carry = 0;
+  for (int r0 = 0; r0 < t.R; r0 += NT) {
     const int r = r0 + tid;
-    const int64_t n = r < t.R ? p.own[r + 1] : 0;
-    const int64_t upto = carry + plan_scan(n, ws, &total);
-    if (r < t.R) p.own[r + 1] = upto;
+    PrefixReq q = {};
+    if (r < t.R) {
+      if constexpr (FEW) q.tiles = l.tiles[r];
+      else q.tiles = p.reqs[r].tiles;
+    }
+    q.upto = carry + plan_scan<NT>((Sum)q.tiles, ws, &total);
+    if (r < t.R) {
+      const PrefixTokens k = tokens(r);
+      q.tok = k.a;
+      q.tok_end = k.b;
+      q.draft0 = length(r) - (k.b - k.a);
+      q.len = (int)min((int64_t)length(r), width);
+      p.reqs[r] = q;
+      if constexpr (FEW) l.upto[r] = (int)q.upto;
+    }
     carry += total;
   }
+  int64_t groups = 0;  // rows are below 2^30, and 2^8 sets below 2^31 row groups
+  for (int s0 = 0; s0 < p.S; s0 += NT) {
+    const int s = s0 + tid;
+    const Sum n = s < p.S ? (sets[s].M + kTreeRows - 1) / kTreeRows : 0;
+    const int64_t sum = groups + plan_scan<NT>(n, ws, &total);
+    if (s < p.S) before[s] = (int)min(sum - n, (int64_t)INT32_MAX);
+    groups += total;
+  }
+  const int n_groups = (int)min(groups, (int64_t)p.most);  // more only if sets overlap
+  if (tid == 0) before[p.S] = n_groups;
   __syncthreads();
   int64_t line = 0;
-  for (int g0 = 0; g0 < n_groups; g0 += kPlanThreads) {
+  PrefixGroup mine = {};  // row group tid
+  for (int g0 = 0; g0 < n_groups; g0 += NT) {
     const int i = g0 + tid;
     PrefixGroup q = {};
     int s = 0;
     if (i < n_groups) {
-      s = plan_last(p.before, p.S, i);
-      const PrefixSet set = p.sets[s];
+      s = plan_last([&](int k) { return before[k]; }, p.S, i);
+      const PrefixSet set = sets[s];
       q.first = set.first;
       q.M = set.M;
-      q.g = i - p.before[s];
+      q.g = i - before[s];
       q.P = set.P;
       q.lead = set.lead;
       const int m1 = min((q.g + 1) * kTreeRows, q.M) - 1;
       const int t0 = q.first + (uint32_t)(q.g * kTreeRows) / (uint32_t)t.H;
       const int t1 = q.first + (uint32_t)m1 / (uint32_t)t.H;
-      int r1;
-      if (t.cu == nullptr) {
-        q.r0 = min(t0, t.R - 1);
-        r1 = min(t1, t.R - 1);
-      } else {
-        q.r0 = set.lead + plan_last(t.cu + set.lead, set.end - set.lead, t0);
-        r1 = max(q.r0, set.lead + plan_last(t.cu + set.lead, set.end - set.lead, t1));
-      }
+      auto from = [&](int k) { return token0(set.lead + k); };
+      q.r0 = set.lead + plan_last(from, set.end - set.lead, t0);
+      const int r1 = max(q.r0, set.lead + plan_last(from, set.end - set.lead, t1));
       // at most 2^19 shared tiles and those of 128 requests
-      q.tiles = (int)max((int64_t)1, min(prefix_tiles(q.P) + p.own[r1 + 1] - p.own[q.r0],
-                                         (int64_t)1 << 30));
+      q.tiles = (int)max((int64_t)1,
+                         min((int64_t)prefix_tiles(q.P) + upto(r1 + 1) - upto(q.r0), (int64_t)1 << 30));
     }
-    const int64_t upto = line + plan_scan(q.tiles, ws, &total);
+    const int64_t sum = line + plan_scan<NT>((Sum)q.tiles, ws, &total);
     if (i < n_groups) {
       p.groups[i] = q;
-      p.line[i] = upto - q.tiles;
-      if (i < kTreeWGs) s_cells[i].group = s;
+      p.line[i] = sum - q.tiles;
+      if (i < kTreeWGs) {
+        s_cells[i].group = s;
+        s_cells[i].place = q.tiles;
+      }
+      if (g0 == 0) mine = q;
     }
     line += total;
   }
   if (tid == 0) p.line[n_groups] = line;
 
-  // as tree_plan: cells of kt tiles if 256 of them do, within a fifth of equal runs
+  // As tree_plan: cells of kt tiles if 256 of them do, within a fifth of equal runs.  64
+  // sizes are looked at together.
   const int64_t per = max((int64_t)kTreeMinTiles, (line + kTreeWGs - 1) / kTreeWGs);
   const int64_t most = max((int64_t)kTreeMinTiles, line / (kTreeWGs * 4 / 5));
-  int64_t kt = 0;
-  __syncthreads();
-  if (n_groups <= kTreeWGs) {
-    const int tiles = tid < n_groups ? p.groups[tid].tiles : 0;
-    kt = per;
-    while (true) {
-      int64_t units;
-      plan_scan(tiles ? (tiles + kt - 1) / kt : 0, ws, &units);
-      if (units <= kTreeWGs) break;
-      if (kt >= most) {
-        kt = 0;
-        break;
-      }
-      const int64_t over = kt * (min(units, (int64_t)2 * kTreeWGs) - kTreeWGs) / (2 * kTreeWGs);
-      kt = min(most, kt + max(max((int64_t)1, (most - per) / 8), over));
-    }
+  uint32_t kt = 0;
+  if (n_groups <= kTreeWGs) {  // tiles of a row group: below 2^31, kt too
+    __syncthreads();
+    const uint32_t size = (uint32_t)(per + (most - per) * lane / 63);
+    int units = 0;
+    for (int i = wave; i < n_groups; i += NT / 64)
+      units += (int)(((uint32_t)s_cells[i].place + size - 1) / size);
+    if (wave == 0) s_units[lane] = 0;
+    __syncthreads();
+    atomicAdd(&s_units[lane], units);
+    __syncthreads();
+    const uint64_t fits = __ballot(s_units[lane] <= kTreeWGs);
+    if (fits) kt = (uint32_t)(per + (most - per) * __builtin_ctzll(fits) / 63);
   }
   if (tid == 0) {
     t.plan[0] = kt;
@@ -178,15 +269,13 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(PrefixParams 
   if (kt == 0) return;
   // The cells of a set stand cell by cell, row group by row group, so that the workgroups
   // of an XCD read the same keys at the same time.
-  const int tiles = tid < n_groups ? p.groups[tid].tiles : 0;
   int n = 0, cell = 1;
-  if (tiles) {
-    n = (int)((tiles + kt - 1) / kt);
-    cell = (tiles + n - 1) / n;
-    n = (tiles + cell - 1) / cell;
+  if (mine.tiles) {
+    n = (int)(((uint32_t)mine.tiles + kt - 1) / kt);
+    cell = ((uint32_t)mine.tiles + n - 1) / (uint32_t)n;
+    n = ((uint32_t)mine.tiles + cell - 1) / (uint32_t)cell;
   }
-  int64_t units;
-  const int place0 = (int)(plan_scan(n, ws, &units) - n);
+  const int place0 = (int)plan_scan<NT>((Sum)n, ws, &total) - n, units = (int)total;
   if (tid < n_groups) {
     p.groups[tid].cells = n;
     p.groups[tid].place0 = place0;
@@ -195,25 +284,26 @@ __global__ void __launch_bounds__(kPlanThreads) prefix_plan_kernel(PrefixParams 
     s_cells[tid].place = place0;
   }
   if (tid >= units && tid < kTreeWGs) p.runs[tid] = {-1, 0, 0, -1};
+  if (tid == 0) s_uneven = 0;
+  __syncthreads();
+  if (tid < n_groups && n != s_cells[before[s_cells[tid].group]].lo) s_uneven = 1;
   __syncthreads();
   if (tid < units) {
     // the row group and cell of unit tid in row group order
-    int i = 0, hi = n_groups;
-    while (hi - i > 1) {
-      const int mid = (i + hi) >> 1;
-      if (s_cells[mid].place <= tid) i = mid;
-      else hi = mid;
-    }
+    const int i = plan_last([&](int k) { return s_cells[k].place; }, n_groups, tid);
     const PrefixRun me = s_cells[i];
-    const int c = tid - me.place;
-    int rank = 0;  // units before it in the order of the runs
-    for (int k = 0; k < n_groups; k++) {
-      const PrefixRun o = s_cells[k];
-      rank += o.group < me.group ? o.lo
-              : o.group > me.group ? 0 : min(o.lo, c) + (k < i && o.lo > c ? 1 : 0);
+    const int c = tid - me.place, lo = before[me.group], hi = min(before[me.group + 1], n_groups);
+    int rank = s_cells[lo].place;  // units before it in the order of the runs
+    if (!s_uneven) {
+      rank += c * (hi - lo) + i - lo;
+    } else {
+#pragma unroll 4
+      for (int k = lo; k < hi; k++) {
+        const int o = s_cells[k].lo;
+        rank += min(o, c) + (k < i && o > c ? 1 : 0);
+      }
     }
-    const int all = p.groups[i].tiles;
-    p.runs[rank] = {i, c * me.hi, min(all, (c + 1) * me.hi), me.lo == 1 ? -1 : tid};
+    p.runs[rank] = {i, c * me.hi, min(p.groups[i].tiles, (c + 1) * me.hi), me.lo == 1 ? -1 : tid};
   }
 }
 
@@ -249,7 +339,7 @@ extern "C" size_t mi355_dsa_mla_prefix_workspace_size(int64_t n_tok, int n_head,
   return up16((size_t)2 * kTreeWGs * prefix_part_waves(n_tok, n_head) * (kTreePartWave + 64) *
               sizeof(float)) +
          64 + up16(most * sizeof(PrefixGroup)) + up16(kTreeWGs * sizeof(PrefixRun)) +
-         up16((most + 1) * 8) + up16(((size_t)n_req + 1) * 8) + up16(n_set * sizeof(PrefixSet)) +
+         up16((most + 1) * 8) + up16((size_t)n_req * sizeof(PrefixReq)) + up16(n_set * sizeof(PrefixSet)) +
          up16(((size_t)n_set + 1) * 4);
 }
 
@@ -308,7 +398,7 @@ extern "C" int mi355_dsa_mla_prefix_attention(
   p.groups = reinterpret_cast<PrefixGroup*>(take((size_t)most * sizeof(PrefixGroup)));
   p.runs = reinterpret_cast<PrefixRun*>(take(kTreeWGs * sizeof(PrefixRun)));
   p.line = reinterpret_cast<int64_t*>(take(((size_t)most + 1) * 8));
-  p.own = reinterpret_cast<int64_t*>(take(((size_t)n_req + 1) * 8));
+  p.reqs = reinterpret_cast<PrefixReq*>(take((size_t)n_req * sizeof(PrefixReq)));
   p.sets = reinterpret_cast<PrefixSet*>(take((size_t)n_set * sizeof(PrefixSet)));
   p.before = reinterpret_cast<int32_t*>(take(((size_t)n_set + 1) * 4));
   t.R = n_req;
@@ -333,7 +423,10 @@ extern "C" int mi355_dsa_mla_prefix_attention(
   const size_t lds = kv_fp8 ? sizeof(PrefixSmem<true>) : sizeof(PrefixSmem<false>);
   int rc = reserve_lds(reinterpret_cast<const void*>(kern), lds, "mla_prefix");
   if (rc != MI355_DSA_OK) return rc;
-  prefix_plan_kernel<<<1, kPlanThreads, 0, st>>>(p);
+  if (n_req <= kPlanFew && n_set <= kPlanFew && most <= kPlanFew &&
+      (int64_t)max_blocks * page_size <= kPlanWidth)
+    prefix_plan_kernel<true><<<1, kPlanFew, 0, st>>>(p);
+  else prefix_plan_kernel<false><<<1, kPlanThreads, 0, st>>>(p);
   DSA_LAUNCH_CHECK("mla_prefix plan");
   kern<<<kTreeWGs, kTreeThreads, lds, st>>>(p);
   DSA_LAUNCH_CHECK("mla_prefix");

@@ -19,6 +19,12 @@ struct PrefixGroup {
 struct PrefixSet {  // requests that share
   int first, M, P, lead, end;  // lead .. end - 1
 };
+struct PrefixReq {  // a request
+  int64_t upto;  // sum of the own tiles of the requests up to and with it
+  int tiles;     // its own
+  int len, draft0;  // positions that can be visible, position of its first drafted token
+  int tok, tok_end;
+};
 struct PrefixRun {  // cells: the piece of a workgroup
   int group, lo, hi, place;
 };
@@ -32,7 +38,7 @@ struct PrefixParams {
   PrefixGroup* groups;  // [most]
   PrefixRun* runs;      // [kTreeWGs]
   int64_t* line;        // [most + 1] the row groups' places on the line of tiles
-  int64_t* own;         // [R + 1] sums of the requests' own tiles
+  PrefixReq* reqs;      // [R]
   PrefixSet* sets;      // [S]
   int32_t* before;      // [S + 1] row groups of the sets before
 };
@@ -119,21 +125,18 @@ __device__ __forceinline__ PrefixKeys prefix_keys(const PrefixParams& p, const P
   if (t < shared)
     return {it.lead, 0, it.P, INT32_MAX, t, min(shared, it.hi), 0, 0, 0, min(shared, it.hi)};
   // the request in whose own tiles t lies
-  const int64_t from = tree_uniform(p.own[it.r0]) + t - shared;
+  int64_t from = t - shared;
   for (int r = it.r0; r < p.t.R; r += 64) {
-    const int k = min(r + (tree_tid() & 63), p.t.R - 1);
-    const int64_t end = p.own[k + 1];
-    const uint64_t hit = __ballot(end > from);
+    const PrefixReq q = p.reqs[min(r + (tree_tid() & 63), p.t.R - 1)];
+    if (r == it.r0) from += shfl64(q.upto - q.tiles, 0);
+    const uint64_t hit = __ballot(q.upto > from);
     if (!hit) continue;
-    const int lane = __builtin_ctzll(hit), q = min(r + lane, p.t.R - 1);
-    const int64_t stop = shfl64(end, lane);
-    const int tiles = (int)(stop - tree_uniform(p.own[q]));
-    const int lo = (int)(from - (stop - tiles)), hi = (int)min((int64_t)tiles, (int64_t)lo + it.hi - t);
-    const PrefixTokens tok = prefix_tokens(p.t, q);
-    const int seq = __builtin_amdgcn_readfirstlane(max(0, p.t.seq_lens[q]));
-    const int64_t width = (int64_t)p.t.max_blocks * p.t.page_size;
-    const int a = __builtin_amdgcn_readfirstlane(tok.a), b = __builtin_amdgcn_readfirstlane(tok.b);
-    return {q, it.P, (int)min((int64_t)seq, width), seq - (b - a), lo, hi, 1, a, b, t + hi - lo};
+    const int k = __builtin_ctzll(hit);
+    auto get = [&](int x) { return __builtin_amdgcn_readlane(x, k); };
+    const int tiles = get(q.tiles), lo = (int)(from - (shfl64(q.upto, k) - tiles));
+    const int hi = (int)min((int64_t)tiles, (int64_t)lo + it.hi - t);
+    return {min(r + k, p.t.R - 1), it.P, get(q.len), get(q.draft0), lo, hi, 1, get(q.tok),
+            get(q.tok_end), t + hi - lo};
   }
   return {0, 0, 0, 0, 0, 0, 0, 0, 0, it.hi};
 }

@@ -402,10 +402,12 @@ __device__ __forceinline__ void tree_attention(const TreeParams& p) {
         qf[s] = *reinterpret_cast<const f16x8*>(qrow + 16 * s + 8 * hf);
       const int tok = it.first + (uint32_t)m / (uint32_t)p.H;
       sh.see[32 * wave() + c] = SHARED && p.mask == nullptr ? 1 : (uint64_t)p.mask[tok];
-      const f16 sg = (f16)p.q_sign;
-      const f16x8 sg8 = {sg, sg, sg, sg, sg, sg, sg, sg};
+      if (p.q_sign != 1.f) {  // else nothing waits for Q before the first product
+        const f16 sg = (f16)p.q_sign;
+        const f16x8 sg8 = {sg, sg, sg, sg, sg, sg, sg, sg};
 #pragma unroll
-      for (int s = 0; s < kLatentDim / 16; s++) qf[s] *= sg8;
+        for (int s = 0; s < kLatentDim / 16; s++) qf[s] *= sg8;
+      }
     }
 
     hw_own_agprs();

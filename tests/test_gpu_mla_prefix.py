@@ -114,6 +114,15 @@ def test_equal_runs(pkg, lib, dev):
     check(call(pkg, c, dev), oracle(c))
 
 
+@pytest.mark.parametrize("n,size", [(1100, 1100), (600, 1), (40, 30)])
+def test_many_requests(pkg, lib, dev, n, size):
+    """More requests, sets and row groups than the division holds in LDS: one set of many
+    requests, many sets of one, and more row groups than a workgroup has threads."""
+    sets = [(16, [(1 + (7 * i + s) % 40, 1) for i in range(size)]) for s in range(n // size if size > 30 else n)]
+    c = make(sets, 2 if size != 30 else 110, 16, "fp16", seed=n)
+    check(call(pkg, c, dev), oracle(c))
+
+
 def test_the_same_rows_whatever_is_said_to_be_shared(pkg, lib, dev):
     """Less than what is shared, none, too much (clamped to the shortest request's context),
     negative; one group, or each request alone."""
