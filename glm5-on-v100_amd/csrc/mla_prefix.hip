@@ -11,14 +11,16 @@
 // matrix product, 128 of them to a key tile, as a request's are in tree attention, whose
 // kernel this is (mla_tree_kernel.h): 32 requests of 64 heads read a 32k prefix 16 times
 // from one XCD's L2 instead of once a request from memory.  Each row group then goes on
-// with the own keys of its requests, one after the other, with the rows of the others
-// masked: the accumulators stay where they are, and no partial result is written for the
-// seam.  A row group's shared and own tiles stand in one line, which is cut as tree
-// attention cuts a request's: in cells that all row groups of a set begin at the same
-// time, or in equal runs where cells would leave workgroups idle.
+// with the own keys of its requests, packed in tiles one request after the other, where each
+// row sees those of its request: the accumulators stay where they are, and no partial
+// result is written for the seam.  A row group's shared and own tiles stand in one line, which is
+// cut as tree attention cuts a request's: in cells that all row groups of a set begin at
+// the same time, or in equal runs where cells would leave workgroups idle.
 //
-// An own key's row that holds an infinity or NaN is zeroed in LDS and counts as a NaN
-// score for the rows that see it, so that the others are untouched.
+// A key that is not finite gives a score that is not, to every row: where a wave finds one
+// among the scores that it masks, it clears that key's values in LDS before the product
+// with P, so that 0 times infinity does not reach the rows that do not see the key; in those
+// that do the score counts as NaN.
 #include "mla_tree_kernel.h"
 
 namespace mi355dsa {
@@ -27,7 +29,7 @@ constexpr int kPlanThreads = 1024;
 // Requests, sets and row groups (one a thread), and positions of a block table, up to which
 // the division keeps its tables in LDS and its sums in 32 bits
 constexpr int kPlanFew = 256;
-constexpr int64_t kPlanWidth = 1 << 20;  // 256 row groups of 129 runs of 2^15 tiles: below 2^31
+constexpr int64_t kPlanWidth = 1 << 20;  // 256 requests of 2^20 keys, 256 row groups of 129 x 2^15 tiles
 
 // Inclusive sum over the workgroup's threads, and the total
 template <int NT>
@@ -84,7 +86,7 @@ template <bool FEW>
 struct PlanLds {};
 template <>
 struct PlanLds<true> {
-  int tok[kPlanFew], end[kPlanFew], len[kPlanFew], tiles[kPlanFew], upto[kPlanFew];
+  int tok[kPlanFew], end[kPlanFew], len[kPlanFew], real[kPlanFew], upto[kPlanFew];
   PrefixSet sets[kPlanFew];
   int before[kPlanFew + 1], cu[kPlanFew + 1], shared[kPlanFew];
 };
@@ -115,7 +117,7 @@ __global__ void __launch_bounds__(FEW ? kPlanFew : kPlanThreads) prefix_plan_ker
     if constexpr (FEW) return l.tok[r];
     else return t.cu == nullptr ? r : t.cu[r];
   };
-  auto upto = [&](int r) -> Sum {  // own tiles of the requests before r
+  auto upto = [&](int r) -> Sum {  // own keys of the requests before r
     if (r == 0) return 0;
     if constexpr (FEW) return l.upto[r - 1];
     else return p.reqs[r - 1].upto;
@@ -133,7 +135,7 @@ __global__ void __launch_bounds__(FEW ? kPlanFew : kPlanThreads) prefix_plan_ker
       l.tok[tid] = k.a;
       l.end[tid] = k.b;
       l.len[tid] = max(0, t.seq_lens[tid]);
-      l.tiles[tid] = 0;
+      l.real[tid] = 0;
     }
     if (tid <= p.S) l.cu[tid] = p.cu_shared[tid];
     if (tid == 0) l.cu[p.S] = p.cu_shared[p.S];
@@ -160,9 +162,9 @@ __global__ void __launch_bounds__(FEW ? kPlanFew : kPlanThreads) prefix_plan_ker
     for (int r = lead + lane; r < end; r += 64) {
       const PrefixTokens k = tokens(r);
       const int len = (int)min((int64_t)length(r), width);
-      const int tiles = k.b > k.a && len > P ? prefix_tiles(len - P) : 0;
-      if constexpr (FEW) l.tiles[r] = tiles;
-      else p.reqs[r].tiles = tiles;
+      const int keys = k.b > k.a && len > P ? len - P : 0;
+      if constexpr (FEW) l.real[r] = keys;
+      else p.reqs[r].real = keys;
     }
     if (lane == 0) {
       int first = 0, last = 0;
@@ -179,17 +181,17 @@ __global__ void __launch_bounds__(FEW ? kPlanFew : kPlanThreads) prefix_plan_ker
     const int r = r0 + tid;
     PrefixReq q = {};
     if (r < t.R) {
-      if constexpr (FEW) q.tiles = l.tiles[r];
-      else q.tiles = p.reqs[r].tiles;
+      if constexpr (FEW) q.real = l.real[r];
+      else q.real = p.reqs[r].real;
+      q.own = t.H % 32 == 0 ? prefix_tiles(q.real) * kTreeTile : q.real;
     }
-    q.upto = carry + plan_scan<NT>((Sum)q.tiles, ws, &total);
+    q.upto = carry + plan_scan<NT>((Sum)q.own, ws, &total);
     if (r < t.R) {
       const PrefixTokens k = tokens(r);
-      q.tok = k.a;
-      q.tok_end = k.b;
       q.draft0 = length(r) - (k.b - k.a);
-      q.len = (int)min((int64_t)length(r), width);
       p.reqs[r] = q;
+      if (p.request != nullptr)
+        for (int i = k.a; i < k.b; i++) p.request[i] = r;
       if constexpr (FEW) l.upto[r] = (int)q.upto;
     }
     carry += total;
@@ -225,9 +227,9 @@ __global__ void __launch_bounds__(FEW ? kPlanFew : kPlanThreads) prefix_plan_ker
       auto from = [&](int k) { return token0(set.lead + k); };
       q.r0 = set.lead + plan_last(from, set.end - set.lead, t0);
       const int r1 = max(q.r0, set.lead + plan_last(from, set.end - set.lead, t1));
-      // at most 2^19 shared tiles and those of 128 requests
-      q.tiles = (int)max((int64_t)1,
-                         min((int64_t)prefix_tiles(q.P) + upto(r1 + 1) - upto(q.r0), (int64_t)1 << 30));
+      // at most 2^23 shared keys and those of 128 requests
+      q.own = (int)min((int64_t)upto(r1 + 1) - upto(q.r0), (int64_t)1 << 30);
+      q.tiles = max(1, prefix_tiles(q.P) + prefix_tiles(q.own));
     }
     const int64_t sum = line + plan_scan<NT>((Sum)q.tiles, ws, &total);
     if (i < n_groups) {
@@ -316,8 +318,8 @@ __global__ void __launch_bounds__(S == 1 ? 256 : 64 * S) prefix_merge_kernel(Pre
   tree_merge<S, true>(p.t);
 }
 
-// Positions of a block table at most: tiles of a row group stay within 32 bits
-constexpr int64_t kPrefixWidth = (int64_t)1 << 24;
+// Positions of a block table at most: keys of a row group, of 129 tables, stay within 31 bits
+constexpr int64_t kPrefixWidth = (int64_t)1 << 23;
 
 static int64_t prefix_most(int64_t T, int H, int S) {
   return T * H / kTreeRows + (S < T ? S : T);
@@ -339,7 +341,7 @@ extern "C" size_t mi355_dsa_mla_prefix_workspace_size(int64_t n_tok, int n_head,
   return up16((size_t)2 * kTreeWGs * prefix_part_waves(n_tok, n_head) * (kTreePartWave + 64) *
               sizeof(float)) +
          64 + up16(most * sizeof(PrefixGroup)) + up16(kTreeWGs * sizeof(PrefixRun)) +
-         up16((most + 1) * 8) + up16((size_t)n_req * sizeof(PrefixReq)) + up16(n_set * sizeof(PrefixSet)) +
+         up16((most + 1) * 8) + up16((size_t)n_req * sizeof(PrefixReq)) + up16((size_t)n_tok * 4) + up16(n_set * sizeof(PrefixSet)) +
          up16(((size_t)n_set + 1) * 4);
 }
 
@@ -399,6 +401,8 @@ extern "C" int mi355_dsa_mla_prefix_attention(
   p.runs = reinterpret_cast<PrefixRun*>(take(kTreeWGs * sizeof(PrefixRun)));
   p.line = reinterpret_cast<int64_t*>(take(((size_t)most + 1) * 8));
   p.reqs = reinterpret_cast<PrefixReq*>(take((size_t)n_req * sizeof(PrefixReq)));
+  int32_t* request = reinterpret_cast<int32_t*>(take((size_t)n_tok * 4));
+  p.request = cu_seqlens_q ? request : nullptr;
   p.sets = reinterpret_cast<PrefixSet*>(take((size_t)n_set * sizeof(PrefixSet)));
   p.before = reinterpret_cast<int32_t*>(take(((size_t)n_set + 1) * 4));
   t.R = n_req;

@@ -8,9 +8,11 @@
 namespace mi355dsa {
 
 // A row group: up to kTreeRows (token, head) rows of requests that share.  Its keys stand
-// in tiles: the shared ones, then the own ones of each of its requests in turn.
+// in tiles: the shared ones, and from the next tile on the own ones of its requests, each
+// request's behind the one before it -- from the next tile on where a wave's 32 rows are of
+// one request (heads a multiple of 32), so that the waves of others can be idle.
 struct PrefixGroup {
-  int tiles;
+  int tiles, own;  // own keys
   int first, M, g;  // first token of the sharing requests, their rows, which 128 of them
   int P, lead;      // shared positions, the request through whose table they are read
   int r0;           // its first request
@@ -20,10 +22,10 @@ struct PrefixSet {  // requests that share
   int first, M, P, lead, end;  // lead .. end - 1
 };
 struct PrefixReq {  // a request
-  int64_t upto;  // sum of the own tiles of the requests up to and with it
-  int tiles;     // its own
-  int len, draft0;  // positions that can be visible, position of its first drafted token
-  int tok, tok_end;
+  int64_t upto;  // sum of the own keys of the requests up to and with it
+  int own;       // its own, up to the next tile's (see PrefixGroup)
+  int real;      // without that
+  int draft0;    // position of its first drafted token
 };
 struct PrefixRun {  // cells: the piece of a workgroup
   int group, lo, hi, place;
@@ -39,6 +41,7 @@ struct PrefixParams {
   PrefixRun* runs;      // [kTreeWGs]
   int64_t* line;        // [most + 1] the row groups' places on the line of tiles
   PrefixReq* reqs;      // [R]
+  int32_t* request;     // [T] of a token (cu null: its number)
   PrefixSet* sets;      // [S]
   int32_t* before;      // [S + 1] row groups of the sets before
 };
@@ -57,7 +60,7 @@ __device__ __forceinline__ int prefix_tiles(int64_t keys) { return (int)((keys +
 // ---- a workgroup's pieces ----
 struct PrefixItem {
   int group;  // -1: none
-  int first, M, g, P, lead, r0;
+  int first, M, g, P, lead, own, r0;
   int lo, hi;  // tiles
   int place;   // of its partial, -1: o is written
 };
@@ -77,7 +80,7 @@ __device__ __forceinline__ int prefix_search(const int64_t* x, int n, int64_t v)
 // run goes on with, -1: not known.
 __device__ __forceinline__ PrefixItem prefix_find(const PrefixParams& p, const TreePlan& pl, int run,
                                                   int64_t& at, int next) {
-  PrefixItem it = {-1, 0, 0, 0, 0, 0, 0, 0, 0, -1};
+  PrefixItem it = {-1, 0, 0, 0, 0, 0, 0, 0, 0, 0, -1};
   const int n_groups = __builtin_amdgcn_readfirstlane((int)p.t.plan[2]);
   int gi;
   if (pl.kt > 0) {
@@ -106,40 +109,11 @@ __device__ __forceinline__ PrefixItem prefix_find(const PrefixParams& p, const T
   it.g = __builtin_amdgcn_readfirstlane(g.g);
   it.P = __builtin_amdgcn_readfirstlane(g.P);
   it.lead = __builtin_amdgcn_readfirstlane(g.lead);
+  it.own = __builtin_amdgcn_readfirstlane(g.own);
   it.r0 = __builtin_amdgcn_readfirstlane(g.r0);
   return it;
 }
 
-// Keys that stand in a row: positions base + 32 lo .. (below len) of block-table row r
-struct PrefixKeys {
-  int r, base, len;
-  int draft0;  // position of the request's first drafted token
-  int lo, hi;  // tiles
-  int own;     // 1: seen by the rows of tokens tok .. tok_end - 1 alone
-  int tok, tok_end;
-  int next;  // tile of the row group that comes after them
-};
-// Those of the piece from its tile t on; none: lo = hi
-__device__ __forceinline__ PrefixKeys prefix_keys(const PrefixParams& p, const PrefixItem& it, int t) {
-  const int shared = prefix_tiles(it.P);
-  if (t < shared)
-    return {it.lead, 0, it.P, INT32_MAX, t, min(shared, it.hi), 0, 0, 0, min(shared, it.hi)};
-  // the request in whose own tiles t lies
-  int64_t from = t - shared;
-  for (int r = it.r0; r < p.t.R; r += 64) {
-    const PrefixReq q = p.reqs[min(r + (tree_tid() & 63), p.t.R - 1)];
-    if (r == it.r0) from += shfl64(q.upto - q.tiles, 0);
-    const uint64_t hit = __ballot(q.upto > from);
-    if (!hit) continue;
-    const int k = __builtin_ctzll(hit);
-    auto get = [&](int x) { return __builtin_amdgcn_readlane(x, k); };
-    const int tiles = get(q.tiles), lo = (int)(from - (shfl64(q.upto, k) - tiles));
-    const int hi = (int)min((int64_t)tiles, (int64_t)lo + it.hi - t);
-    return {min(r + k, p.t.R - 1), it.P, get(q.len), get(q.draft0), lo, hi, 1, get(q.tok),
-            get(q.tok_end), t + hi - lo};
-  }
-  return {0, 0, 0, 0, 0, 0, 0, 0, 0, it.hi};
-}
 // x of LDS, the same in every lane, in scalar registers
 template <typename T>
 __device__ __forceinline__ T prefix_uniform(const T& x) {
@@ -150,6 +124,105 @@ __device__ __forceinline__ T prefix_uniform(const T& x) {
     reinterpret_cast<int*>(&r)[i] =
         __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(&x)[i]);
   return r;
+}
+
+// ---- own keys ----
+// Of the row group's own keys, numbered from 0, those of a request: from .. end - 1, its
+// first drafted token the one `draft` (all within a request's own keys, or past their end).
+struct PrefixOwn {
+  int from, end, draft, r;
+};
+// Token of the row group's last row, from that of its first one
+__device__ __forceinline__ int prefix_last_token(const PrefixItem& it, int H) {
+  const int m0 = it.g * kTreeRows, m1 = min(m0 + kTreeRows, it.M) - 1;
+  return (int)((uint32_t)m1 / (uint32_t)H) - (int)((uint32_t)m0 / (uint32_t)H);
+}
+// By the whole workgroup: the own keys of the row group's tokens, and of its rows
+__device__ __forceinline__ void prefix_own(const PrefixParams& p, const PrefixItem& it, PrefixOwn* tok,
+                                           PrefixOwn* row) {
+  const int H = p.t.H, i = tree_tid(), m0 = it.g * kTreeRows;
+  const int skip = (int)((uint32_t)m0 / (uint32_t)H);
+  if (i <= prefix_last_token(it, H)) {
+    const int t = it.first + skip + i;
+    const int r = min(max(p.request == nullptr ? t : p.request[t], 0), p.t.R - 1);
+    const PrefixReq a = p.reqs[it.r0], q = p.reqs[r];
+    const int from = (int)(q.upto - q.own - (a.upto - a.own));
+    tok[i] = {from, from + q.real, from + q.draft0 - it.P, r};
+  }
+  __syncthreads();
+  if (i < kTreeRows) {
+    const int m = min(m0 + i, it.M - 1);
+    row[i] = tok[(int)((uint32_t)m / (uint32_t)H) - skip];
+  }
+  __syncthreads();
+}
+// A segment of own keys from own0 on: its tiles and keys, and the first one that may be
+// hidden from some row (its first drafted token, if it is one request's).  Many keys of a request
+// make a segment of their own: 4 us to begin it, against the power of waves that see none of
+// it and the mask of every tile (32 requests of 64 heads, 32768 shared fp8 keys and 500 own
+// ones: 203 us with all own keys in one segment, 191 so).
+struct PrefixSpan {
+  int tiles, keys, draft;
+};
+constexpr int kPrefixAlone = 8;  // tiles
+__device__ __forceinline__ PrefixSpan prefix_span(const PrefixItem& it, int H, const PrefixOwn* tok,
+                                                  int own0) {
+  const int n = prefix_last_token(it, H) + 1, lane = tree_tid() & 63;
+  PrefixSpan s = {INT32_MAX / kTreeTile, it.own - own0, 0};
+  // the first token whose request's keys end past own0, and the first long one behind it
+  for (int i = 0; i < n; i += 64) {
+    const PrefixOwn o = tok[min(i + lane, n - 1)];
+    const int from = max(o.from, own0), tiles = (o.end - from + kTreeTile - 1) / kTreeTile;
+    const bool alone = from % kTreeTile == 0 && H % 32 == 0;
+    const uint64_t hit = __ballot(o.end > own0 && ((tiles >= kPrefixAlone && alone) || n == 1 || tok[0].r == tok[n - 1].r));
+    if (!hit) continue;
+    const int k = __builtin_ctzll(hit);
+    auto get = [&](int x) { return __builtin_amdgcn_readlane(x, k); };
+    if (get(from) > own0) {  // up to it
+      s.keys = get(from) - own0;
+      s.tiles = s.keys / kTreeTile;
+    } else {
+      s = {get(tiles), get(o.end) - own0, get(o.draft) - own0};
+    }
+    break;
+  }
+  return s;
+}
+// The cache rows of own keys own0 .. + keys - 1; whether this thread found one missing
+__device__ __forceinline__ bool prefix_rows(const TreeParams& p, const PrefixItem& it,
+                                            const PrefixOwn* tok, int own0, int keys, int32_t* rows) {
+  const int n = prefix_last_token(it, p.H) + 1;
+  bool gap = false;
+  for (int k = tree_tid(); k < keys; k += 256) {
+    const int key = own0 + k;
+    int lo = 0, hi = n;  // the last token whose request's keys begin at or before it
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (tok[mid].from <= key) lo = mid;
+      else hi = mid;
+    }
+    const PrefixOwn o = tok[lo];
+    const int pos = it.P + key - o.from;
+    const int pg = (int)((uint64_t)(uint32_t)pos * p.page_mul >> p.page_shift);
+    int64_t row = -1;
+    if (key >= o.from && key < o.end && pg < p.max_blocks) {
+      const int b = p.bt[(int64_t)o.r * p.max_blocks + pg];
+      if (b >= 0) row = (int64_t)b * p.page_size + (pos - pg * p.page_size);
+    }
+    if (row >= p.n_kv_rows) row = -1;
+    rows[k] = (int)row;
+    gap |= row < 0;
+  }
+  return gap;
+}
+// Which of the 32 keys from key0 on a row sees, its drafted tokens by their mask
+__device__ __forceinline__ uint32_t prefix_visible(const PrefixOwn& o, uint64_t see, int key0) {
+  auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; };
+  const int shift = o.draft - key0;
+  uint32_t keys = below(o.end - key0) & ~below(o.from - key0);
+  if (shift < 32)
+    keys &= shift >= 0 ? (uint32_t)(see << shift) | below(shift) : shift > -64 ? (uint32_t)(see >> -shift) : 0u;
+  return keys;
 }
 
 // Partials of a row group, for the merge: the first at k0, the others from k1 on, step apart

@@ -54,11 +54,11 @@ struct TreeSmem {
 };
 template <bool FP8>
 struct PrefixSmem : TreeSmem<FP8> {
-  uint32_t in[kTreeRows];  // ~0: the row is one of the segment's request, or none at all
-  // of each wave: next row group of its run, the item, the keys that it is at
-  int32_t group[kTreeWaves];
+  PrefixOwn tok[kTreeRows];  // own keys of the item's tokens, and of its rows
+  PrefixOwn row[kTreeRows];
+  // of each wave: next row group of its run, the item, its next tile, the segment's first own key
+  int32_t group[kTreeWaves], next[kTreeWaves], own0[kTreeWaves];
   PrefixItem it[kTreeWaves];
-  PrefixKeys ks[kTreeWaves];
 };
 static_assert(sizeof(PrefixSmem<false>) <= 160 * 1024 && sizeof(PrefixSmem<true>) <= 160 * 1024,
               "one workgroup per CU");
@@ -307,6 +307,36 @@ __device__ __forceinline__ uint32_t tree_clean(uint32_t* flags, uint8_t* slot, i
   return __builtin_amdgcn_readfirstlane(flags[0] | flags[1] << 8 | flags[2] << 16 | flags[3] << 24);
 }
 
+// Those of the keys of a tile that hold an infinity or NaN
+__device__ __forceinline__ uint32_t tree_bad(const uint8_t* slot, uint32_t keys) {
+  const int lane = tree_tid() & 63;
+  uint32_t found = 0;
+  while (keys) {
+    const int k = __builtin_ctz(keys);
+    keys &= keys - 1;
+    bool bad = false;
+    for (int i = lane; i < 4 * kTreeBlocks; i += 64) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(slot + 2048 * (i >> 2) + 64 * k + 16 * (i & 3));
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        bad |= (x[j] & 0x7c00u) == 0x7c00u || (x[j] & 0x7c000000u) == 0x7c000000u;
+    }
+    if (__any(bad)) found |= 1u << k;
+  }
+  return found;
+}
+// Zeros in place of such keys: nothing but NaN comes of them in the rows that see them.
+__device__ __forceinline__ void tree_zero(uint8_t* slot, uint32_t keys) {
+  const int lane = tree_tid() & 63;
+  while (keys) {
+    const int k = __builtin_ctz(keys);
+    keys &= keys - 1;
+    for (int i = lane; i < 4 * kTreeBlocks; i += 64)
+      *reinterpret_cast<u32x4*>(slot + 2048 * (i >> 2) + 64 * k + 16 * (i & 3)) = (u32x4){0u, 0u, 0u, 0u};
+  }
+  asm volatile("" ::: "memory");
+}
+
 // PE_BF16: the rope values of the (fp8) rows are bf16.  SHARED: the groups' keys are those
 // of mla_prefix_plan.h (the kernel's parameters are PrefixParams).
 template <bool FP8, bool PE_BF16, bool SHARED>
@@ -376,6 +406,7 @@ __device__ __forceinline__ void tree_attention(const TreeParams& p) {
       sh.at[mine] = at;
       sh.group[mine] = it.group + 1;
       sh.it[mine] = it;
+      sh.next[mine] = it.lo;
       sh.item[mine] = (u32x4){(uint32_t)it.first, (uint32_t)M, (uint32_t)it.g, (uint32_t)it.place};
     } else {
       it = tree_find(p, plan, at, false);
@@ -414,65 +445,85 @@ __device__ __forceinline__ void tree_attention(const TreeParams& p) {
     unroll<256>([&](auto i) { hw_zero<i>(); });
     float m_run = -1e30f, l_part = 0.f;  // m: of the raw scores; l: this lane's keys only
 
-    auto page_of = [&](int pos) { return (int)((uint64_t)(uint32_t)pos * p.page_mul >> p.page_shift); };
-    bool first_seg = true;
-    // Segments: of the one request's keys; SHARED: of the shared ones, then of those of
-    // each request in turn, what is left of them in LDS between the segments
+    // The keys in segments whose pages are resolved together.  SHARED: the shared keys are
+    // those of a request; the own ones stand one after the other in tiles, each key's row
+    // resolved (a page size of one).
     int seg = piece.lo;
-    if constexpr (SHARED)
-      sh.ks[wave()] = prefix_keys(tree_kernarg<PrefixParams>(), it, piece.lo);
     while (true) {
-      PrefixKeys ks;
+      bool first = false;  // segment of the piece
+      int bt_row, k_hi, t_hi, seg_lo;
+      int draft0;  // SHARED: tiles that reach past it are masked; else drafted token 0's position
+      int own0 = -1;  // SHARED: the segment's first own key
       if constexpr (SHARED) {
         const int mine = wave();
-        ks = prefix_uniform(sh.ks[mine]);
-        if (ks.lo >= ks.hi) {
-          const PrefixItem it = prefix_uniform(sh.it[mine]);
-          if (ks.next >= it.hi) break;
-          ks = prefix_keys(tree_kernarg<PrefixParams>(), it, ks.next);
-          if (ks.lo >= ks.hi) break;
+        const PrefixItem it = prefix_uniform(sh.it[mine]);
+        const int shared = prefix_tiles(it.P);
+        seg = __builtin_amdgcn_readfirstlane(sh.next[mine]);
+        first = seg == it.lo;
+        if (seg >= it.hi || (it.own == 0 && seg >= shared)) break;
+        seg_lo = seg * kTreeTile;
+        draft0 = INT32_MAX;
+        bt_row = it.lead;
+        k_hi = it.P;
+        t_hi = min(shared, it.hi);
+        if (seg >= shared) {
+          __syncthreads();  // tok and row are free
+          own0 = (seg - shared) * kTreeTile;
+          if (own0 == 0 || first) prefix_own(tree_kernarg<PrefixParams>(), it, sh.tok, sh.row);
+          const PrefixSpan span = prefix_span(it, tree_params().H, sh.tok, own0);
+          draft0 = span.draft;
+          seg_lo = 0;
+          t_hi = min(min(it.hi - seg, span.tiles), kTreePages / kTreeTile);
+          k_hi = span.keys;
         }
-        seg = ks.lo;
       } else {
-        ks = {it.r, 0, it.len, max(0, p.seq_lens[it.r]) - it.n, 0, piece.hi, 0, 0, 0, 0};
-        if (seg >= ks.hi || seg * kTreeTile >= min(ks.hi * kTreeTile, ks.len)) break;
+        bt_row = it.r;
+        draft0 = max(0, p.seq_lens[it.r]) - it.n;
+        t_hi = piece.hi;
+        k_hi = min(t_hi * kTreeTile, it.len);
+        seg_lo = seg * kTreeTile;
+        if (seg >= t_hi || seg_lo >= k_hi) break;
+        first = seg == piece.lo;
       }
-      const int bt_row = ks.r, draft0 = ks.draft0;  // position of drafted token 0
-      const int t_hi = ks.hi;
-      const int k_hi = SHARED ? ks.len : min(t_hi * kTreeTile, ks.len);
+      const bool packed = SHARED && own0 >= 0;
+      const uint32_t page_mul = packed ? 1u << 31 : p.page_mul, page_shift = packed ? 31 : p.page_shift;
+      const int page_size = packed ? 1 : p.page_size;
+      auto page_of = [&](int pos) { return (int)((uint64_t)(uint32_t)pos * page_mul >> page_shift); };
       // tiles of this segment: as many as its pages cover
-      const int seg_lo = SHARED ? ks.base + seg * kTreeTile : seg * kTreeTile;
       const int pg0 = page_of(seg_lo);
-      const int64_t room = (int64_t)(pg0 + kTreePages) * p.page_size - (int64_t)seg_lo;
+      const int64_t room = (int64_t)(pg0 + kTreePages) * page_size - (int64_t)seg_lo;
       const int ntiles =
-          SHARED ? (int)min((int64_t)(t_hi - seg), room / kTreeTile)
-                 : (int)min((int64_t)(min(t_hi * kTreeTile, k_hi + kTreeTile - 1) / kTreeTile - seg),
-                            room / kTreeTile);
+          (int)min((int64_t)(min(t_hi * kTreeTile, k_hi + kTreeTile - 1) / kTreeTile - seg_lo / kTreeTile),
+                   room / kTreeTile);
       seg += ntiles;
+      if constexpr (SHARED) {
+        sh.next[wave()] = seg;
+        sh.own0[wave()] = own0;
+      }
       const int keys = min(ntiles * kTreeTile, k_hi - seg_lo);  // of the segment
       __syncthreads();  // blk and the ring are free
       if (tree_tid() == 0) sh.gap = 0;
-      if constexpr (SHARED) {
-        ks.lo = seg;
-        sh.ks[wave()] = ks;
-        const u32x4 item = sh.item[wave()];
-        if (tree_tid() < kTreeRows) {
-          const uint32_t m = item[2] * kTreeRows + tree_tid();
-          const int tok = (int)(item[0] + m / (uint32_t)p.H);
-          sh.in[tree_tid()] =
-              !ks.own || m >= item[1] || (tok >= ks.tok && tok < ks.tok_end) ? ~0u : 0u;
-        }
-      }
       __syncthreads();
       {
-        const int n = page_of(seg_lo + keys - 1) - pg0 + 1;
-        const int64_t blocks = (p.n_kv_rows + p.page_size - 1) / p.page_size;
-        bool gap = p.n_kv_rows % p.page_size != 0;
-        for (int j = tree_tid(); j < n; j += kTreeThreads) {
-          const int b = p.bt[(int64_t)bt_row * p.max_blocks + pg0 + j];
-          const bool ok = b >= 0 && b < blocks;
-          gap |= !ok;
-          sh.blk[j] = ok ? b : -1;
+        bool gap = false;
+        auto pages = [&]() {
+          const TreeParams now = SHARED ? tree_params() : p;
+          const int n = page_of(seg_lo + keys - 1) - pg0 + 1;
+          const int64_t blocks = (now.n_kv_rows + now.page_size - 1) / now.page_size;
+          gap = now.n_kv_rows % now.page_size != 0;
+          for (int j = tree_tid(); j < n; j += kTreeThreads) {
+            const int b = now.bt[(int64_t)bt_row * now.max_blocks + pg0 + j];
+            const bool ok = b >= 0 && b < blocks;
+            gap |= !ok;
+            sh.blk[j] = ok ? b : -1;
+          }
+        };
+        if constexpr (SHARED) {
+          if (packed)
+            gap = prefix_rows(tree_params(), prefix_uniform(sh.it[wave()]), sh.tok, own0, keys, sh.blk);
+          else pages();
+        } else {
+          pages();
         }
         if (__any(gap) && (tree_tid() & 63) == 0) sh.gap = 1;
       }
@@ -484,7 +535,7 @@ __device__ __forceinline__ void tree_attention(const TreeParams& p) {
         const int pos = seg_lo + key;
         const int pg = page_of(pos);
         const int b = sh.blk[pg - pg0];
-        const uint32_t row = (uint32_t)b * (uint32_t)p.page_size + (uint32_t)(pos - pg * p.page_size);
+        const uint32_t row = (uint32_t)b * (uint32_t)page_size + (uint32_t)(pos - pg * page_size);
         return b >= 0 && row < (uint32_t)p.n_kv_rows ? (int)row : -1;
       };
       // the row of the key that this lane fetches of a tile, and its bytes
@@ -496,11 +547,11 @@ __device__ __forceinline__ void tree_attention(const TreeParams& p) {
       auto row_begin = [&](int tile) {
         const int key = tile * kTreeTile + 16 * (w & 1) + ((tree_tid() & 63) >> 2);
         const int pos = seg_lo + min(key, keys - 1), pg = page_of(pos);
-        row_off = key < keys ? pos - pg * p.page_size : -1;
+        row_off = key < keys ? pos - pg * page_size : -1;
         row_blk = sh.blk[pg - pg0];
       };
       auto row_end = [&]() {
-        const uint32_t row = (uint32_t)row_blk * (uint32_t)p.page_size + (uint32_t)row_off;
+        const uint32_t row = (uint32_t)row_blk * (uint32_t)page_size + (uint32_t)row_off;
         return (row_blk | row_off) >= 0 && row < (uint32_t)p.n_kv_rows ? (int)row : -1;
       };
       auto bytes_of = [&](int row) {
@@ -516,27 +567,19 @@ __device__ __forceinline__ void tree_attention(const TreeParams& p) {
       // maximum beside the product of P and V of tile i.  Every chain of dependent
       // instructions is spread over the steps (a wave alone on its SIMD waits for
       // each), and the first operands of a product are read in the one before it.
-      // SHARED: keys of a request in a wave with rows of others too are treated as drafted
-      // ones that some rows do not see; waves without a row of it are idle
-      bool mixed = false, busy = active;
+      auto is_draft = [&](int tile) { return seg_lo + tile * kTreeTile + kTreeTile > draft0; };
+      // SHARED: waves without a row that sees the segment are idle, half of them with 64 heads
+      bool busy = active;
       if constexpr (SHARED) {
-        const int l = tree_tid() & 63, mine = wave();
-        const uint64_t a = __ballot(sh.in[l] != 0), b = __ballot(sh.in[64 + l] != 0);
-        const uint32_t rows[4] = {(uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32)};
-#pragma unroll
-        for (int i = 0; i < kTreeWaves; i++) {
-          mixed |= rows[i] != 0 && rows[i] != ~0u;
-          busy &= i != mine || rows[i] != 0;
+        if (packed) {
+          const PrefixOwn o = sh.row[32 * wave() + (tree_tid() & 31)];
+          busy = active && __any(o.from < own0 + keys && o.end > own0);
         }
       }
-      auto is_draft = [&](int tile) {
-        return (SHARED && mixed) || seg_lo + tile * kTreeTile + kTreeTile > draft0;
-      };
-      auto clean_from = [&](int tile) {
-        return SHARED && mixed ? 0 : draft0 - seg_lo - tile * kTreeTile;
-      };
       // slots of the tiles i .. i + 3 (fp8: i + 2), bytes
       int s0 = 0, s1 = kTreeSlotBytes, s2 = 2 * kTreeSlotBytes, s3 = FP8 ? 0 : 3 * kTreeSlotBytes;
+      // keys of a masked tile that are not finite.  Of tile i: their scores become NaN;
+      // SHARED: of the next one: their values are cleared before its product with P
       uint32_t dirty = 0;
       if constexpr (FP8) {
         // tiles 0 and 1 converted, 2 and 3 on their way
@@ -565,7 +608,8 @@ __device__ __forceinline__ void tree_attention(const TreeParams& p) {
         asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
       }
       lds_barrier();  // tiles 0 and 1 are in
-      if (is_draft(0)) dirty = tree_clean(sh.dirty, sh.ring[0], wave(), clean_from(0));
+      if constexpr (!SHARED)
+        if (is_draft(0)) dirty = tree_clean(sh.dirty, sh.ring[0], wave(), draft0 - seg_lo);
 
       constexpr int A = tree_ahead(FP8);
       f32x16 s;             // scores of tile i, then their exponentials
@@ -574,21 +618,47 @@ __device__ __forceinline__ void tree_attention(const TreeParams& p) {
       int up = 0;           // O has to be scaled
       TreeFrag<A> kf, vf;
       TreeAddr kb;
-      auto mask = [&](f32x16& s, int tile) {
+      auto mask = [&](f32x16& s, int tile, const uint8_t* slot) {
         const bool draft = is_draft(tile);
+        if constexpr (SHARED) dirty = 0;
         if (!gaps && !draft && (tile + 1) * kTreeTile <= keys) return;
         hw_settle();
         asm volatile("" : "+v"(s));  // no use of S above the wait
         const int l = tree_tid(), h4 = (l >> 3) & 4;  // 4 hf
         // keys with a row; 32 lanes look at one each
         uint32_t vis = (uint32_t)__ballot(row_at(tile * kTreeTile + (l & 31)) >= 0);
-        if (draft) vis &= tree_visible(sh.see[32 * wave() + (l & 31)], draft0 - seg_lo - tile * kTreeTile);
-        if constexpr (SHARED)
-          if (draft) vis &= sh.in[32 * wave() + (l & 31)];
+        if constexpr (SHARED) {
+          if (draft) {
+            const int at = 32 * wave() + (l & 31);
+            vis &= prefix_visible(sh.row[at], sh.see[at], sh.own0[wave()] + tile * kTreeTile);
+          }
+        } else {
+          if (draft) vis &= tree_visible(sh.see[32 * wave() + (l & 31)], draft0 - seg_lo - tile * kTreeTile);
+        }
         vis >>= h4;
+        if constexpr (SHARED) {
+          // 0 times a score is NaN where the score is not finite
+          float bad = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; e++) bad = __builtin_fmaf(s[e], 0.f, bad);
+          if (draft && __any(bad != bad)) {
+            // a key that is not finite gives such a score to every row
+            uint32_t every = 0;
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+              const uint64_t lanes = __ballot(!(__builtin_fabsf(s[e]) < INFINITY));
+              every |= ((uint32_t)lanes == ~0u ? 1u : 0u) << (8 * (e >> 2) + (e & 3));
+              every |= ((uint32_t)(lanes >> 32) == ~0u ? 1u : 0u) << (8 * (e >> 2) + 4 + (e & 3));
+            }
+            dirty = every ? tree_bad(slot, every) : 0;
+            const uint32_t nan = dirty >> h4;
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[e] = tree_pick(nan, e, NAN, s[e]);
+          }
+        }
 #pragma unroll
         for (int e = 0; e < 16; e++) s[e] = tree_pick(vis, e, s[e], -INFINITY);
-        if (dirty) {
+        if (!SHARED && dirty) {
           const uint32_t nan = vis & (dirty >> h4);
 #pragma unroll
           for (int e = 0; e < 16; e++) s[e] = tree_pick(nan, e, NAN, s[e]);
@@ -610,14 +680,14 @@ __device__ __forceinline__ void tree_attention(const TreeParams& p) {
         kb = tree_addr(lds0 + ka0, 0);
         tree_kfirst(kf, kb);
         tree_qk(s, qf, kf, kb, [](auto) {});
-        mask(s, 0);
+        mask(s, 0, sh.ring[0]);
         hw_settle();
         asm volatile("" : "+v"(s));
         mt = fmaxf(s[0], s[1]);
 #pragma unroll
         for (int e = 2; e < 16; e++) mt = fmaxf(mt, s[e]);
         mt = xor32_max(mt);
-        follow(SHARED ? first_seg : seg_lo == piece.lo * kTreeTile);
+        follow(SHARED ? first : seg_lo == piece.lo * kTreeTile);
         kb = tree_addr(lds0 + s1 + ka0, 0);
         tree_kfirst(kf, kb);
       }
@@ -629,8 +699,13 @@ __device__ __forceinline__ void tree_attention(const TreeParams& p) {
         const bool more = i + 1 < ntiles;
         // tile i + 1 is in, and every wave is done with tile i - 1, in whose place
         // tile i + 3 goes
-        if (more && is_draft(i + 1))
-          dirty = tree_clean(sh.dirty, sh.ring[0] + s1, wave(), clean_from(i + 1));
+        if constexpr (SHARED) {
+          // every wave has its scores of tile i, and reads its values only after this
+          if (dirty && busy) tree_zero(sh.ring[0] + s0, dirty);
+        } else {
+          if (more && is_draft(i + 1))
+            dirty = tree_clean(sh.dirty, sh.ring[0] + s1, wave(), draft0 - seg_lo - (i + 1) * kTreeTile);
+        }
         uint8_t* const raw = sh.raw[FP8 ? i & 1 : 0][FP8 ? w : 0];
         // fp8: the wave's share of tile i + 2 has landed
         if constexpr (FP8) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
@@ -705,7 +780,7 @@ __device__ __forceinline__ void tree_attention(const TreeParams& p) {
           };
           if (more) tree_qk(sn, qf, kf, kb, side);
           else unroll<36>(side);
-          if (more) mask(sn, i + 1);
+          if (more) mask(sn, i + 1, sh.ring[0] + s1);
           float m2 = -INFINITY;
           constexpr int kLast = 31 - A;  // the last V operand is read here
           tree_pv(pb, vf, vb, [&](auto uc) {
@@ -762,7 +837,6 @@ __device__ __forceinline__ void tree_attention(const TreeParams& p) {
         s3 = was;
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the DMA past the end too
-      first_seg = false;
     }
 
     // ---- o and lse, or the piece's partial ----

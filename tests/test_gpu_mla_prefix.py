@@ -229,6 +229,17 @@ def test_nan_query_stays_in_its_row(pkg, lib, dev):
     check((o, lse), want)
 
 
+@pytest.mark.parametrize("H", [4, 32, 64])
+def test_nan_queries_of_a_request(pkg, lib, dev, H):
+    """All rows of a wave, or some: their scores of every key are NaN, the keys are not."""
+    c = make([(64, [(9, 1), (70, 1), (3, 2)])], H, 16, "fp16", seed=20)
+    want = oracle(c)
+    c["q"][1] = math.nan
+    got = call(pkg, c, dev)
+    assert bool(torch.isnan(got[0][1]).all()) and bool(torch.isnan(got[1][1]).all())
+    check(got, want, torch.tensor([True, False, True, True]))
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.07, 1.5])
 def test_scales(pkg, lib, dev, scale):
     c = make([(48, [(9, 1), (70, 1), (3, 1)])], 16, 16, "fp16", seed=11, spread=0.3)
