@@ -173,14 +173,15 @@ __device__ __forceinline__ PrefixSpan prefix_span(const PrefixItem& it, int H, c
   for (int i = 0; i < n; i += 64) {
     const PrefixOwn o = tok[min(i + lane, n - 1)];
     const int from = max(o.from, own0), tiles = (o.end - from + kTreeTile - 1) / kTreeTile;
-    const bool alone = from % kTreeTile == 0 && H % 32 == 0;
-    const uint64_t hit = __ballot(o.end > own0 && ((tiles >= kPrefixAlone && alone) || n == 1 || tok[0].r == tok[n - 1].r));
+    const bool one = tok[0].r == tok[n - 1].r;
+    const bool alone = tiles >= kPrefixAlone && from % kTreeTile == 0 && H % 32 == 0;
+    const uint64_t hit = __ballot(o.end > own0 && (one || alone));
     if (!hit) continue;
     const int k = __builtin_ctzll(hit);
     auto get = [&](int x) { return __builtin_amdgcn_readlane(x, k); };
     if (get(from) > own0) {  // up to it
       s.keys = get(from) - own0;
-      s.tiles = s.keys / kTreeTile;
+      s.tiles = max(1, s.keys / kTreeTile);
     } else {
       s = {get(tiles), get(o.end) - own0, get(o.draft) - own0};
     }

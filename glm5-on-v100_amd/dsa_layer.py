@@ -45,7 +45,8 @@ decode would give: rotary positions of q and k_pe with the latent rows written i
 the same launch (rope_concat_and_cache_mla), the indexer's key rotated and stored,
 step 3, the attention, step 5.  Where the block table holds at most topk positions
 the selection keeps every key and the attention is tree attention, one matrix
-product of all heads of a draft and their request's context; in longer tables it is
+product of all heads of a draft and their request's context (told of requests that share
+their first positions, of all their drafts and those); in longer tables it is
 steps 2 and 4, each drafted token with its own selection out of what it sees.
 
 All buffers come from torch's caching allocator; nothing here synchronises
@@ -58,7 +59,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import _cache_ops, _lib, _sm70_ops, mla_tree, paging, rope
+from . import _cache_ops, _lib, _sm70_ops, mla_prefix, mla_tree, paging, rope
 from .ops import _check, _no_grad, _rows16, _stream
 
 KT = 64  # key tile the prefill logits launch is rounded to (sparse_attn_indexer.py:753)
@@ -392,7 +393,9 @@ class DsaLayer:
                     cu_seqlens_q: torch.Tensor, tree_mask: torch.Tensor,
                     idx_k: torch.Tensor | None = None, interleaved: bool = True,
                     idx_q: torch.Tensor | None = None,
-                    idx_w: torch.Tensor | None = None) -> torch.Tensor:
+                    idx_w: torch.Tensor | None = None,
+                    cu_shared: torch.Tensor | None = None,
+                    shared_lens: torch.Tensor | None = None) -> torch.Tensor:
         """Every request's tree of drafted tokens in one step.  q [T, H, P + 64] fp16,
         kv_c [T, 512] and k_pe [T, 64], not rotated; positions [T] are the tokens'
         places in the text (context length + depth in the tree, mla_tree.tree_masks),
@@ -405,8 +408,11 @@ class DsaLayer:
         of more than topk positions needs idx_q [T, 32, 128], rotated as idx_k is, and
         idx_w [T, 32]: every token attends to the topk of its visible positions that the
         indexer chooses, as in decode (last_idx), with the indexer's keys in the cache or
-        given as idx_k.  q, k_pe, idx_k and idx_q stay as they are.  Returns out
-        [T, H * V], zero for tokens of no request."""
+        given as idx_k.  cu_shared and shared_lens (mla_prefix.shared_prefix_attention; the
+        groups cover the requests) tell which requests hold their first positions in the
+        same rows: where every key is attended to, those are read once for all of them.  q,
+        k_pe, idx_k and idx_q stay as they are.  Returns out [T, H * V], zero for tokens of
+        no request (of no group)."""
         T = slot_mapping.numel()
         _check(q.dim() == 3 and q.shape == (T, self.w.n_heads, self.w.nope_dim + 64),
                "q must be [T, H, P + 64], a slot for each token")
@@ -415,6 +421,9 @@ class DsaLayer:
         # the rest of what later launches would refuse: none may follow a written cache
         _no_grad(q, kv_c, k_pe, idx_k, idx_q, idx_w)
         mla_tree._check_trees(T, block_table, seq_lens, cu_seqlens_q, tree_mask, q.device)
+        _check((cu_shared is None) == (shared_lens is None), "cu_shared and shared_lens go together")
+        if cu_shared is not None:
+            mla_prefix._check_shared(cu_shared, shared_lens, q.device)
         P, R = self.w.nope_dim, block_table.shape[0]
         choose = R > 0 and block_table.shape[1] * self.latent_cache.shape[-2] > self.topk
         if idx_k is not None:
@@ -461,8 +470,13 @@ class DsaLayer:
         H = self.w.n_heads
         o = torch.zeros(T, H, 512, dtype=torch.float16, device=q.device)
         lse = torch.full((T, H), float("-inf"), dtype=torch.float32, device=q.device)
-        mla_tree.tree_attention(ql, self.latent_cache, block_table, seq_lens, cu_seqlens_q,
-                                tree_mask, self.w.scale, o, lse)
+        if cu_shared is None:
+            mla_tree.tree_attention(ql, self.latent_cache, block_table, seq_lens, cu_seqlens_q,
+                                    tree_mask, self.w.scale, o, lse)
+        else:
+            mla_prefix.shared_prefix_attention(ql, self.latent_cache, block_table, seq_lens,
+                                               cu_shared, shared_lens, self.w.scale,
+                                               cu_seqlens_q, tree_mask, o, lse)
         self.last_idx, self.last_o, self.last_lse = None, o, lse
         return v_up(o, self.w)
 
