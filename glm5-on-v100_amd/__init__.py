@@ -11,8 +11,8 @@ tests/conftest.py).
 from . import (_lib, ops, _sm70_ops, _cache_ops, dsa_layer, mla_prefill, mla_prefix,  # noqa: F401
                mla_tree, paging, rope, synthetic, w4)
 
-__all__ = ["_lib", "ops", "_sm70_ops", "_cache_ops", "dsa_layer", "mla_prefill", "mla_prefix", "mla_tree",
-           "paging", "rope", "synthetic", "w4", "load_library"]
+__all__ = ["_lib", "ops", "_sm70_ops", "_cache_ops", "dsa_layer", "mla_prefill", "mla_prefix",
+           "mla_tree", "paging", "rope", "synthetic", "w4", "load_library"]
 
 
 def load_library():

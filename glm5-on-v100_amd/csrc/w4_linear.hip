@@ -216,8 +216,7 @@ __global__ void __launch_bounds__(64 * (XI == 1 ? 8 : 4)) w4_linear_kernel(W4Par
     // the block is in: what was sent after it may be on its way
     constexpr int kLater = XD > 1 ? (D - 1) * (R::kLoads + XI) : (D > 1 ? R::kLoads : 0);
     static_assert(kLater < 64, "vmcnt");
-    if (XD == 1 && D > 2 && it == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLater) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLater) : "memory");
     u32x4 x[MT][4], q[NT];
     uint32_t sz[NT][GPB];
     const uint32_t from = ring + slot * R::kQ, xfrom = xring + (XD > 1 ? slot * XI * 1024 : 0);
@@ -461,8 +460,7 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(W4Weights p, int symme
     for (int s = kSteps * e; s < kSteps * (e + 1); s++) {
       uint32_t code[8];
 #pragma unroll
-      for (int i = 0; i < 8; i++)
-      {
+      for (int i = 0; i < 8; i++) {
         const float y = v[s][i] * r;
         const float q = safe ? __builtin_fmaf(__builtin_fmaf(-y, sc, v[s][i]), r, y) : v[s][i] / sc;
         code[i] = (uint32_t)__builtin_amdgcn_fmed3f(__builtin_rintf(q) + z, 0.f, 15.f);

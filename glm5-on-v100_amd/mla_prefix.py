@@ -33,7 +33,7 @@ def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     token r at position seq_lens[r] - 1, which sees everything up to itself.  With
     cu_seqlens_q and tree_mask: each request's drafted tokens, as in
     mla_tree.tree_attention.  kv_cache, block_table, seq_lens, scale and pe_dtype are as there;
-    the block table holds less than 2^24 positions.
+    the block table holds less than 2^23 positions.
 
     Returns o [T, H, 512] fp16 and lse [T, H] fp32; a row that sees nothing has o = 0
     and lse = -inf.  Rows of no request, and of requests of no group, stay as they were in

@@ -2,8 +2,8 @@
 
 Schemas are the reference's, verbatim (patches/glm5-v100-sm70-glue.patch:
 494-565; persistent_topk from its call sites, reference/
-sparse_attn_indexer.py:632-639 and :873-880); rope.py, _cache_ops.py and
-mla_tree.py define those that the reference lacks.  Each op validates its tensors
+sparse_attn_indexer.py:632-639 and :873-880); rope.py, _cache_ops.py, mla_tree.py,
+mla_prefix.py, paging.py and w4.py define those that the reference lacks.  Each op validates its tensors
 the way the reference's TORCH_CHECKs do (same conditions, RuntimeError),
 then calls the C ABI on the current stream.  Only the CUDA (= HIP on ROCm)
 dispatch key has a kernel: CPU tensors raise, there is no silent fallback.
@@ -490,8 +490,8 @@ CACHE_OPS = ("concat_and_cache_mla",)
 
 
 def define(schema: str, impl) -> None:
-    """Adds an op without a counterpart in the reference (rope.py, _cache_ops.py and
-    mla_tree.py define theirs when the package is imported).  Their Python functions call
+    """Adds an op without a counterpart in the reference (rope.py, _cache_ops.py, mla_tree.py,
+    mla_prefix.py, paging.py and w4.py define theirs when the package is imported).  Their Python functions call
     the kernel directly (a dispatch costs half of a short call) and the op where they are
     traced."""
     name = schema.partition("(")[0]

@@ -173,10 +173,35 @@ def _shared_lengths(out, block_table, seq_lens, cu_shared, page_size):
             block_table.data_ptr(), seq_lens.data_ptr(), R, W, page_size, ws.data_ptr(), 4 * R)
 
 
+# The ops may be called with any tensors: what the functions above make.
+def _written(x, shape, dtype, dev, name: str) -> None:
+    _check(x.shape == shape and x.dtype == dtype and x.is_contiguous() and x.device == dev,
+           f"{name} must be contiguous {dtype} {list(shape)} on the GPU")
+
+
 def _op_extend(slots, pos, cu, granted, block_table, seq_lens, new_tokens, free_pages, free_count,
                page_size):
+    R, dev, T = seq_lens.numel(), block_table.device, slots.numel()
+    _written(slots, (T,), torch.int32, dev, "slot_mapping")
+    _written(pos, (T,), torch.int32, dev, "positions")
+    _written(cu, (R + 1,), torch.int32, dev, "cu_seqlens_q")
+    _written(granted, (R,), torch.bool, dev, "granted")
     _extend((slots, pos, cu, granted), block_table, seq_lens, new_tokens, free_pages, free_count,
-            page_size, slots.size(0))
+            page_size, T)
+
+
+def _op_token_tables(out, lens, block_table, seq_lens, cu_seqlens_q):
+    _check(out.dim() == 2 and block_table.dim() == 2 and out.size(1) <= block_table.size(1),
+           "out must be [tokens, cols] of a block table's first columns")
+    _written(out, tuple(out.shape), torch.int32, block_table.device, "out")
+    _written(lens, (out.size(0),), torch.int32, block_table.device, "lens")
+    _token_tables(out, lens, block_table, seq_lens, cu_seqlens_q)
+
+
+def _op_shared_lengths(out, block_table, seq_lens, cu_shared, page_size):
+    _check(cu_shared.dim() == 1 and cu_shared.size(0) >= 1, "cu_shared must be int32 [groups + 1]")
+    _written(out, (cu_shared.size(0) - 1,), torch.int32, block_table.device, "out")
+    _shared_lengths(out, block_table, seq_lens, cu_shared, page_size)
 
 
 ops.define("extend_tables(Tensor(a!) slot_mapping, Tensor(b!) positions, Tensor(c!) cu_seqlens_q, "
@@ -185,6 +210,6 @@ ops.define("extend_tables(Tensor(a!) slot_mapping, Tensor(b!) positions, Tensor(
 ops.define("truncate_tables(Tensor(a!) block_table, Tensor(b!) seq_lens, Tensor new_lens, "
            "Tensor(c!) free_pages, Tensor(d!) free_count, int page_size) -> ()", _truncate)
 ops.define("token_tables(Tensor(a!) out, Tensor(b!) lens, Tensor block_table, Tensor seq_lens, "
-           "Tensor cu_seqlens_q) -> ()", _token_tables)
+           "Tensor cu_seqlens_q) -> ()", _op_token_tables)
 ops.define("shared_lengths(Tensor(a!) out, Tensor block_table, Tensor seq_lens, Tensor cu_shared, "
-           "int page_size) -> ()", _shared_lengths)
+           "int page_size) -> ()", _op_shared_lengths)

@@ -31,14 +31,18 @@ class W4Weight:
     dtype: torch.dtype
 
     def __post_init__(self):
-        _check(self.dtype in _DTYPE_CODE, "w4: fp16 or bf16 weights")
-        _check(self.group in (32, 64, 128), "w4: group must be 32, 64 or 128")
-        _check(self.k % 8 == 0, "w4: K must be a multiple of 8")
-        t, b = -(-self.n // 16), -(-self.k // 128)
-        _check(self.q.shape == (t, b, 64, 4) and self.sz.shape == (t, b * (128 // self.group), 16)
-               and self.q.dtype == torch.int32 and self.sz.dtype == torch.int32
-               and self.q.is_contiguous() and self.sz.is_contiguous()
-               and self.sz.device == self.q.device, "w4: q and sz are not of weights [n, k]")
+        _check_weights(self.q, self.sz, self.n, self.k, self.group, self.dtype)
+
+
+def _check_weights(q, sz, n: int, k: int, group: int, dtype: torch.dtype) -> None:
+    _check(dtype in _DTYPE_CODE, "w4: fp16 or bf16 weights")
+    _check(group in (32, 64, 128), "w4: group must be 32, 64 or 128")
+    _check(k % 8 == 0, "w4: K must be a multiple of 8")
+    t, b = -(-n // 16), -(-k // 128)
+    _check(q.shape == (t, b, 64, 4) and sz.shape == (t, b * (128 // group), 16)
+           and q.dtype == torch.int32 and sz.dtype == torch.int32 and q.is_contiguous()
+           and sz.is_contiguous() and sz.device == q.device,
+           "w4: q and sz are not of weights [n, k]")
 
 
 def _empty(n: int, k: int, group: int, dtype: torch.dtype, dev) -> W4Weight:
@@ -53,7 +57,8 @@ def w4_quantize(weight: torch.Tensor, group: int = 128, symmetric: bool = False)
     """Quantises weight [N, K] (fp16 or bf16, K a multiple of 8) group by group: with lo and
     hi the least and largest value of a group and 0, scale = (hi - lo) / 15 and zero point
     RN(-lo / scale), or (symmetric) max(hi / 7, -lo / 8) and 8; codes are
-    clamp(RN(w / scale) + zero point, 0, 15).  Scales are of the weights' type."""
+    clamp(RN(w / scale) + zero point, 0, 15).  Scales are of the weights' type.  A group
+    that holds an infinity has no finite scale; NaN does not count and has some code."""
     _no_grad(weight)
     _check(weight.dim() == 2, "weight must be 2-D [N, K]")
     w = _empty(weight.size(0), weight.size(1), group, weight.dtype, weight.device)
@@ -75,15 +80,19 @@ def w4_pack(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
     """Weights quantised elsewhere: codes uint8 [N, K] (their low four bits), scales fp16
     or bf16 [N, ceil(K / group)], zeros uint8 of that shape, or None for 8."""
     _check(codes.dim() == 2 and codes.dtype == torch.uint8, "codes must be uint8 [N, K]")
-    n, k = codes.shape
-    w = _empty(n, k, group, scales.dtype, codes.device)
-    _check(scales.shape == (n, -(-k // group)), "scales must be [N, ceil(K / group)]")
-    _check(zeros is None or (zeros.shape == scales.shape and zeros.dtype == torch.uint8),
-           "zeros must be uint8 [N, ceil(K / group)]")
+    w = _empty(codes.size(0), codes.size(1), group, scales.dtype, codes.device)
+    _check_scales(codes, scales, zeros, group)
     _no_grad(scales)
     run = ops.op("w4_pack") if _traced(codes) else _pack
     run(w.q, w.sz, codes, scales, zeros, group)
     return w
+
+
+def _check_scales(codes, scales, zeros, group) -> None:
+    n, k = codes.shape
+    _check(scales.shape == (n, -(-k // group)), "scales must be [N, ceil(K / group)]")
+    _check(zeros is None or (zeros.shape == scales.shape and zeros.dtype == torch.uint8),
+           "zeros must be uint8 [N, ceil(K / group)]")
 
 
 def _pack(q, sz, codes, scales, zeros, group):
@@ -98,8 +107,9 @@ def _pack(q, sz, codes, scales, zeros, group):
 
 def w4_linear(x: torch.Tensor, w: W4Weight, out: torch.Tensor | None = None) -> torch.Tensor:
     """x [M, K] times the transposed weights: [M, N] in x's type (the weights'), M at most
-    64 rows.  Weights enter unrounded, sums are fp32.  Prefill-sized products: w4_dequant
-    and a matrix product."""
+    64 rows.  Weights enter unrounded, sums are fp32.  Of x in bf16, a value from 2^122 on or
+    an infinity may make NaN of its row of y where the product is infinite.  Prefill-sized
+    products: w4_dequant and a matrix product."""
     _no_grad(x)
     _check(x.dim() == 2 and x.size(1) == w.k, "x must be [M, K]")
     _check(x.dtype == w.dtype, "x must have the weights' type")
@@ -107,11 +117,15 @@ def w4_linear(x: torch.Tensor, w: W4Weight, out: torch.Tensor | None = None) -> 
     if out is None:
         out = torch.empty(x.size(0), w.n, dtype=x.dtype, device=x.device)
     else:
-        _check(out.shape == (x.size(0), w.n) and out.dtype == x.dtype and out.is_contiguous()
-               and out.device == x.device, "out must be contiguous [M, N] of x's type")
+        _check_out(out, x, w.n)
     run = ops.op("w4_linear") if _traced(x) else _linear
     run(out, x, w.q, w.sz, w.group)
     return out
+
+
+def _check_out(out, x, n: int) -> None:
+    _check(out.shape == (x.size(0), n) and out.dtype == x.dtype and out.is_contiguous()
+           and out.device == x.device, "out must be contiguous [M, N] of x's type")
 
 
 def _linear(y, x, q, sz, group):
@@ -143,9 +157,38 @@ def _dequant(out, q, sz, group):
             _DTYPE_CODE[out.dtype], out.size(0), out.size(1), group)
 
 
+# The ops may be called with any tensors: what the functions above have checked, or made.
+def _op_quantize(q, sz, weight, group, symmetric):
+    _check(weight.dim() == 2 and q.device == weight.device, "weight must be 2-D [N, K]")
+    _check_weights(q, sz, *weight.shape, group, weight.dtype)
+    _quantize(q, sz, weight, group, symmetric)
+
+
+def _op_pack(q, sz, codes, scales, zeros, group):
+    _check(codes.dim() == 2 and codes.dtype == torch.uint8 and q.device == codes.device,
+           "codes must be uint8 [N, K]")
+    _check_weights(q, sz, *codes.shape, group, scales.dtype)
+    _check_scales(codes, scales, zeros, group)
+    _pack(q, sz, codes, scales, zeros, group)
+
+
+def _op_linear(y, x, q, sz, group):
+    _check(x.dim() == 2 and y.dim() == 2, "x must be [M, K], y [M, N]")
+    _check_out(y, x, y.size(1))
+    _check_weights(q, sz, y.size(1), x.size(1), group, x.dtype)
+    _linear(y, x, q, sz, group)
+
+
+def _op_dequant(out, q, sz, group):
+    _check(out.dim() == 2 and out.is_contiguous() and out.device == q.device,
+           "out must be contiguous [N, K]")
+    _check_weights(q, sz, *out.shape, group, out.dtype)
+    _dequant(out, q, sz, group)
+
+
 ops.define("w4_quantize(Tensor(a!) q, Tensor(b!) sz, Tensor weight, int group, bool symmetric) -> ()",
-           _quantize)
+           _op_quantize)
 ops.define("w4_pack(Tensor(a!) q, Tensor(b!) sz, Tensor codes, Tensor scales, Tensor? zeros, "
-           "int group) -> ()", _pack)
-ops.define("w4_linear(Tensor(a!) y, Tensor x, Tensor q, Tensor sz, int group) -> ()", _linear)
-ops.define("w4_dequant(Tensor(a!) out, Tensor q, Tensor sz, int group) -> ()", _dequant)
+           "int group) -> ()", _op_pack)
+ops.define("w4_linear(Tensor(a!) y, Tensor x, Tensor q, Tensor sz, int group) -> ()", _op_linear)
+ops.define("w4_dequant(Tensor(a!) out, Tensor q, Tensor sz, int group) -> ()", _op_dequant)

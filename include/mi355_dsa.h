@@ -177,7 +177,7 @@ int mi355_dsa_mla_tree_attention(void* o, float* lse, const void* q, int64_t n_t
  * the first drafted token of every request of the set, are read through the
  * block-table row of its first request, once for all of its rows.  cu_seqlens_q
  * and tree_mask null: one token a request (n_tok = n_req).  Rows of requests of
- * no set are left as they were.  max_blocks * page_size < 2^24.  A shared
+ * no set are left as they were.  max_blocks * page_size < 2^23.  A shared
  * position counts as it is, an own one whose cache row holds an infinity or NaN
  * does not touch the rows that do not see it (those that do may get NaN for it).
  * It has no counterpart in the reference.

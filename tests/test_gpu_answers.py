@@ -175,3 +175,40 @@ def test_verify_tree_of_a_shared_prompt(pkg, lib, dev, fp8, dtype):
     assert torch.equal(out, pkg.dsa_layer.v_up(A.last_o, A.w))
     B.verify_tree(table=tab, **a)
     assert torch.equal(A.latent_cache, B.latent_cache) and torch.equal(A.idx_k_cache, B.idx_k_cache)
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled(pkg, lib, dev, backend):
+    """The operators in one compiled function, a whole graph: the eager results, bit for bit,
+    and the tables that they write."""
+    g = torch.Generator().manual_seed(9)
+    R, H, page = 3, 16, 16
+    w = pkg.w4.w4_quantize((torch.randn(H * 576, D, generator=g) * D ** -0.5).half().to(dev), 64)
+    cache = torch.randn(16, page, 576, generator=g).half().to(dev)
+    x = torch.randn(R, D, generator=g).half().to(dev)
+    cs, new = (torch.tensor(v, dtype=I32, device=dev) for v in ([0, 3], [1, 1, 1]))
+    mask = torch.ones(R, dtype=torch.int64, device=dev)
+
+    def run(x, bt, seq, free, count):
+        slots, pos, cu, granted = pkg.paging.extend_tables(bt, seq, new, free, count, page, 5)
+        shared = pkg.paging.shared_lengths(bt, seq, cs, page)
+        q = pkg.w4.w4_linear(x, w).view(R, H, 576)
+        o, lse = pkg.mla_prefix.shared_prefix_attention(q, cache, bt, seq, cs, shared, 0.05)
+        o2, lse2 = pkg.mla_prefix.shared_prefix_attention(q, cache, bt, seq, cs, shared, 0.05, cu, mask)
+        rows, lens = pkg.paging.token_tables(bt, seq, cu, 5, 4)
+        v = pkg.w4.w4_dequant(w) + 1
+        pkg.paging.truncate_tables(bt, seq, seq - 3, free, count, page)
+        return slots, pos, cu, granted, shared, o * 2, lse, o2, lse2, rows, lens, v
+
+    got = []
+    for f in (run, torch.compile(run, backend=backend, fullgraph=True)):
+        bt = torch.tensor([[3, 5, 7, -1, -1], [3, 5, 2, -1, -1], [3, 5, 1, -1, -1]], dtype=I32, device=dev)
+        seq = torch.tensor([33, 48, 34], dtype=I32, device=dev)
+        free = torch.tensor([8, 9, 10, 11, 0, 0], dtype=I32, device=dev)
+        count = torch.tensor([4], dtype=I32, device=dev)
+        for _ in range(2):
+            out = f(x, bt, seq, free, count)
+        got.append([*out, bt, seq, free, count])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert got[0][4].tolist() == [32] and bool(got[0][3].all())

@@ -113,3 +113,24 @@ def test_traced(pkg, lib):
     calls = [str(n.target) for n in g.graph.nodes if n.op == "call_function" and ns in str(n.target)]
     assert calls == [f"{ns}.{x}.default" for x in ("extend_tables", "token_tables", "shared_lengths",
                                                   "truncate_tables")]
+
+
+def test_ops_check_what_they_are_given(pkg, lib):
+    """A call of the registered op itself, with outputs that no function of paging has made."""
+    t, op = tensors("cpu"), pkg.ops.IMPLS
+    e = lambda *s, dtype=I32: torch.zeros(*s, dtype=dtype)
+    ins = (t["bt"], t["seq"], t["new"], t["free"], t["count"], 16)
+    outs = [e(5), e(5), e(4), e(3, dtype=torch.bool)]
+    names = ("slot_mapping", "positions", "cu_seqlens_q", "granted")
+    for i, bad in enumerate((e(5, dtype=torch.int64), e(4), e(3), e(3))):
+        with pytest.raises(RuntimeError, match=names[i]):
+            op["extend_tables"](*outs[:i], bad, *outs[i + 1:], *ins)
+    for out, lens in ((e(5, 5), e(5)), (e(5, 2), e(4)), (e(2, 5).t(), e(5)), (e(5), e(5)),
+                      (e(5, 2), e(5, dtype=torch.int64))):
+        with pytest.raises(RuntimeError, match="must be"):
+            op["token_tables"](out, lens, t["bt"], t["seq"], t["cu"])
+    for out in (e(3), e(2, dtype=torch.int64), e(4)[::2]):
+        with pytest.raises(RuntimeError, match="out must"):
+            op["shared_lengths"](out, t["bt"], t["seq"], t["cs"], 16)
+    with pytest.raises(RuntimeError, match="GPU"):
+        op["extend_tables"](*outs, *ins)

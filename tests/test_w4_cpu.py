@@ -118,3 +118,27 @@ def test_traced(pkg, lib):
     calls = [str(n.target) for n in g.graph.nodes if n.op == "call_function" and ns in str(n.target)]
     assert calls == [f"{ns}.{x}.default" for x in ("w4_quantize", "w4_pack", "w4_linear", "w4_linear",
                                                   "w4_dequant")]
+
+
+def test_ops_check_what_they_are_given(pkg, lib):
+    """A call of the registered op itself, with tensors that no function of w4 has made."""
+    op, w = pkg.ops.IMPLS, pkg.w4._empty(20, 64, 32, F16, "cpu")
+    e = lambda *s, dtype=F16: torch.zeros(*s, dtype=dtype)
+    codes, scales = e(20, 64, dtype=torch.uint8), e(20, 2)
+    for name, args, msg in [
+            ("w4_linear", (e(2, 20), e(2, 136), w.q, w.sz, 32), "not of weights"),
+            ("w4_linear", (e(2, 40), e(2, 64), w.q, w.sz, 32), "not of weights"),
+            ("w4_linear", (e(3, 20), e(2, 64), w.q, w.sz, 32), "out must"),
+            ("w4_linear", (e(2, 20).float(), e(2, 64).float(), w.q, w.sz, 32), "fp16 or bf16"),
+            ("w4_linear", (e(2, 20), e(2, 64), w.q, w.sz, 0), "group"),
+            ("w4_quantize", (w.q, w.sz, e(20, 136), 32, False), "not of weights"),
+            ("w4_quantize", (w.q, w.sz[:1], e(20, 64), 32, False), "not of weights"),
+            ("w4_quantize", (w.q, w.sz, e(40, 64), 32, False), "not of weights"),
+            ("w4_pack", (w.q, w.sz, codes, e(20, 1), None, 32), "scales"),
+            ("w4_pack", (w.q, w.sz, codes, scales, e(20, 2), 32), "zeros"),
+            ("w4_pack", (w.q, w.sz, codes[:16], scales[:16], None, 32), "not of weights"),
+            ("w4_dequant", (e(20, 136), w.q, w.sz, 32), "not of weights"),
+            ("w4_dequant", (e(64, 20).t(), w.q, w.sz, 32), "contiguous"),
+            ("w4_dequant", (e(20, 64), w.q, w.sz, 32), "GPU")]:
+        with pytest.raises(RuntimeError, match=msg):
+            op[name](*args)
