@@ -46,6 +46,12 @@ def compile_flags() -> list[str]:
     ]
 
 
+# Flags of one source.  Results of matrix instructions in vector registers, where vector
+# instructions read them: by itself the compiler puts them in accumulation registers, a copy for
+# each, once a kernel may use more than 256 (64 rows at [24576 x 6144] 32 us, so 29;
+# groups of 32 columns 56 and 38).
+SOURCE_FLAGS = {"w4_linear.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
 # Kernels of each source whose generated code the build checks (check_kernels):
 # those that hold values in accumulation registers named in inline asm, which
 # the compiler does not know to be in use.
@@ -179,7 +185,7 @@ def check_kernels(asm: str, own_agprs: list[str], no_spills: list[str] = []) -> 
 def _compile(src: str) -> str:
     name = os.path.basename(src)
     obj = os.path.join(BUILD_DIR, name.replace(".hip", ".o"))
-    cmd = [hipcc(), *compile_flags(), "-c", src, "-o", obj]
+    cmd = [hipcc(), *compile_flags(), *SOURCE_FLAGS.get(name, []), "-c", src, "-o", obj]
     checked = name in OWN_AGPRS or name in NO_SPILLS
     if checked:  # the assembly that the object is made from, beside it
         cmd.append("-save-temps=obj")

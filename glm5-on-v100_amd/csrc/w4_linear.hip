@@ -10,12 +10,13 @@
 // scales stand beside each other too: a word a row and group, the scale in its low half,
 // 16 + z in its high half.
 //
-// A code becomes the operand 16 + c by or-ing it into the mantissa of 16 (exact in fp16
-// and bf16): two instructions a pair.  In fp16 a packed subtraction of 16 + z then leaves
-// c - z, exact too, and with t = sum_k x (c - z) over a group its part of y is s t, in fp32.
-// bf16 has no packed subtraction: t = sum_k x (16 + c) and X = sum_k x, one more MFMA against
-// ones, give s (t - (16 + z) X).  No weight is rounded: the error is that of fp32
-// sums (bf16: of terms up to 31/15 as large), and y's own rounding.
+// In fp16 the nibbles or-ed into the mantissa of 1024 (low ones of a byte) or 64 (high ones)
+// are 1024 + c and 64 + c where they stand, one instruction a pair and a shift a word; a
+// packed subtraction of 1024 + z or 64 + z leaves c - z, all of it exact, and with t = sum_k
+// x (c - z) over a group its part of y is s t, in fp32.  bf16 has no packed subtraction and
+// too short a mantissa: shifted into that of 16 a code is 16 + c, and t = sum_k x (16 + c) and
+// X = sum_k x, one more MFMA against ones, give s (t - (16 + z) X).  No weight is rounded: the
+// error is that of fp32 sums (bf16: of terms up to 31/15 as large), and y's own rounding.
 #include "capi_internal.h"
 #include "dsa_common.h"
 
@@ -26,13 +27,6 @@ typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
 
 constexpr int kW4Rows = 16, kW4Cols = 128;  // of a tile
 constexpr int kW4MaxM = 64;
-
-template <bool BF16>
-struct W4Type {
-  static constexpr uint32_t k16 = BF16 ? 0x41804180u : 0x4c004c00u;  // 16, 16
-  static constexpr int kShift = BF16 ? 3 : 6;  // of a code whose unit is 1 in the mantissa of 16
-  static constexpr uint32_t kMask = 0x000f000fu << kShift;
-};
 
 template <bool BF16>
 __device__ __forceinline__ f32x4 w4_mfma(u32x4 a, u32x4 b, f32x4 c) {
@@ -51,15 +45,40 @@ __device__ __forceinline__ uint32_t w4_bits(float v) {
   if constexpr (BF16) return __builtin_bit_cast(uint16_t, (__bf16)v);
   else return __builtin_bit_cast(uint16_t, (f16)v);
 }
-// the eight codes of a word as 16 + c
+// The constants of w4_operand, in registers: a vector instruction takes no literal beside
+// a scalar register, so that (x & mask) | k would be two.
 template <bool BF16>
-__device__ __forceinline__ u32x4 w4_operand(uint32_t w) {
-  using T = W4Type<BF16>;
+struct W4Const {
+  uint32_t mask[2], k[2];
+};
+template <bool BF16>
+__device__ __forceinline__ W4Const<BF16> w4_const() {
+  W4Const<BF16> r;
+  if constexpr (BF16) r = {{0x00780078u, 0u}, {0x41804180u, 0u}};  // 16, 16
+  else r = {{0x000f000fu, 0x00f000f0u}, {0x64006400u, 0x54005400u}};  // 1024, 1024; 64, 64
+  asm volatile("" : "+s"(r.mask[0]), "+s"(r.mask[1]), "+v"(r.k[0]), "+v"(r.k[1]));
+  return r;
+}
+// the eight codes of a word: bf16 as 16 + c; fp16 as c - z, zero: -(1024 + z) and -(64 + z)
+template <bool BF16>
+__device__ __forceinline__ u32x4 w4_operand(uint32_t w, const W4Const<BF16>& k,
+                                            const f16x2 (&zero)[2]) {
   u32x4 r;
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const int sh = 4 * e - T::kShift;
-    r[e] = ((sh < 0 ? w << -sh : w >> sh) & T::kMask) | T::k16;
+  if constexpr (BF16) {
+    r[0] = ((w << 3) & k.mask[0]) | k.k[0];
+    r[1] = ((w >> 1) & k.mask[0]) | k.k[0];
+    r[2] = ((w >> 5) & k.mask[0]) | k.k[0];
+    r[3] = ((w >> 9) & k.mask[0]) | k.k[0];
+  } else {
+    const uint32_t w8 = w >> 8;
+    auto pair = [&](uint32_t x, int i) {
+      const uint32_t at = (x & k.mask[i]) | k.k[i];
+      return __builtin_bit_cast(uint32_t, (f16x2)(__builtin_bit_cast(f16x2, at) + zero[i]));
+    };
+    r[0] = pair(w, 0);
+    r[1] = pair(w, 1);
+    r[2] = pair(w8, 0);
+    r[3] = pair(w8, 1);
   }
   return r;
 }
@@ -121,23 +140,23 @@ struct W4Ring {
 // NT tiles a workgroup, GPB groups a block of 128 columns.  The blocks are cut in S x WAVES
 // runs, each of one wave.  A wave brings its blocks of weights, scales and x to a ring of its
 // own in LDS (no barrier), reads a block into registers and at once sends for the one that
-// takes its place.  x, which all workgroups read, is what bounds many rows: rows of x go to
-// every workgroup, 786 KB for 64 of 6144 columns, so that NT is large there, and the
-// workgroups begin their runs at different blocks (x's rows, 12 KB apart, would ask the
-// same L2 channels; 1 us of 20).
+// takes its place.  Rows of x go to every workgroup, 786 KB for 64 of 6144 columns, so that
+// NT is large where there are many, and the workgroups begin their runs at different blocks
+// (x's rows, 12 KB apart, would ask the same L2 channels; 1 us of 20).
 //
-// us with memory cold, [24576 x 6144] and [6144 x 24576]: 1 row 17.7 and 16.8 (4.6 TB/s),
-// 16 rows 18.8 and 18.1, 32 rows 21.5 and 20.3, 64 rows 30.0 and 29.8, the latter ones
-// without the join of S > 1 (2 to 4 us).  A kernel that loads x and weights into registers: 17, 21,
-// 26, 46 at the first.  By 64 rows what bounds it is x through the L2: 1.1 MB to each
-// CU, 10 TB/s in all.
+// us with memory cold, [24576 x 6144] and [6144 x 24576], groups of 128: 1 row 17.9 and 18.2
+// (4.6 TB/s), 16 rows 19.0 and 21.4, 32 rows 21.2 and 23.3, 64 rows 29.2 and 31.3, the latter
+// ones with the join of S > 1 (2 to 4 us).  Few rows are bound by memory.  64 rows: without the
+// loads 27, without x alone 29 of the then 33, without the unpacking 29: a wave alone on its
+// SIMD is bound by the instructions that it issues, so codes are unpacked in
+// as few as there are.  Not better: x shared by pairs of waves (31 and 35), two waves on a
+// SIMD, vector instructions spread between the MFMAs by hand (30).
 template <bool BF16, int MT, int XI, int NT, int GPB>
 __global__ void __launch_bounds__(64 * (XI == 1 ? 8 : 4)) w4_linear_kernel(W4Params p) {
   using R = W4Ring<MT, XI, NT, GPB>;
   constexpr int WAVES = R::Shape::kWaves, D = R::Shape::kD, XD = R::Shape::kXD;
   static_assert(XD == D || XD == 1, "x goes with the weights, or one block ahead");
-  // fp16: the zero point comes off the codes (exact), one packed subtraction a pair; bf16
-  // has none, there X is formed
+  // fp16: the zero point comes off the codes; bf16: X is formed
   constexpr bool SUB = !BF16;
   constexpr int kSteps = 4 / GPB;  // MFMAs of a group
   extern __shared__ __align__(16) uint8_t smem[];
@@ -162,6 +181,7 @@ __global__ void __launch_bounds__(64 * (XI == 1 ? 8 : 4)) w4_linear_kernel(W4Par
     for (int i = 0; i < MT; i++) acc[j][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
   constexpr uint32_t kOne = BF16 ? 0x3f803f80u : 0x3c003c00u;
   const u32x4 ones = {kOne, kOne, kOne, kOne};
+  const W4Const<BF16> kc = w4_const<BF16>();
 
   // In LDS the 16-byte piece k of row r of x stands at piece k ^ (r % 16), so that the
   // reads of a piece of 16 rows cover the banks.  Rows past M repeat the last one.
@@ -255,17 +275,16 @@ __global__ void __launch_bounds__(64 * (XI == 1 ? 8 : 4)) w4_linear_kernel(W4Par
         f32x4 t[MT];
 #pragma unroll
         for (int i = 0; i < MT; i++) t[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        const f16x2 zero = __builtin_bit_cast(f16x2, (sz[j][e] >> 16) * 0x10001u);
+        f16x2 zero[2] = {};
+        if constexpr (SUB) {
+          const f16x2 z16 = __builtin_bit_cast(f16x2, (sz[j][e] >> 16) * 0x10001u);
+          zero[0] = (f16x2){(f16)-1008.f, (f16)-1008.f} - z16;
+          zero[1] = (f16x2){(f16)-48.f, (f16)-48.f} - z16;
+        }
 #pragma unroll
         for (int s = 0; s < kSteps; s++) {
-          u32x4 b = w4_operand<BF16>(q[j][kSteps * e + s]);
-          if constexpr (SUB) {
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-              const uint32_t pair = b[k];  // a bit_cast of an element itself reads the first one
-              b[k] = __builtin_bit_cast(uint32_t, (f16x2)(__builtin_bit_cast(f16x2, pair) - zero));
-            }
-          }
+          const uint32_t word = q[j][kSteps * e + s];
+          const u32x4 b = w4_operand<BF16>(word, kc, zero);
 #pragma unroll
           for (int i = 0; i < MT; i++) t[i] = w4_mfma<BF16>(x[i][kSteps * e + s], b, t[i]);
         }
@@ -353,9 +372,11 @@ __global__ void __launch_bounds__(256) w4_join_kernel(W4Params p, int MT, int un
 
 // Tiles of a workgroup and slices of K, by the time that they are expected to take: the
 // workgroups of a CU one after the other, each its blocks at the time that a block of NT tiles was
-// measured to take (us, at sizes that fill the chip), and the join (4 us with its launch).  Slices pay where N
-// alone leaves CUs idle: 64 rows at [6144 x 24576] 54 us with one, 30 and the join
-// with four; at [24576 x 6144] one is best.
+// measured to take (us, at sizes that fill the chip), and the join (4 us with its launch).  Up
+// to 4 rows that time is the memory's, shared by the CUs, and three quarters of it with few
+// of them at work.  Slices pay where N alone leaves CUs idle: 64 rows at [6144 x 24576] 46 us
+// with two, 31 with four and the join; one row there 18 without, 21 with four; at
+// [24576 x 6144] one is best (64 rows 29, with two 37).
 struct W4Plan {
   int nt, s;
 };
@@ -363,16 +384,17 @@ static int w4_row_tiles(int M) { return M <= 16 ? 1 : M <= 32 ? 2 : 4; }
 static W4Plan w4_plan(int M, int N, int K) {
   const int tiles = (N + kW4Rows - 1) / kW4Rows, KB = (K + kW4Cols - 1) / kW4Cols;
   const bool few = M <= 4;
-  const float base = few ? 0.022f : M <= 16 ? 0.06f : M <= 32 ? 0.08f : 0.15f;
-  const float each = few ? 0.045f : M <= 16 ? 0.052f : M <= 32 ? 0.058f : 0.076f;
+  const float base = few ? 0.022f : M <= 16 ? 0.06f : M <= 32 ? 0.072f : 0.13f;
+  const float each = few ? 0.045f : M <= 16 ? 0.052f : M <= 32 ? 0.055f : 0.073f;
   W4Plan best = {1, 1};
   float least = 1e30f;
   for (const int nt : {1, 2, 3, 6}) {
     if (few && nt > 2) break;
     const int64_t groups = (tiles + nt - 1) / nt;
     for (int s = 1; s <= 16 && (s == 1 || 8 * s <= KB); s *= 2) {
-      const int64_t rounds = (groups * s + 255) / 256;
-      float t = (float)rounds * (float)((KB + s - 1) / s) * (base + each * (float)nt);
+      float rounds = (float)((groups * s + 255) / 256);
+      if (few) rounds = fmaxf(0.75f * rounds, (float)(groups * s) / 256.f);
+      float t = rounds * (float)((KB + s - 1) / s) * (base + each * (float)nt);
       if (s > 1) t += 4.f + (float)s * (float)w4_row_tiles(M) * (float)tiles * 2048.f / 6e6f;
       if (t < least) {
         least = t;
