@@ -111,11 +111,11 @@ template <int MT, int XI>
 struct W4Shape;
 template <>
 struct W4Shape<1, 1> {
-  static constexpr int kWaves = 8, kD = 3, kXD = 3;
+  static constexpr int kWaves = 8, kD = 2, kXD = 2;
 };
 template <>
 struct W4Shape<1, 4> {
-  static constexpr int kWaves = 4, kD = 3, kXD = 3;
+  static constexpr int kWaves = 4, kD = 2, kXD = 2;
 };
 template <>
 struct W4Shape<2, 8> {
@@ -144,9 +144,11 @@ struct W4Ring {
 // NT is large where there are many, and the workgroups begin their runs at different blocks
 // (x's rows, 12 KB apart, would ask the same L2 channels; 1 us of 20).
 //
-// us with memory cold, [24576 x 6144] and [6144 x 24576], groups of 128: 1 row 17.9 and 18.2
-// (4.6 TB/s), 16 rows 19.0 and 21.4, 32 rows 21.2 and 23.3, 64 rows 29.2 and 31.3, the latter
-// ones with the join of S > 1 (2 to 4 us).  Few rows are bound by memory.  64 rows: without the
+// us with memory cold, [24576 x 6144] and [6144 x 24576], groups of 128: 1 row 16.5 and 17.9
+// (5.0 TB/s), 16 rows 18.1 and 20.5, 32 rows 21.2 and 23.3, 64 rows 29.2 and 31.0, the latter
+// ones with the join of S > 1 (2 to 4 us); groups of 32 at the first 20, 24, 27, 39.  Few rows
+// are bound by memory; two blocks on their way leave room for a second workgroup on a CU, with
+// three 17.9, 19.0 and (groups of 32) 26, 25.  64 rows: without the
 // loads 27, without x alone 29 of the then 33, without the unpacking 29: a wave alone on its
 // SIMD is bound by the instructions that it issues, so codes are unpacked in
 // as few as there are.  Not better: x shared by pairs of waves (31 and 35), two waves on a
