@@ -41,8 +41,8 @@ template <bool FP8>
 struct TreeSmem {
   uint8_t ring[tree_slots(FP8)][kTreeSlotBytes];
   uint8_t raw[FP8 ? 2 : 1][FP8 ? kTreeWaves : 1][FP8 ? kTreeRaw : 16];
-  uint64_t see[kTreeRows];      // masks of the rows' tokens
   int32_t blk[kTreePages];      // cache blocks of the segment, -1: none
+  uint64_t see[kTreeRows];      // masks of the rows' tokens
   uint32_t dirty[kTreeWaves];
   int gap;  // some block of the segment is missing
   // of each wave, over the loops: first row, rows and group of the request, place of
@@ -337,6 +337,32 @@ __device__ __forceinline__ void tree_zero(uint8_t* slot, uint32_t keys) {
   asm volatile("" ::: "memory");
 }
 
+// Q of a wave by way of LDS (the ring and what follows it, free between two pieces): its n rows
+// are contiguous, and come in whole lines, where a lane's 36 loads of its row touch 32 lines each.
+// The 16-byte piece p of them is source piece p ^ ((p >> 3) & 7), so that reads of eight rows
+// cover the banks.
+static_assert(offsetof(TreeSmem<false>, see) >= kTreeRows * kLatentDim * 2 &&
+                  offsetof(TreeSmem<true>, see) >= kTreeRows * kLatentDim * 2,
+              "Q of the four waves");
+template <class Lds>
+__device__ __forceinline__ void tree_stage_q(f16x8 (&qf)[36], const f16* rows, int at, int n, Lds& sh) {
+  lds_barrier();  // every wave is done with the piece before
+  if (n <= 0) return;
+  const int l = tree_tid() & 63, c = l & 31, hf = l >> 5;
+  uint8_t* const to = sh.ring[0] + at;
+  const int last = n * kLatentDim * 2 - 16, off = 16 * (l ^ (l >> 3));
+#pragma unroll
+  for (int k = 0; k < 36; k++)  // past the last row its end again
+    dma16(reinterpret_cast<const uint8_t*>(rows) + min(1024 * k + off, last), to + 1024 * k);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int s = 0; s < 36; s++) {
+    const int p = 8 * (9 * c + s / 4) + ((2 * (s % 4) + hf) ^ ((c + s / 4) & 7));
+    qf[s] = *reinterpret_cast<const f16x8*>(to + 16 * p);
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the ring is written
+}
+
 // PE_BF16: the rope values of the (fp8) rows are bf16.  SHARED: the groups' keys are those
 // of mla_prefix_plan.h (the kernel's parameters are PrefixParams).
 template <bool FP8, bool PE_BF16, bool SHARED>
@@ -427,12 +453,18 @@ __device__ __forceinline__ void tree_attention(const TreeParams& p) {
     {
       const int c = tree_tid() & 31, hf = (tree_tid() >> 5) & 1;
       const int m = min(m0 + c, M - 1);
-      const f16* qrow = p.q + ((int64_t)it.first * p.H + m) * kLatentDim;
-#pragma unroll
-      for (int s = 0; s < kLatentDim / 16; s++)
-        qf[s] = *reinterpret_cast<const f16x8*>(qrow + 16 * s + 8 * hf);
       const int tok = it.first + (uint32_t)m / (uint32_t)p.H;
-      sh.see[32 * wave() + c] = SHARED && p.mask == nullptr ? 1 : (uint64_t)p.mask[tok];
+      const uint64_t see = SHARED && p.mask == nullptr ? 1 : (uint64_t)p.mask[tok];
+      const f16* rows = p.q + ((int64_t)it.first * p.H + m0) * kLatentDim;  // of the wave, contiguous
+      if constexpr (SHARED) {
+        tree_stage_q(qf, rows, 32 * kLatentDim * 2 * wave(), min(M - m0, 32), sh);
+      } else {
+        const f16* qrow = rows + (m - m0) * kLatentDim;
+#pragma unroll
+        for (int s = 0; s < kLatentDim / 16; s++)
+          qf[s] = *reinterpret_cast<const f16x8*>(qrow + 16 * s + 8 * hf);
+      }
+      sh.see[32 * wave() + c] = see;
       if (p.q_sign != 1.f) {  // else nothing waits for Q before the first product
         const f16 sg = (f16)p.q_sign;
         const f16x8 sg8 = {sg, sg, sg, sg, sg, sg, sg, sg};
