@@ -346,8 +346,8 @@ extern "C" size_t mi355_dsa_mla_prefix_workspace_size(int64_t n_tok, int n_head,
   return up16((size_t)2 * kTreeWGs * prefix_part_waves(n_tok, n_head) * (kTreePartWave + 64) *
               sizeof(float)) +
          64 + up16(most * sizeof(PrefixGroup)) + up16(kTreeWGs * sizeof(PrefixRun)) +
-         up16((most + 1) * 8) + up16((size_t)n_req * sizeof(PrefixReq)) + up16((size_t)n_tok * 4) + up16(n_set * sizeof(PrefixSet)) +
-         up16(((size_t)n_set + 1) * 4);
+         up16((most + 1) * 8) + up16((size_t)n_req * sizeof(PrefixReq)) + up16((size_t)n_tok * 4) +
+         up16((size_t)n_set * sizeof(PrefixSet)) + up16(((size_t)n_set + 1) * 4);
 }
 
 extern "C" int mi355_dsa_mla_prefix_attention(

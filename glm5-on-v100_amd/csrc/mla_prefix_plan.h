@@ -55,7 +55,9 @@ __device__ __forceinline__ PrefixTokens prefix_tokens(const TreeParams& p, int r
   const int a = min(max(p.cu[r], 0), p.T);
   return {a, min(max(p.cu[r + 1], a), p.T)};
 }
-__device__ __forceinline__ int prefix_tiles(int64_t keys) { return (int)((keys + kTreeTile - 1) / kTreeTile); }
+__device__ __forceinline__ int prefix_tiles(int64_t keys) {
+  return (int)((keys + kTreeTile - 1) / kTreeTile);
+}
 
 // ---- a workgroup's pieces ----
 struct PrefixItem {
@@ -222,7 +224,9 @@ __device__ __forceinline__ uint32_t prefix_visible(const PrefixOwn& o, uint64_t 
   const int shift = o.draft - key0;
   uint32_t keys = below(o.end - key0) & ~below(o.from - key0);
   if (shift < 32)
-    keys &= shift >= 0 ? (uint32_t)(see << shift) | below(shift) : shift > -64 ? (uint32_t)(see >> -shift) : 0u;
+    keys &= shift >= 0    ? (uint32_t)(see << shift) | below(shift)
+            : shift > -64 ? (uint32_t)(see >> -shift)
+                          : 0u;
   return keys;
 }
 
