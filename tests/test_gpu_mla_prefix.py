@@ -312,3 +312,17 @@ def test_other_stream_and_graph(pkg, lib, dev):
         check(eager, w2)
         check(r2, w2)
         check(r1, w1 if k % 2 == 0 else ws)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("H,n", [(5, 3), (1, 1), (33, 1), (16, 9)])
+def test_a_bad_last_query_row(pkg, lib, dev, H, n, bad):
+    """The last row of a set in a wave that it does not fill: the others keep their bits."""
+    c = make([(96, [(20, 1)] * n), (32, [(3, 1)] * 2)], H, 16, "fp16", seed=8)
+    want = call(pkg, c, dev)
+    c["q"][n - 1, H - 1, -4:] = bad
+    got = call(pkg, c, dev)
+    rest = torch.ones(n + 2, H, dtype=torch.bool, device=dev)
+    rest[n - 1, H - 1] = False
+    assert torch.equal(got[0][rest], want[0][rest]) and torch.equal(got[1][rest], want[1][rest])
+    assert not bool(got[1][n - 1, H - 1].isfinite()) or bad == math.inf
