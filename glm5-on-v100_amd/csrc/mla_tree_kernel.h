@@ -325,14 +325,18 @@ __device__ __forceinline__ uint32_t tree_bad(const uint8_t* slot, uint32_t keys)
   }
   return found;
 }
-// Zeros in place of such keys: nothing but NaN comes of them in the rows that see them.
+// Zeros in place of the values of such keys: nothing but NaN comes of them in the rows that
+// see them.  The 64 pieces of the value blocks, one a lane, and no more: the scores of the tile
+// are there, and fp8 rows have a ring of three, in which another wave may have sent for the rope
+// values of tile i + 3, to the rope blocks of the slot of tile i.
 __device__ __forceinline__ void tree_zero(uint8_t* slot, uint32_t keys) {
+  static_assert(4 * (kValueDim / 32) == 64, "a piece a lane");
   const int lane = tree_tid() & 63;
+  uint8_t* const at = slot + 2048 * (lane >> 2) + 16 * (lane & 3);
   while (keys) {
     const int k = __builtin_ctz(keys);
     keys &= keys - 1;
-    for (int i = lane; i < 4 * kTreeBlocks; i += 64)
-      *reinterpret_cast<u32x4*>(slot + 2048 * (i >> 2) + 64 * k + 16 * (i & 3)) = (u32x4){0u, 0u, 0u, 0u};
+    *reinterpret_cast<u32x4*>(at + 64 * k) = (u32x4){0u, 0u, 0u, 0u};
   }
   asm volatile("" ::: "memory");
 }

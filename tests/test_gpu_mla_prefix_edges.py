@@ -1,0 +1,52 @@
+"""Attention over a shared prefix where keys of one request stand beside those of others:
+rows that are not finite.  Oracle and tolerances as in test_gpu_mla_prefix."""
+import math
+
+import pytest
+import torch
+from test_gpu_mla_prefix import call, check, make, oracle
+
+pytestmark = pytest.mark.gpu
+I32 = torch.int32
+
+
+def row_of(c, r, p):
+    return int(c["bt"][r, p // c["page"]]) * c["page"] + p % c["page"]
+
+
+def spoil(c, rows, bad):
+    """Every value of the rows, or (fp8) their scales and rope values."""
+    if c["rows"].dtype == torch.uint8:
+        c["rows"][rows, 512:528] = torch.full((4,), bad).view(torch.uint8)
+        c["rows"][rows, 528:] = torch.full((64,), bad, dtype=torch.float16).view(torch.uint8)
+    else:
+        c["rows"][rows] = bad
+
+
+def bf16_rope(c):
+    """The cache's rope values as bf16, and (first) the case that the oracle sees."""
+    b = c["rows"][:, 528:].contiguous().view(torch.float16).to(torch.bfloat16)
+    seen = dict(c, rows=c["rows"].clone())
+    seen["rows"][:, 528:] = b.to(torch.float16).view(torch.uint8)
+    c["rows"][:, 528:] = b.view(torch.uint8)
+    return seen, c
+
+
+@pytest.mark.parametrize("kv", ["fp16", "fp8", "bf16 rope"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("H", [4, 16])
+def test_whole_tiles_of_bad_rows(pkg, lib, dev, kv, bad, H):
+    """A request whose own rows are all bad, in front of others' rows in one line of tiles, six
+    tiles long, with waves that have no rows; then a bad tile in the middle of it."""
+    for first, sizes in [(0, [40, 70, 50, 60]), (1, [30, 40, 70, 60])]:
+        c = make([(64, [(n, 1) for n in sizes])], H, 16, "fp16" if kv == "fp16" else "fp8", seed=first)
+        seen, c = bf16_rope(c) if kv == "bf16 rope" else (c, c)
+        want = oracle(seen)
+        rows = [row_of(c, first, p) for p in range(64, 64 + sizes[first])]
+        spoil(c, torch.tensor(rows), bad)
+        if kv == "bf16 rope":
+            c["rows"][torch.tensor(rows), 528:] = torch.full((64,), bad, dtype=torch.bfloat16).view(torch.uint8)
+        more = dict(pe_dtype=torch.bfloat16) if kv == "bf16 rope" else {}
+        got = call(pkg, c, dev, **more)
+        check(got, want, torch.arange(4) != first)
+        assert not bool(got[0][first].isfinite().any()) and bool(got[1][first].isnan().all())
