@@ -151,12 +151,15 @@ __global__ void __launch_bounds__(FEW ? kPlanFew : kPlanThreads) prefix_plan_ker
   for (int s = wave; s < p.S; s += NT / 64) {
     const int lead = min(max(cu_shared[s], 0), t.R), end = min(max(cu_shared[s + 1], lead), t.R);
     // what every token sees: positions before the first drafted one
-    int ctx = INT32_MAX;
+    int ctx = INT32_MAX, row = INT32_MAX;
     for (int r = lead + lane; r < end; r += 64) {
       const PrefixTokens k = tokens(r);
-      if (k.b > k.a) ctx = min(ctx, length(r) - (k.b - k.a));
+      if (k.b <= k.a) continue;
+      ctx = min(ctx, length(r) - (k.b - k.a));
+      row = min(row, r);
     }
     ctx = wave_min_i32(ctx);
+    row = wave_min_i32(row);
     int P = 0;
     if (ctx != INT32_MAX) P = (int)min((int64_t)max(0, min(shared[s], ctx)), width);
     for (int r = lead + lane; r < end; r += 64) {
@@ -172,7 +175,7 @@ __global__ void __launch_bounds__(FEW ? kPlanFew : kPlanThreads) prefix_plan_ker
         first = tokens(lead).a;
         last = max(first, tokens(end - 1).b);
       }
-      sets[s] = {first, (last - first) * t.H, P, lead, end};
+      sets[s] = {first, (last - first) * t.H, P, lead, end, row};
     }
   }
   __syncthreads();
@@ -220,7 +223,7 @@ __global__ void __launch_bounds__(FEW ? kPlanFew : kPlanThreads) prefix_plan_ker
       q.M = set.M;
       q.g = i - before[s];
       q.P = set.P;
-      q.lead = set.lead;
+      q.lead = set.row;
       const int m1 = min((q.g + 1) * kTreeRows, q.M) - 1;
       const int t0 = q.first + (uint32_t)(q.g * kTreeRows) / (uint32_t)t.H;
       const int t1 = q.first + (uint32_t)m1 / (uint32_t)t.H;

@@ -20,6 +20,7 @@ struct PrefixGroup {
 };
 struct PrefixSet {  // requests that share
   int first, M, P, lead, end;  // lead .. end - 1
+  int row;  // the first of them that has a token: it holds all of P, as others need not
 };
 struct PrefixReq {  // a request
   int64_t upto;  // sum of the own keys of the requests up to and with it

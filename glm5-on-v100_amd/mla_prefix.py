@@ -25,9 +25,10 @@ def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
                             pe_dtype: torch.dtype = torch.float16):
     """The requests cu_shared[g] .. cu_shared[g + 1] - 1 (int32 [groups + 1]) hold their first
     shared_lens[g] positions (int32 [groups]; paging.shared_lengths finds them) in the
-    same cache rows, which are read through the first one's block-table row.  A group may
-    be one request, and share nothing; positions that a drafted token takes, or that the
-    shortest request of a group lacks, do not count as shared.
+    same cache rows, which are read through the block-table row of the first one that has a
+    token.  A group may be one request, and share nothing; positions that a drafted token
+    takes, or that the shortest request of a group lacks, do not count as shared (requests
+    without a token, which cu_seqlens_q may have, are not looked at).
 
     q [T, H, 576] fp16 (q_latent form).  Without cu_seqlens_q: one token a request, T of them,
     token r at position seq_lens[r] - 1, which sees everything up to itself.  With

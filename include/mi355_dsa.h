@@ -174,9 +174,10 @@ int mi355_dsa_mla_tree_attention(void* o, float* lse, const void* q, int64_t n_t
  * same arguments and results) where the requests cu_shared[g] .. cu_shared[g + 1]
  * - 1 (int32 [n_set + 1]) of set g hold their first shared_lens[g] positions
  * (int32 [n_set]) in the same cache rows.  Those, at most the positions before
- * the first drafted token of every request of the set, are read through the
- * block-table row of its first request, once for all of its rows.  cu_seqlens_q
- * and tree_mask null: one token a request (n_tok = n_req).  Rows of requests of
+ * the first drafted token of every request of the set that has a token, are
+ * read through the block-table row of the first such request, once for all of
+ * its rows.  cu_seqlens_q and tree_mask null: one token a request (n_tok =
+ * n_req).  Rows of requests of
  * no set are left as they were.  max_blocks * page_size < 2^23.  A shared
  * position counts as it is, an own one whose cache row holds an infinity or NaN
  * does not touch the rows that do not see it (those that do may get NaN for it).

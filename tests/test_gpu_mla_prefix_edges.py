@@ -1,5 +1,6 @@
 """Attention over a shared prefix where keys of one request stand beside those of others:
-rows that are not finite.  Oracle and tolerances as in test_gpu_mla_prefix."""
+rows that are not finite, requests without a token.  Oracle and tolerances as in
+test_gpu_mla_prefix."""
 import math
 
 import pytest
@@ -50,3 +51,16 @@ def test_whole_tiles_of_bad_rows(pkg, lib, dev, kv, bad, H):
         got = call(pkg, c, dev, **more)
         check(got, want, torch.arange(4) != first)
         assert not bool(got[0][first].isfinite().any()) and bool(got[1][first].isnan().all())
+
+
+@pytest.mark.parametrize("kv", ["fp16", "fp8"])
+@pytest.mark.parametrize("H", [4, 32])
+def test_first_requests_without_a_token(pkg, lib, dev, kv, H):
+    """Groups whose first requests take no part in the step: ended, with no page left, or short,
+    with fewer pages than the others share."""
+    c = make([(320, [(9, 0), (70, 2), (5, 1), (12, 3)]), (64, [(9, 0)]), (96, [(3, 0), (4, 0), (40, 1)]),
+              (200, [(20, 2), (6, 1)])], H, 16, kv, seed=2)
+    c["bt"][0], c["seq"][0] = -1, 0
+    c["bt"][5, 2:], c["seq"][5] = -1, 32
+    c["bt"][6], c["seq"][6] = -1, 0
+    check(call(pkg, c, dev), oracle(c))
