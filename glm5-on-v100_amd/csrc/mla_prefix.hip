@@ -191,7 +191,8 @@ __global__ void __launch_bounds__(FEW ? kPlanFew : kPlanThreads) prefix_plan_ker
     q.upto = carry + plan_scan<NT>((Sum)q.own, ws, &total);
     if (r < t.R) {
       const PrefixTokens k = tokens(r);
-      q.draft0 = length(r) - (k.b - k.a);
+      // past the table nothing is drafted; and sums with it stay within 31 bits
+      q.draft0 = (int)min((int64_t)(length(r) - (k.b - k.a)), width);
       p.reqs[r] = q;
       if (p.request != nullptr)
         for (int i = k.a; i < k.b; i++) p.request[i] = r;

@@ -26,7 +26,7 @@ struct PrefixReq {  // a request
   int64_t upto;  // sum of the own keys of the requests up to and with it
   int own;       // its own, up to the next tile's (see PrefixGroup)
   int real;      // without that
-  int draft0;    // position of its first drafted token
+  int draft0;    // position of its first drafted token, at most the table's width
 };
 struct PrefixRun {  // cells: the piece of a workgroup
   int group, lo, hi, place;

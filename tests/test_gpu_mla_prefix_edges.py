@@ -1,6 +1,6 @@
 """Attention over a shared prefix where keys of one request stand beside those of others:
-rows that are not finite, requests without a token.  Oracle and tolerances as in
-test_gpu_mla_prefix."""
+rows that are not finite, requests without a token, lengths past the table.  Oracle and
+tolerances as in test_gpu_mla_prefix."""
 import math
 
 import pytest
@@ -63,4 +63,15 @@ def test_first_requests_without_a_token(pkg, lib, dev, kv, H):
     c["bt"][0], c["seq"][0] = -1, 0
     c["bt"][5, 2:], c["seq"][5] = -1, 32
     c["bt"][6], c["seq"][6] = -1, 0
+    check(call(pkg, c, dev), oracle(c))
+
+
+@pytest.mark.parametrize("kv", ["fp16", "fp8"])
+@pytest.mark.parametrize("H", [4, 32])
+@pytest.mark.parametrize("n", [1, 3])
+def test_lengths_near_2_31(pkg, lib, dev, kv, H, n):
+    """Lengths past the table, of requests behind others in a row group: every key that the table
+    holds is context."""
+    c = make([(16, [(90, n), (20, n), (40, n)]), (0, [(35, 1), (50, n)])], H, 16, kv, seed=3)
+    c["seq"][1], c["seq"][2], c["seq"][4] = 2 ** 31 - 1, 2 ** 31 - 60, 2 ** 31 - 1
     check(call(pkg, c, dev), oracle(c))
