@@ -15,8 +15,13 @@
 // packed subtraction of 1024 + z or 64 + z leaves c - z, all of it exact, and with t = sum_k
 // x (c - z) over a group its part of y is s t, in fp32.  bf16 has no packed subtraction and
 // too short a mantissa: shifted into that of 16 a code is 16 + c, and t = sum_k x (16 + c) and
-// X = sum_k x, one more MFMA against ones, give s (t - (16 + z) X).  No weight is rounded: the
-// error is that of fp32 sums (bf16: of terms up to 31/15 as large), and y's own rounding.
+// X = sum_k x, one more MFMA against ones, give s (t - (16 + z) X).  128 terms of 31 |x| would
+// pass the end of the range for x from 2^116 on, whatever c - z and s make of them: codes and
+// ones enter 2^-12 as large and y is multiplied by 2^12, both exact: x has no bit below 2^-133,
+// so that its terms are multiples of 2^-145, which fp32 holds (of y, 2^-138 a group is lost).
+// No weight is rounded: the error is that of fp32 sums, and y's own rounding.  In fp16 their
+// terms are x (c - z) and vanish where c = z; in bf16 two sums of terms of up to 31 |x| are
+// subtracted, an error in units of 31 s sum |x| whatever c - z is.
 #include "capi_internal.h"
 #include "dsa_common.h"
 
@@ -51,15 +56,20 @@ template <bool BF16>
 struct W4Const {
   uint32_t mask[2], k[2];
 };
+constexpr float kW4Up = 0x1p12f;  // of bf16 products, their codes 2^-12 as large
+template <bool BF16>
+__device__ __forceinline__ uint16_t w4_result(float v) {
+  return (uint16_t)w4_bits<BF16>(BF16 ? v * kW4Up : v);
+}
 template <bool BF16>
 __device__ __forceinline__ W4Const<BF16> w4_const() {
   W4Const<BF16> r;
-  if constexpr (BF16) r = {{0x00780078u, 0u}, {0x41804180u, 0u}};  // 16, 16
+  if constexpr (BF16) r = {{0x00780078u, 0u}, {0x3b803b80u, 0u}};  // 2^-8, 2^-8
   else r = {{0x000f000fu, 0x00f000f0u}, {0x64006400u, 0x54005400u}};  // 1024, 1024; 64, 64
   asm volatile("" : "+s"(r.mask[0]), "+s"(r.mask[1]), "+v"(r.k[0]), "+v"(r.k[1]));
   return r;
 }
-// the eight codes of a word: bf16 as 16 + c; fp16 as c - z, zero: -(1024 + z) and -(64 + z)
+// the eight codes of a word: bf16 as 2^-12 (16 + c); fp16 as c - z, zero: -(1024 + z), -(64 + z)
 template <bool BF16>
 __device__ __forceinline__ u32x4 w4_operand(uint32_t w, const W4Const<BF16>& k,
                                             const f16x2 (&zero)[2]) {
@@ -181,7 +191,7 @@ __global__ void __launch_bounds__(64 * (XI == 1 ? 8 : 4)) w4_linear_kernel(W4Par
   for (int j = 0; j < NT; j++)
 #pragma unroll
     for (int i = 0; i < MT; i++) acc[j][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  constexpr uint32_t kOne = BF16 ? 0x3f803f80u : 0x3c003c00u;
+  constexpr uint32_t kOne = BF16 ? 0x39803980u : 0x3c003c00u;  // bf16: 2^-12
   const u32x4 ones = {kOne, kOne, kOne, kOne};
   const W4Const<BF16> kc = w4_const<BF16>();
 
@@ -346,7 +356,7 @@ __global__ void __launch_bounds__(64 * (XI == 1 ? 8 : 4)) w4_linear_kernel(W4Par
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         const int m = 16 * i + 4 * g + r;
-        if (m < p.M) p.y[(int64_t)m * p.N + n] = (uint16_t)w4_bits<BF16>(acc[j][i][r]);
+        if (m < p.M) p.y[(int64_t)m * p.N + n] = w4_result<BF16>(acc[j][i][r]);
       }
   }
 }
@@ -368,7 +378,7 @@ __global__ void __launch_bounds__(256) w4_join_kernel(W4Params p, int MT, int un
 #pragma unroll
   for (int r = 0; r < 4; r++) {
     const int m = 16 * i + 4 * (lane >> 4) + r;
-    if (m < p.M) p.y[(int64_t)m * p.N + n] = (uint16_t)w4_bits<BF16>(v[r]);
+    if (m < p.M) p.y[(int64_t)m * p.N + n] = w4_result<BF16>(v[r]);
   }
 }
 

@@ -107,9 +107,11 @@ def _pack(q, sz, codes, scales, zeros, group):
 
 def w4_linear(x: torch.Tensor, w: W4Weight, out: torch.Tensor | None = None) -> torch.Tensor:
     """x [M, K] times the transposed weights: [M, N] in x's type (the weights'), M at most
-    64 rows.  Weights enter unrounded, sums are fp32.  Of x in bf16, a value from 2^122 on or
-    an infinity may make NaN of its row of y where the product is infinite.  Prefill-sized
-    products: w4_dequant and a matrix product."""
+    64 rows.  Weights enter unrounded, sums are fp32.  In bf16 two sums are subtracted, so
+    that fp32's error is in units of 31 * scale * sum |x| of a group whatever its codes
+    (fp16: of |x (code - zero point)|), and an infinity of x makes its row of y NaN, also
+    where the formula gives an infinity.  Prefill-sized products: w4_dequant and a matrix
+    product."""
     _no_grad(x)
     _check(x.dim() == 2 and x.size(1) == w.k, "x must be [M, K]")
     _check(x.dtype == w.dtype, "x must have the weights' type")
