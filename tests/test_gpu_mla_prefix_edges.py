@@ -1,6 +1,6 @@
 """Attention over a shared prefix where keys of one request stand beside those of others:
-rows that are not finite, requests without a token, lengths past the table.  Oracle and
-tolerances as in test_gpu_mla_prefix."""
+rows that are not finite, requests without a token, lengths past the table, own keys in several
+segments.  Oracle and tolerances as in test_gpu_mla_prefix."""
 import math
 
 import pytest
@@ -74,4 +74,31 @@ def test_lengths_near_2_31(pkg, lib, dev, kv, H, n):
     holds is context."""
     c = make([(16, [(90, n), (20, n), (40, n)]), (0, [(35, 1), (50, n)])], H, 16, kv, seed=3)
     c["seq"][1], c["seq"][2], c["seq"][4] = 2 ** 31 - 1, 2 ** 31 - 60, 2 ** 31 - 1
+    check(call(pkg, c, dev), oracle(c))
+
+
+def pooled(sets, H, page, seed):
+    """As make, with the pages of all requests out of a pool of 256."""
+    g = torch.Generator().manual_seed(seed)
+    lens = [P + n for P, reqs in sets for n in reqs]
+    W = max(-(-n // page) for n in lens)
+    bt = torch.randint(0, 256, (len(lens), W), generator=g).int()
+    cs = [0]
+    for P, reqs in sets:
+        bt[cs[-1]:cs[-1] + len(reqs), :P // page] = bt[cs[-1], :P // page].clone()
+        cs.append(cs[-1] + len(reqs))
+    R = len(lens)
+    return dict(q=torch.randn(R, H, 576, generator=g).half(), page=page, bt=bt,
+                rows=torch.randn(256 * page, 576, generator=g).half(), seq=torch.tensor(lens, dtype=I32),
+                mask=torch.ones(R, dtype=torch.int64), cu=torch.arange(R + 1, dtype=I32),
+                cs=torch.tensor(cs, dtype=I32), shared=torch.tensor([P for P, _ in sets], dtype=I32))
+
+
+@pytest.mark.parametrize("sets,H", [
+    ([(0, [2500 + i % 9])for i in range(300)], 1),              # one request's keys
+    ([(16, [900, 870 + i % 60, 905]) for i in range(300)], 4),  # keys of three
+    ([(0, [4100, 40, 70 + i % 30]) for i in range(130)], 32)])  # many of one, then others'
+def test_more_own_keys_than_a_segment_takes(pkg, lib, dev, sets, H):
+    """A workgroup's piece holds more than the 64 tiles of own keys that are resolved at a time."""
+    c = pooled(sets, H, 16, seed=H)
     check(call(pkg, c, dev), oracle(c))
