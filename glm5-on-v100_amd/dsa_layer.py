@@ -45,8 +45,8 @@ decode would give: rotary positions of q and k_pe with the latent rows written i
 the same launch (rope_concat_and_cache_mla), the indexer's key rotated and stored,
 step 3, the attention, step 5.  Where the block table holds at most topk positions
 the selection keeps every key and the attention is tree attention, one matrix
-product of all heads of a draft and their request's context (told of requests that share
-their first positions, of all their drafts and those); in longer tables it is
+product of all heads of a draft and their request's context (told of many requests that
+share their first positions, of all their drafts and those); in longer tables it is
 steps 2 and 4, each drafted token with its own selection out of what it sees.
 
 All buffers come from torch's caching allocator; nothing here synchronises
@@ -410,9 +410,9 @@ class DsaLayer:
         indexer chooses, as in decode (last_idx), with the indexer's keys in the cache or
         given as idx_k.  cu_shared and shared_lens (mla_prefix.shared_prefix_attention; the
         groups cover the requests) tell which requests hold their first positions in the
-        same rows: where every key is attended to, those are read once for all of them.  q,
-        k_pe, idx_k and idx_q stay as they are.  Returns out [T, H * V], zero for tokens of
-        no request (of no group)."""
+        same rows: where every key is attended to, and that is faster (mla_prefix.pays),
+        those are read once for all of them.  q, k_pe, idx_k and idx_q stay as they are.
+        Returns out [T, H * V], zero for tokens of no request."""
         T = slot_mapping.numel()
         _check(q.dim() == 3 and q.shape == (T, self.w.n_heads, self.w.nope_dim + 64),
                "q must be [T, H, P + 64], a slot for each token")
@@ -470,7 +470,8 @@ class DsaLayer:
         H = self.w.n_heads
         o = torch.zeros(T, H, 512, dtype=torch.float16, device=q.device)
         lse = torch.full((T, H), float("-inf"), dtype=torch.float32, device=q.device)
-        if cu_shared is None:
+        if cu_shared is None or not mla_prefix.pays(
+                T, H, R, shared_lens.shape[0], block_table.shape[1] * self.latent_cache.shape[-2]):
             mla_tree.tree_attention(ql, self.latent_cache, block_table, seq_lens, cu_seqlens_q,
                                     tree_mask, self.w.scale, o, lse)
         else:

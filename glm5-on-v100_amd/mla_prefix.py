@@ -16,6 +16,24 @@ from .mla_tree import _check_trees
 from .ops import _check, _contig, _launch, _no_grad, _traced
 
 
+def pays(n_tok: int, n_head: int, n_req: int, n_group: int, positions: int) -> bool:
+    """Whether drafted trees of requests that share most of `positions` are expected to be
+    attended to faster here than by tree_attention, from what the host knows.
+
+    Row groups of 128 (token, head) rows meet each 32 keys as one tile: tree attention needs
+    ceil(n_head * tokens / 128) of them for each request, here the requests' rows fill them
+    together.  A tile spared saves 3 to 5 ns, and the division of the work, a launch of its own,
+    costs 8 to 12 us.  us here / by tree attention, 16 heads, one token a request, 2048
+    positions of fp16 rows: 16 requests 40 / 36, 64 (3520 tiles spared) 51 / 52, 128 56 / 82; 64
+    heads: 64 (1984) 66 / 56, 128 (4032) 81 / 88.  Tree attention's workgroups each sum over
+    all requests: with two drafted tokens of 64 heads, where no tile is spared, 128 requests
+    117 / 114, 160 137 / 148, 256 170 / 190; but 160 groups of one request 171 / 159, 130 of
+    two (16 heads, 1024 positions) 100 / 140."""
+    alone = n_req * -(-n_tok * n_head // (128 * max(n_req, 1)))
+    spared = (alone - n_tok * n_head // 128 - n_group) * (positions // 32)
+    return (n_req > 128 and 2 * n_group <= n_req) or spared >= 3500
+
+
 def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor,
                             seq_lens: torch.Tensor, cu_shared: torch.Tensor,
                             shared_lens: torch.Tensor, scale: float,
