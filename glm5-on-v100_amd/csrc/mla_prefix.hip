@@ -21,6 +21,15 @@
 // among the scores that it masks, it clears that key's values in LDS before the product
 // with P, so that 0 times infinity does not reach the rows that do not see the key; in those
 // that do the score counts as NaN.
+//
+// As in tree attention the weights, with their lift of 2^6, are rounded to fp16 for the matrix
+// product with V (2^-11 of a weight; sums and O are fp32).  Error of o against 64 bits, fp16 rows:
+// 2.1e-4 to 2.5e-4 of o's size, of which 2.1e-4 are the rounding of o itself.
+//
+// Past 256 row groups there are no cells, the runs are equal shares of the line, and past 256
+// requests or sets too the division works in global memory: 128 requests of 9 drafted tokens,
+// 64 heads, 8192 shared positions (576 row groups) 1196 us, 1.11 PFLOP/s, tree attention 1252; 300
+// requests of one token 380 and 550.
 #include "mla_tree_kernel.h"
 
 namespace mi355dsa {

@@ -154,14 +154,16 @@ struct W4Ring {
 // NT is large where there are many, and the workgroups begin their runs at different blocks
 // (x's rows, 12 KB apart, would ask the same L2 channels; 1 us of 20).
 //
-// us with memory cold, [24576 x 6144] and [6144 x 24576], groups of 128: 1 row 16.5 and 17.9
-// (5.0 TB/s), 16 rows 18.1 and 20.5, 32 rows 21.2 and 23.3, 64 rows 29.2 and 31.0, the latter
-// ones with the join of S > 1 (2 to 4 us); groups of 32 at the first 20, 24, 27, 39.  Few rows
-// are bound by memory; two blocks on their way leave room for a second workgroup on a CU, with
-// three 17.9, 19.0 and (groups of 32) 26, 25.  64 rows: without the
-// loads 27, without x alone 29 of the then 33, without the unpacking 29: a wave alone on its
-// SIMD is bound by the instructions that it issues, so codes are unpacked in
-// as few as there are.  Not better: x shared by pairs of waves (31 and 35), two waves on a
+// us a call of a graph, weights (80 MB with scales) not in the caches, [24576 x 6144] and
+// [6144 x 24576], fp16, groups of 128: 1 row 17.6 and 18.4 (4.6 and 4.4 TB/s), 16 rows 19.0 and
+// 21.6, 32 rows 22.3 and 24.5, 64 rows 31.0 and 32.5, the latter ones with the join of S > 1
+// (2 to 4 us); groups of 32 at the first 21, 25, 28, 40.  bf16 at the first 17.6, 19.2, 23.2, 33.0,
+// groups of 32 22, 25, 30, 46.  Weights that the last-level cache holds: 1 row 16.0 at the second, 64
+// rows 27.4 at the first.  Few rows are bound by memory; two blocks on their way leave room for a
+// second workgroup on a CU (three: 1.4 and 0.9 us more at 1 and 16 rows, with groups of 32 6
+// and 1).  64 rows, of the then 33 us: without the loads 27, without x alone 29, without the
+// unpacking 29: a wave alone on its SIMD is bound by the instructions that it issues, so codes
+// are unpacked in as few as there are.  Not better: x shared by pairs of waves (31 and 35), two waves on a
 // SIMD, vector instructions spread between the MFMAs by hand (30).
 template <bool BF16, int MT, int XI, int NT, int GPB>
 __global__ void __launch_bounds__(64 * (XI == 1 ? 8 : 4)) w4_linear_kernel(W4Params p) {
@@ -386,9 +388,13 @@ __global__ void __launch_bounds__(256) w4_join_kernel(W4Params p, int MT, int un
 // workgroups of a CU one after the other, each its blocks at the time that a block of NT tiles was
 // measured to take (us, at sizes that fill the chip), and the join (4 us with its launch).  Up
 // to 4 rows that time is the memory's, shared by the CUs, and three quarters of it with few
-// of them at work.  Slices pay where N alone leaves CUs idle: 64 rows at [6144 x 24576] 46 us
-// with two, 31 with four and the join; one row there 18 without, 21 with four; at
-// [24576 x 6144] one is best (64 rows 29, with two 37).
+// of them at work.  From 5 rows on, workgroups past 256 count as a round of their own, although
+// up to 16 rows the LDS lets two or three share a CU: one CU's share of memory and L2 does not
+// grow by it (264 workgroups of one tile at [4224 x 6144], 16 rows, 11.4 us, 132 of two 9.0).  Of all
+// plans of 1, 2, 4 and 8 slices at N of 2112 to 24576, K of 6144 and 24576 and 8, 16, 32 and 64 rows the
+// rule takes the fastest, or one within 2 % (to 16 rows) and 7 %.  Slices pay where N alone leaves CUs
+// idle: 64 rows at [6144 x 24576] 81 us with one, 48 with two, 34 with four and the join, 39
+// with eight; at [24576 x 6144] one is best (64 rows 31, with two 38).
 struct W4Plan {
   int nt, s;
 };

@@ -46,7 +46,10 @@ def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     same cache rows, which are read through the block-table row of the first one that has a
     token.  A group may be one request, and share nothing; positions that a drafted token
     takes, or that the shortest request of a group lacks, do not count as shared (requests
-    without a token, which cu_seqlens_q may have, are not looked at).
+    without a token, which cu_seqlens_q may have, are not looked at).  So an ended request of
+    length 0 that stays in its group with a token ends the sharing, though not the results: 32
+    answers over 32768 positions 166 us, with one ended 235, or 171 where cu_shared puts it
+    into a group of its own.
 
     q [T, H, 576] fp16 (q_latent form).  Without cu_seqlens_q: one token a request, T of them,
     token r at position seq_lens[r] - 1, which sees everything up to itself.  With

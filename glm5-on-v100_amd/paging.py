@@ -153,7 +153,8 @@ def shared_lengths(block_table: torch.Tensor, seq_lens: torch.Tensor, cu_shared:
     """int32 [groups]: the leading positions that the requests of each group hold in the
     same pages (group g: requests cu_shared[g] .. cu_shared[g + 1] - 1, int32
     [groups + 1]) -- whole pages, at most the shortest of their lengths.  0 for a group
-    of no request, the length of one that is alone."""
+    of no request, or with one of length 0 (an ended answer, a padded row: to be given a
+    group of its own); the length of one that is alone."""
     _check(cu_shared.dim() == 1 and cu_shared.size(0) >= 1, "cu_shared must be int32 [groups + 1]")
     out = torch.empty(cu_shared.size(0) - 1, dtype=torch.int32, device=block_table.device)
     run = ops.op("shared_lengths") if _traced(block_table) else _shared_lengths

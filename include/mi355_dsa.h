@@ -181,7 +181,9 @@ int mi355_dsa_mla_tree_attention(void* o, float* lse, const void* q, int64_t n_t
  * no set are left as they were.  max_blocks * page_size < 2^23.  A shared
  * position counts as it is, an own one whose cache row holds an infinity or NaN
  * does not touch the rows that do not see it (those that do may get NaN for it).
- * It has no counterpart in the reference.
+ * A request of length 0 that has a token ends the sharing of its set.  The
+ * workspace has room for two partial results of every workgroup: 34 MB for up to
+ * 32 rows, 134 MB for more than 96.  It has no counterpart in the reference.
  */
 size_t mi355_dsa_mla_prefix_workspace_size(int64_t n_tok, int n_head, int n_req, int n_set);
 int mi355_dsa_mla_prefix_attention(void* o, float* lse, const void* q, int64_t n_tok, int n_head,
@@ -596,13 +598,14 @@ int mi355_dsa_attn_fp8_quantize(uint8_t* q, float* s, const void* w, int N, int 
  * 16 (n / 16) + c, columns 128 (k / 128) + 32 i + 8 g .. +7, bits 4 e .. +3 the
  * column 2 e (e < 4) or 2 e - 7 of them.  sz: for each tile its 128 / group
  * groups, 16 words each: the row's scale in the low half, 16 + z as a dtype
- * number in the high half.  Rows past N have any code and a scale of any
+ * number in the high half (also where every z is 8).  Rows past N have any code and a scale of any
  * finite value.
  */
 
 /* y [M, N] (contiguous) = x [M, K] (rows x_stride elements apart, 16-byte
  * aligned) times the transposed weights, M <= 64, K < 2^24: fp32 sums of
- * unrounded weights, rounded once.  The workspace (16-byte aligned) carries
+ * unrounded weights, rounded once.  bf16: the difference of two sums of terms of
+ * up to 31 |x| a group; an infinity of x makes its row NaN.  The workspace (16-byte aligned) carries
  * nothing between calls; 0 bytes means none. */
 size_t mi355_dsa_w4_linear_workspace_size(int M, int N, int K);
 int mi355_dsa_w4_linear(void* y, const void* x, int64_t x_stride, const int32_t* q,
